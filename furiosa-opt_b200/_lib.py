@@ -55,6 +55,12 @@ class Epilogue(C.Structure):
                 ("residual", C.c_void_p)]
 
 
+class PagedCacheDesc(C.Structure):
+    """`fopt_paged_cache`: the four images of a paged 4-bit key / value cache and their shape."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pages", C.c_int32), ("page_size", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
 # (name, restype, argtypes) for every symbol the header declares.
 _VP, _I32, _I64, _SZ, _CP = C.c_void_p, C.c_int32, C.c_int64, C.c_size_t, C.c_char_p
 SIGNATURES = [
@@ -118,6 +124,13 @@ SIGNATURES = [
     ("fopt_contraction", _I32, [_VP, _VP, C.c_int, _VP, _VP, C.c_int, _VP, _VP, _VP, _VP, C.POINTER(Epilogue)]),
     ("fopt_contraction_host", _I32, [_VP, _VP, C.c_int, _VP, _VP, C.c_int, _VP, _VP, _VP, _VP, C.POINTER(Epilogue)]),
     ("fopt_attention", _I32, [_VP, _VP, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _I32, C.c_float, _I32, C.c_float]),
+    ("fopt_rope_create", _I32, [C.POINTER(C.c_double), _I32, C.c_int, C.c_double, C.POINTER(_VP)]),
+    ("fopt_rope_free", _I32, [_VP]),
+    ("fopt_rotary", _I32, [_VP, _VP, _VP, C.c_int, _VP, _VP, _I32, _I32, _I32, _I64, _I64]),
+    ("fopt_cache_append", _I32, [_VP, C.POINTER(PagedCacheDesc), _VP, _VP, C.c_int, _I64, _I64, _VP, _VP, _VP, _I32]),
+    ("fopt_cache_read", _I32, [_VP, _VP, _VP, C.c_int, C.POINTER(PagedCacheDesc), _VP, _I32]),
+    ("fopt_cache_attention", _I32, [_VP, _VP, _VP, C.POINTER(PagedCacheDesc), _VP, _VP, _VP, _I32, _I32, _I32, _I32,
+                                    C.c_float, _I32]),
     ("fopt_comm_unique_id", _I32, [_VP]),
     ("fopt_comm_init", _I32, [_VP, _I32, _I32, _VP]),
     ("fopt_comm_destroy", _I32, [_VP]),

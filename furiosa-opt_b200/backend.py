@@ -369,6 +369,13 @@ class B200:
     def sync(self):
         check(_lib.lib().fopt_sync(self.ctx), self.ctx)
 
+    def set_stream(self, handle: Optional[int]) -> None:
+        """Runs the following calls on another CUDA stream of the device (a cudaStream_t as an integer; 0
+        is the legacy default stream); None goes back to the backend's own stream. Ordering the streams
+        against each other is the caller's."""
+        # the library takes a null handle as its own stream; 1 is the runtime's name for the legacy one
+        check(_lib.lib().fopt_set_stream(self.ctx, None if handle is None else handle or 1), self.ctx)
+
     def set_exact_fold(self, exact: bool):
         check(_lib.lib().fopt_set_exact_fold(self.ctx, int(exact)), self.ctx)
         self._exact_fold = bool(exact)
@@ -685,6 +692,103 @@ class B200:
         check(_lib.lib().fopt_attention(self.ctx, o.ptr, q.ptr, k.ptr, v.ptr, batch, seq, hq, hkv, head_dim,
                                         C.c_float(sc), int(causal), C.c_float(eps)), self.ctx)
         return o
+
+    # ---- rotary positions and the paged 4-bit cache (see kvcache.py) ----
+    @staticmethod
+    def _rows(name: str, s: Storage, tokens: int, width: int, offset: int, stride: Optional[int]):
+        """(address, token stride) of `tokens` rows of `width` elements within a storage."""
+        stride = width if stride is None else stride
+        if offset < 0 or stride < width:
+            raise ValueError(f"{name}: rows of {width} elements at offset {offset}, stride {stride}")
+        if tokens and offset + (tokens - 1) * stride + width > s.n:
+            raise ValueError(f"{name}: {tokens} rows of {width} elements exceed the storage's {s.n}")
+        return s.addr + offset * dtypes.BITS[s.dtype] // 8, stride
+
+    @staticmethod
+    def _indices(name: str, s: Storage, n: Optional[int] = None) -> int:
+        if s.dtype != "i32" or (n is not None and s.n != n):
+            raise ValueError(f"{name} must be i32" + (f" with {n} entries" if n is not None else ""))
+        return s.n
+
+    def rotary(self, x: Storage, positions: Storage, rope, heads: int, head_dim: int = 128,
+               out: Optional[Storage] = None, x_offset: int = 0, x_stride: Optional[int] = None) -> Storage:
+        """Rotates the heads of each token by its position: x holds rows of `heads` x `head_dim` bf16 or
+        f32 values (`x_stride` elements apart, from `x_offset` on), positions one i32 a row. The result is
+        [tokens, heads, head_dim], in `out` if given; with `out` x itself, the rows are rotated in place."""
+        tokens = self._indices("rotary: positions", positions)
+        if x.dtype not in ("bf16", "f32"):
+            raise ValueError("rotary: bf16 or f32 values")
+        row = heads * head_dim
+        src, stride = self._rows("rotary", x, tokens, row, x_offset, x_stride)
+        if out is None:
+            out = Storage(self, x.dtype, tokens * row, zero=False)
+        elif out.dtype != x.dtype or (out is not x and out.n != tokens * row):
+            raise ValueError("rotary: the output is [tokens, heads, head_dim] of the input's type")
+        out._will_write()
+        dst, dst_stride = (src, stride) if out is x else (out.addr, row)
+        check(_lib.lib().fopt_rotary(self.ctx, dst, src, _lib.DTYPES[x.dtype], positions.ptr, rope.handle, tokens,
+                                     heads, head_dim, stride, dst_stride), self.ctx)
+        return out
+
+    def cache_append(self, cache, k: Storage, v: Storage, slots: Storage, positions: Optional[Storage] = None,
+                     rope=None, k_offset: int = 0, k_stride: Optional[int] = None, v_offset: int = 0,
+                     v_stride: Optional[int] = None) -> None:
+        """Stores each token's keys (rotated by its position first when `rope` is given) and values, bf16
+        or f32 rows of [cache.heads, cache.head_dim], at its slot (page * page_size + slot of the page;
+        negative: no token). Two tokens of one call must not name one slot."""
+        tokens = self._indices("cache_append: slots", slots)
+        if rope is not None:
+            if positions is None:
+                raise ValueError("cache_append: a rotation needs positions")
+            self._indices("cache_append: positions", positions, tokens)
+        if k.dtype != v.dtype or k.dtype not in ("bf16", "f32"):
+            raise ValueError("cache_append: bf16 or f32 keys and values")
+        row = cache.heads * cache.head_dim
+        kp, ks = self._rows("cache_append: keys", k, tokens, row, k_offset, k_stride)
+        vp, vs = self._rows("cache_append: values", v, tokens, row, v_offset, v_stride)
+        cache._will_write()
+        check(_lib.lib().fopt_cache_append(self.ctx, C.byref(cache.desc()), kp, vp, _lib.DTYPES[k.dtype], ks, vs,
+                                           slots.ptr, positions.ptr if rope is not None else None,
+                                           rope.handle if rope is not None else None, tokens), self.ctx)
+
+    def cache_read(self, cache, slots: Storage, dtype: str = "bf16", out=None):
+        """The keys and values stored at the slots, as two [slots, heads, head_dim] storages of `dtype`
+        (or those of the pair `out`); rows of negative slots are left as they were (0 in new storages)."""
+        n = self._indices("cache_read: slots", slots)
+        size = n * cache.heads * cache.head_dim
+        k, v = out if out is not None else (Storage(self, dtype, size), Storage(self, dtype, size))
+        if k.dtype != v.dtype or k.dtype not in ("bf16", "f32") or k.n != size or v.n != size:
+            raise ValueError("cache_read: two bf16 or f32 outputs of [slots, heads, head_dim]")
+        k._will_write()
+        v._will_write()
+        check(_lib.lib().fopt_cache_read(self.ctx, k.ptr, v.ptr, _lib.DTYPES[k.dtype], C.byref(cache.desc()),
+                                         slots.ptr, n), self.ctx)
+        return k, v
+
+    def cache_attention(self, q: Storage, cache, table: Storage, q_start: Storage, kv_len: Storage, heads: int,
+                        scale: Optional[float] = None, causal: bool = True, out: Optional[Storage] = None) -> Storage:
+        """softmax(scale q K^T) V over the cache, for sequences of any lengths in one call: sequence b has
+        the bf16 query rows q_start[b] .. q_start[b + 1] - 1 ([heads, head_dim] each) and kv_len[b] keys in
+        the pages of its row of `table`. Causal: its queries are its last tokens. Rows behind the last
+        sequence are left as they were (0 in a new output)."""
+        batch = self._indices("cache_attention: kv_len", kv_len)
+        self._indices("cache_attention: q_start", q_start, batch + 1)
+        entries = self._indices("cache_attention: table", table)
+        row = heads * cache.head_dim
+        if q.dtype != "bf16" or row <= 0 or q.n % row:
+            raise ValueError("cache_attention: bf16 queries of [tokens, heads, head_dim]")
+        if not batch or entries % batch:
+            raise ValueError("cache_attention: the table has a row of equal length for each sequence")
+        if out is None:
+            out = Storage(self, "bf16", q.n)
+        elif out.dtype != "bf16" or out.n != q.n or out is q:
+            raise ValueError("cache_attention: the output is another storage laid out as q")
+        out._will_write()
+        sc = scale if scale is not None else cache.head_dim ** -0.5
+        check(_lib.lib().fopt_cache_attention(self.ctx, out.ptr, q.ptr, C.byref(cache.desc()), table.ptr, q_start.ptr,
+                                              kv_len.ptr, batch, q.n // row, entries // batch, heads, C.c_float(sc),
+                                              int(causal)), self.ctx)
+        return out
 
     # ---- host transfers (backend/mod.rs:220-238) ----
     def to_hbm(self, host_values, Element: Mapping, dtype: str, Dst: Optional[Mapping] = None) -> Storage:

@@ -113,9 +113,57 @@ struct fopt_graph {
   cudaGraphExec_t exec = nullptr;
   std::unordered_set<void*> owned;  // allocations of the capture that it did not free
   bool launched = false;
+  void* cache_ws = nullptr;         // this graph's own cache-attention workspace
+  size_t cache_ws_bytes = 0;
+  std::vector<void*> outgrown;      // smaller workspaces that earlier calls of the capture recorded
   int64_t kernels = 0;              // kernels the captured step launches (counted per replay)
   int64_t launches_before = 0;
 };
+
+namespace fopt {
+
+// Zeroed device memory that calls on one stream, or the calls of one captured graph, take turns with.
+// Eager calls share a buffer per stream and each graph has its own, so that launches which may overlap
+// (two streams, two graphs, a graph beside eager calls) never share one. Callers leave its counters zero.
+void* cache_workspace(fopt_ctx* ctx, size_t bytes) {
+  auto zeroed = [&](size_t n) {
+    void* p = nullptr;
+    cuda_check(cudaMalloc(&p, n), "cache workspace alloc");
+    // on a stream of its own: the context's may be capturing
+    cudaStream_t s;
+    cuda_check(cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking), "cache workspace stream");
+    cudaError_t e = cudaMemsetAsync(p, 0, n, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    cudaStreamDestroy(s);
+    cuda_check(e, "cache workspace clear");
+    return p;
+  };
+  if (fopt_graph* g = ctx->capture) {
+    if (bytes > g->cache_ws_bytes) {
+      if (g->cache_ws) g->outgrown.push_back(g->cache_ws);
+      g->cache_ws = nullptr;
+      g->cache_ws_bytes = 0;
+      g->cache_ws = zeroed(bytes);
+      g->cache_ws_bytes = bytes;
+    }
+    return g->cache_ws;
+  }
+  auto& ws = ctx->cache_ws[ctx->stream];
+  if (bytes > ws.second) {
+    if (ws.first) cuda_check(cudaFree(ws.first), "cache workspace free");  // waits for its last reader
+    ws = {nullptr, 0};
+    ws.first = zeroed(bytes);
+    ws.second = bytes;
+  }
+  return ws.first;
+}
+
+static void release_graph_ws(fopt_graph* g) {
+  if (g->cache_ws) cudaFree(g->cache_ws);
+  for (void* p : g->outgrown) cudaFree(p);
+}
+
+}  // namespace fopt
 
 extern "C" {
 
@@ -153,6 +201,8 @@ fopt_status fopt_destroy(fopt_ctx* ctx) {
   if (ctx->scratch) cudaFree(ctx->scratch);
   if (ctx->gemm_ws) cudaFree(ctx->gemm_ws);
   if (ctx->gemm_cnt) cudaFree(ctx->gemm_cnt);
+  for (auto& kv : ctx->cache_ws)
+    if (kv.second.first) cudaFree(kv.second.first);
   for (void* p : ctx->retired) cudaFree(p);
   if (ctx->copy_in) cudaStreamDestroy(ctx->copy_in);
   if (ctx->copy_out) cudaStreamDestroy(ctx->copy_out);
@@ -176,6 +226,7 @@ static void check_device_error(fopt_ctx* ctx) {
   cuda_check(cudaMemcpy(&code, ctx->dev_err, sizeof(code), cudaMemcpyDeviceToHost), "error word read");
   if (code) {
     cuda_check(cudaMemset(ctx->dev_err, 0, sizeof(code)), "error word clear");
+    if (code >= kBadIndex) throw Fail{FOPT_ERR_INVALID, bad_index_message(code)};
     ctx->gemm_cnt_dirty = true;
     throw Fail{FOPT_ERR_TIMEOUT, "a kernel's bounded wait expired (code " + std::to_string(code) + ")"};
   }
@@ -295,6 +346,7 @@ fopt_status fopt_capture_end(fopt_ctx* ctx, fopt_graph** out) {
     ctx->deferred_free.clear();
     if (e != cudaSuccess) {
       if (g->graph) cudaGraphDestroy(g->graph);
+      release_graph_ws(g);
       delete g;
       cuda_check(e, "graph capture");
     }
@@ -326,6 +378,7 @@ fopt_status fopt_graph_destroy(fopt_ctx* ctx, fopt_graph* g) {
     cuda_check(cudaStreamSynchronize(ctx->stream), "sync");
     if (g->exec) cudaGraphExecDestroy(g->exec);
     if (g->graph) cudaGraphDestroy(g->graph);
+    release_graph_ws(g);
     delete g;
     if (--ctx->graphs_alive == 0) {
       for (void* p : ctx->retired) cudaFree(p);

@@ -90,6 +90,7 @@ struct fopt_ctx {
   uint32_t* gemm_cnt = nullptr;  // arrival counters of the split tiles (zero between launches)
   size_t gemm_cnt_n = 0;
   bool gemm_cnt_dirty = false;
+  std::map<cudaStream_t, std::pair<void*, size_t>> cache_ws;  // cache-attention workspace of each stream
   cudaStream_t copy_in = nullptr, copy_out = nullptr;  // host <-> device pipelines of the host-buffer calls
   void* pinned[2] = {nullptr, nullptr};  // host staging for file -> device streaming
   cudaEvent_t pinned_ev[2] = {nullptr, nullptr};
@@ -139,6 +140,34 @@ inline void launched(fopt_ctx* ctx, const char* what) {
 }
 
 void* scratch(fopt_ctx* ctx, size_t bytes);
+void* cache_workspace(fopt_ctx* ctx, size_t bytes);
+
+// Codes of the device error word from kBadIndex on report an index in device data that a kernel skipped
+// (FOPT_ERR_INVALID); smaller ones are expired waits.
+constexpr int kBadIndex = 0x1000;
+constexpr int kBadSlot = kBadIndex, kBadPage = kBadIndex + 1, kBadLength = kBadIndex + 2, kBadStart = kBadIndex + 3;
+inline const char* bad_index_message(int code) {
+  switch (code) {
+    case kBadSlot: return "a cache slot past the cache's pages";
+    case kBadPage: return "a page number outside the cache";
+    case kBadLength: return "a sequence length below 0 or past its table's pages";
+    default: return "query starts that do not ascend within the tokens";
+  }
+}
+
+// Makes the context's device current for a call and puts the caller's back.
+struct DeviceGuard {
+  int was = -1;
+  explicit DeviceGuard(const fopt_ctx* ctx) {
+    cuda_check(cudaGetDevice(&was), "cudaGetDevice");
+    if (was == ctx->device) was = -1;
+    else cuda_check(cudaSetDevice(ctx->device), "cudaSetDevice");
+  }
+  ~DeviceGuard() {
+    if (was >= 0) cudaSetDevice(was);
+  }
+  DeviceGuard(const DeviceGuard&) = delete;
+};
 
 KWalk to_kwalk(const Walk& w);
 bool to_kwalk32(const KWalk& w, KWalk32& out);

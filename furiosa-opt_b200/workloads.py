@@ -9,10 +9,12 @@
   -> residual -> RMSNorm -> gate/up -> SwiGLU -> down -> residual. The norm, quantisation and
   activation steps are vector-engine ops (map / zip / reduce / broadcast relayout); the projections
   are contractions with the fused dequant epilogue; attention is the fused kernel. Rotary position
-  embedding is not part of the config and is omitted.
+  embedding is not part of the config: `forward` omits it. `step` is the block as a server runs it, over
+  the new tokens of cached sequences: rotary positions, the paged 4-bit cache and attention over it.
 """
 from __future__ import annotations
 
+import copy
 import os
 
 import numpy as np
@@ -20,6 +22,7 @@ import numpy as np
 from . import dtypes, ops
 from ._lib import FOPT_ERR_UNSUPPORTED, FoptError
 from .backend import B200, Mapping, Storage
+from .kvcache import CacheBatch, PagedCache, Rope
 
 
 # ---------------------------------------------------------------------------------------------
@@ -216,9 +219,18 @@ class DecoderBlockW8A8:
 
     def proj(self, q: Storage, s_tok: Storage, w: Storage, s_w: Storage, k_ax: str, n_ax: str,
              residual: Storage = None) -> Storage:
-        m = self.m
-        return self.be.contraction_dequant(q, w, m(f"[T, {k_ax}]"), m(f"[{n_ax}, {k_ax}]"), m(f"[T, {n_ax}, {k_ax}]"),
-                                           m(f"[T, {n_ax}]"), s_tok, s_w, n_ax, residual=residual)
+        be, m = self.be, self.m
+        maps = (m(f"[T, {k_ax}]"), m(f"[{n_ax}, {k_ax}]"), m(f"[T, {n_ax}, {k_ax}]"), m(f"[T, {n_ax}]"))
+        try:
+            return be.contraction_dequant(q, w, *maps, s_tok, s_w, n_ax, residual=residual)
+        except FoptError as e:
+            if e.status != FOPT_ERR_UNSUPPORTED or residual is not None:
+                raise
+        # token counts off the tensor-core tiles: the integer product, then the epilogue's chain by itself
+        acc = be.contraction_wide(q, w, *maps)
+        rs = be.relayout(s_tok, m("[T]"), maps[3], allow_broadcast=True)
+        cs = be.relayout(s_w, m(f"[{n_ax}]"), maps[3], allow_broadcast=True)
+        return be.zip3_with(acc, rs, cs, _prog_dequant(), "bf16")
 
     def proj_residual(self, q, s_tok, w, s_w, k_ax, n_ax, x):
         """x + proj(...), the residual add in the projection's epilogue when `fuse_residual`."""
@@ -233,13 +245,47 @@ class DecoderBlockW8A8:
 
     def forward(self, x: Storage) -> Storage:
         """x: bf16 [T, H] -> bf16 [T, H]."""
+        return self._block(x, lambda Q, K, V: self.be.attention(Q, K, V, self.batch, self.seq, self.Hq, self.Hkv, 128,
+                                                                causal=True))
+
+    def step(self, x: Storage, cache: PagedCache, batch: CacheBatch, rope: Rope) -> Storage:
+        """The block over the new tokens of a batch of cached sequences (whole prompts, pieces of them or
+        single tokens, mixed): queries and keys rotated by their positions, keys and values appended to
+        the cache, attention over all that it then holds. x: bf16 [T, H], batch.tokens = T rows of which
+        those behind the last sequence are padding (their output means nothing)."""
+        if cache.heads != self.Hkv or cache.head_dim != 128 or batch.tokens != self.T:
+            raise ValueError("step: the cache or the batch is not of this block's shape")
+
+        def attend(Q, K, V):
+            be = self.be
+            be.rotary(Q, batch.positions, rope, self.Hq, out=Q)
+            be.cache_append(cache, K, V, batch.slots, positions=batch.positions, rope=rope)
+            return be.cache_attention(Q, cache, batch.table, batch.q_start, batch.kv_len, self.Hq)
+
+        return self._block(x, attend)
+
+    def with_tokens(self, T: int, batch: int = 1) -> "DecoderBlockW8A8":
+        """The same weights for steps of another number of tokens (T a multiple of batch)."""
+        if T <= 0 or T % batch:
+            raise ValueError("with_tokens: T must be a positive multiple of batch")
+        b = copy.copy(self)
+        b.T, b.batch, b.seq = T, batch, T // batch
+        b.ax = dict(self.ax, T=T)
+        b.__dict__.pop("_mappings", None)
+        b.g1, b.g2 = (b.be.relayout(b.be.from_vec(b.m("[H]"), self.host[g], "f32"), b.m("[H]"), b.m("[T, H]"), True)
+                      for g in ("g1", "g2"))
+        b.fuse_residual = not os.environ.get("FOPT_NO_RESIDUAL_EPILOGUE")
+        b.fuse_swiglu = self.SWIGLU_EPILOGUE and self.F % 128 == 0
+        return b
+
+    def _block(self, x: Storage, attend) -> Storage:
         be = self.be
         xf = be.map(x, ops.cast("bf16", "f32"), "f32")
         q, s = self.quantize(self.rmsnorm(xf, self.g1), "H")
         Q = self.proj(q, s, self.wq, self.sq, "H", "Q")
         K = self.proj(q, s, self.wk, self.sk, "H", "V")
         V = self.proj(q, s, self.wv, self.sv, "H", "V")
-        att = be.attention(Q, K, V, self.batch, self.seq, self.Hq, self.Hkv, 128, causal=True)
+        att = attend(Q, K, V)
         qa, sa = self.quantize(be.map(att, ops.cast("bf16", "f32"), "f32"), "H")
         h1 = self.proj_residual(qa, sa, self.wo, self.so, "H", "Q", x)
         h1f = be.map(h1, ops.cast("bf16", "f32"), "f32")
@@ -309,6 +355,11 @@ class DecoderBlockW8A8TP(DecoderBlockW8A8):
         self.wu, self.su = up("[FL, H]", rows(h["wu"][0], self.F_l), "i8"), up("[FL]", rows(h["wu"][1], self.F_l), "f32")
         self.wo = up("[Q, QL]", cols(h["wo"][0], Ql), "i8")
         self.wd = up("[Q, FL]", cols(h["wd"][0], self.F_l), "i8")
+
+    def step(self, *args, **kw):
+        raise NotImplementedError("step: the cache is not sharded across ranks")
+
+    with_tokens = step
 
     def _amax_across(self, amax: Storage) -> None:
         self.dist.allreduce(self.be, amax, "Max")

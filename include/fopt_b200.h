@@ -363,6 +363,73 @@ fopt_status fopt_attention(fopt_ctx* ctx, void* o, const void* q, const void* k,
                            int32_t seq, int32_t hq, int32_t hkv, int32_t head_dim, float scale, int32_t causal,
                            float eps);
 
+/* ---- rotary positions and the paged 4-bit key / value cache ----
+ * What a decoder needs around attention to answer token by token. The reference's transformer example
+ * rotates and caches on its own tensors per step; here a token's keys are rotated, quantised and
+ * stored in one pass and attention reads the stored form.
+ *
+ * A rotation turns pair p of a head's channels by positions[t] * inv_freq[p] radians and scales it by
+ * `magnitude` (1 unless a long-context scaling asks for more). HALF pairs channel p with p + n_pairs,
+ * INTERLEAVED 2 p with 2 p + 1; channels from 2 * n_pairs on pass through. At most 128 pairs. The angle
+ * is reduced exactly (64-bit fixed-point turns) and its sine and cosine are correct to f32 at any
+ * position, negative ones included. The handle is host memory; calls copy it by value, so it may be
+ * freed while they are in flight and captured graphs keep their own copy. */
+typedef struct fopt_rope fopt_rope;
+typedef enum { FOPT_ROPE_HALF = 0, FOPT_ROPE_INTERLEAVED = 1 } fopt_rope_layout;
+fopt_status fopt_rope_create(const double* inv_freq, int32_t n_pairs, fopt_rope_layout layout, double magnitude,
+                             fopt_rope** out);
+fopt_status fopt_rope_free(fopt_rope* rope);
+/* out[t, h, :] = rotate(x[t, h, :], positions[t]) for bf16 or f32 values; token t's heads start at
+ * x + t * x_stride elements (head-major, head_dim each) and go to out + t * out_stride. Products and
+ * sums are f32, one rounding each, and a bf16 result is rounded once. out may be x itself (the same
+ * pointer and stride); any other overlap is the caller's error. */
+fopt_status fopt_rotary(fopt_ctx* ctx, void* out, const void* x, fopt_dtype dtype, const int32_t* positions,
+                        const fopt_rope* rope, int32_t tokens, int32_t heads, int32_t head_dim, int64_t x_stride,
+                        int64_t out_stride);
+
+/* The cache: `pages` pages of `page_size` slots (a multiple of 16) for `heads` key / value heads of
+ * head_dim 64, 128 or 256 channels D. Mappings of the four 16-byte aligned images (P page, H head, S
+ * slot of the page):
+ *   k        i4    [P, H, S, D % 32 / 8, D / 32, D % 8]
+ *   v        i4    [P, H, S, D % 32 / 4, D / 32, D % 4]
+ *   k_scale, v_scale  bf16  [P, H, S, D / 32, 2]: (step, offset) of each group of 32 channels
+ * A value is code * step + offset. Quantising a group x: step = bf16((max - min) / 15), offset =
+ * bf16(min + 8 step), code = round-half-even((x - offset) / step) clipped to [-8, 7], in f32, and code
+ * 0 where step is 0. What a 4-bit code cannot say is stored as the nearest that it can: NaN as 0, and
+ * magnitudes above 2^100 (infinities) as 2^100, so every stored value is finite. */
+typedef struct fopt_paged_cache {
+  void* k;
+  void* v;
+  void* k_scale;
+  void* v_scale;
+  int32_t pages, page_size, heads, head_dim;
+} fopt_paged_cache;
+/* Token t's keys k[t, H, D] (rotated by positions[t] first when rope is given) and values v[t, H, D]
+ * (bf16 or f32, token strides in elements) go to slot slots[t] = page * page_size + slot of the page. A
+ * negative slot is no token: nothing is stored for it. A slot past the cache is skipped and reported
+ * as FOPT_ERR_INVALID by the next fopt_sync / fopt_d2h. Two tokens of one call must not name one slot. */
+fopt_status fopt_cache_append(fopt_ctx* ctx, const fopt_paged_cache* cache, const void* k, const void* v,
+                              fopt_dtype dtype, int64_t k_stride, int64_t v_stride, const int32_t* slots,
+                              const int32_t* positions, const fopt_rope* rope, int32_t tokens);
+/* The inverse move: out_k / out_v [n, H, D] (bf16 or f32) receive the values stored at the n slots;
+ * rows of negative slots are left as they were. */
+fopt_status fopt_cache_read(fopt_ctx* ctx, void* out_k, void* out_v, fopt_dtype dtype, const fopt_paged_cache* cache,
+                            const int32_t* slots, int32_t n);
+/* softmax(scale q K^T) V over the cache for `batch` sequences of any lengths in one call. Sequence b has
+ * the query tokens q_start[b] .. q_start[b + 1] - 1 of q [tokens, hq, D] (bf16; q_start has batch + 1
+ * entries) and the kv_len[b] keys whose key i lies in page table[b * table_width + i / page_size], slot i %
+ * page_size. Causal: the queries are the sequence's last tokens, so query j of n sees keys 0 ..
+ * kv_len[b] - n + j; otherwise every query sees all kv_len[b]. Query head h reads key head h / (hq / H).
+ * o [tokens, hq, D] bf16: a row that sees no key is 0; rows of tokens past q_start[batch] are left
+ * as they were. Scores, maxima, sums and the output accumulate in f32. Reads nothing but the keys in
+ * range: table entries and cache slots past kv_len may hold anything. A page number outside the cache
+ * (its keys count as zeros), a length past table_width pages (cut) or a q_start that is not ascending
+ * within 0 .. tokens (clamped) is reported as FOPT_ERR_INVALID by the next fopt_sync / fopt_d2h. All
+ * lengths are device data, so a captured call replays over growing sequences. */
+fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* q, const fopt_paged_cache* cache,
+                                 const int32_t* table, const int32_t* q_start, const int32_t* kv_len, int32_t batch,
+                                 int32_t tokens, int32_t table_width, int32_t hq, float scale, int32_t causal);
+
 /* ---- collectives over the Chip axis (memory.rs:657-679, 1186-1233; context.rs:164-235) ---- */
 /* NCCL unique id (128 bytes) for rank 0 to broadcast through the host plumbing. */
 fopt_status fopt_comm_unique_id(void* id128);

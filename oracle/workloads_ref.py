@@ -69,9 +69,10 @@ def _round_half_away(y: np.ndarray) -> np.ndarray:
 
 
 def decoder_ref(x_bits: np.ndarray, host: dict, T, H, Hq, Hkv, F, batch, seq, eps=1e-5,
-                att_override=None) -> np.ndarray:
+                att_override=None, attend=None) -> np.ndarray:
     """The W8A8 block. `att_override` (bf16 bits [T, H]) replaces the attention output, so that the
-    rest of the chain can be compared on the attention values a kernel produced."""
+    rest of the chain can be compared on the attention values a kernel produced; `attend` computes it
+    from the projections' bf16 bits (Q, K, V)."""
     KV = Hkv * 128
 
     def rmsnorm(x, g, width):
@@ -96,7 +97,9 @@ def decoder_ref(x_bits: np.ndarray, host: dict, T, H, Hq, Hkv, F, batch, seq, ep
     x = _f32(x_bits).reshape(T, H)
     q, s = quant(rmsnorm(x, host["g1"], H))
     Q, K, V = proj(q, s, "wq"), proj(q, s, "wk"), proj(q, s, "wv")
-    if att_override is None:
+    if attend is not None:
+        att = np.asarray(attend(Q, K, V), np.uint16).reshape(-1)
+    elif att_override is None:
         att = attention(Q.reshape(-1), K.reshape(-1), V.reshape(-1), batch, seq, Hq, Hkv, 128, 128 ** -0.5, True)
     else:
         att = np.asarray(att_override, np.uint16).reshape(-1)
