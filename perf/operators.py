@@ -286,9 +286,10 @@ def run(state):
 # the framework's operators
 # ---------------------------------------------------------------------------------------------
 class _Memory:
-    """A storage's device memory for torch (no copy)."""
+    """A storage's device memory for torch (no copy; a tensor over it keeps the storage)."""
 
     def __init__(self, storage, shape, kind):
+        self.storage = storage
         self.__cuda_array_interface__ = {"shape": shape, "typestr": kind, "data": (storage.addr, False), "version": 3}
 
 
@@ -330,6 +331,7 @@ def _hold(s, case):
     if case["op"] == "attention":
         h["q"] = _copied(fb, be, s["q"], "bf16")
         h["out"] = fb.Storage(be, "bf16", s["q"].numel())
+        h["seen"] = _tensor(h["out"], tuple(s["q"].shape))
         for name in ("table", "q_start", "kv_len"):
             h[name] = _copied(fb, be, s[name], "i32")
     else:
@@ -338,6 +340,7 @@ def _hold(s, case):
         if case["op"] == "rotary":
             h["row"] = _copied(fb, be, s["row"], case["dtype"])
             h["out"] = fb.Storage(be, case["dtype"], s["x"].numel())
+            h["seen"] = _tensor(h["out"], tuple(s["x"].shape))
         else:
             for name in ("k", "v"):
                 h[name] = _copied(fb, be, s[name], case["dtype"])
@@ -345,6 +348,7 @@ def _hold(s, case):
             slots = case["pages"] * case["page"]
             h["all"] = _copied(fb, be, torch.arange(slots, device="cuda", dtype=torch.int32), "i32")
             h["out"] = [fb.Storage(be, "bf16", slots * case["heads"] * case["dim"]) for _ in range(2)]
+            h["seen"] = {n: _tensor(o, (slots, case["heads"], case["dim"])) for n, o in zip("kv", h["out"])}
     if case["op"] != "rotary":
         pages = s["cache"]["k"].shape[0]
         h["cache"] = fb.PagedCache(be, pages, case["page"], case["heads"], case["dim"])
@@ -358,15 +362,13 @@ def _own(s, case):
     if case["op"] == "rotary":
         be.rotary(h["row"], h["positions"], h["rope"], case["heads"], case["dim"], out=h["out"],
                   x_offset=case["extra"], x_stride=case["heads"] * case["dim"] + case["extra"])
-        return _tensor(h["out"], tuple(s["x"].shape))
-    if case["op"] == "append":
+    elif case["op"] == "append":
         be.cache_append(h["cache"], h["k"], h["v"], h["slots"], positions=h["positions"], rope=h["rope"])
-        k, v = be.cache_read(h["cache"], h["all"], out=h["out"])
-        shape = (case["pages"] * case["page"], case["heads"], case["dim"])
-        return {"k": _tensor(k, shape), "v": _tensor(v, shape)}
-    be.cache_attention(h["q"], h["cache"], h["table"], h["q_start"], h["kv_len"], case["heads"] * case["group"],
-                       causal=case["causal"], out=h["out"])
-    return _tensor(h["out"], tuple(s["q"].shape))
+        be.cache_read(h["cache"], h["all"], out=h["out"])
+    else:
+        be.cache_attention(h["q"], h["cache"], h["table"], h["q_start"], h["kv_len"], case["heads"] * case["group"],
+                           causal=case["causal"], out=h["out"])
+    return h["seen"]
 
 
 # ---------------------------------------------------------------------------------------------
