@@ -79,6 +79,10 @@ class Cache:
     def values(self, n):
         return values(self.codes[n], self.step[n], self.offset[n])
 
+    def parts(self, n):
+        """|code * step| + |offset|: the size of what sums to a value, which may cancel in it."""
+        return values(np.abs(self.codes[n]), self.step[n], np.abs(self.offset[n]))
+
     def image(self, n):
         """The codes in the order of the cache's image (flat)."""
         w = 8 if n == "k" else 4
@@ -90,18 +94,19 @@ class Cache:
 
 
 def attention(q, cache, table, q_start, kv_len, scale, causal=True):
-    """q f32 [T, Hq, D]; table [B, W]. Returns (o, a): the output in f64 and sum_i p_i |v_i| of every output
-    element (what roundings of the probabilities are measured by). Rows of no sequence are NaN."""
+    """q f32 [T, Hq, D]; table [B, W]. Returns (o, a): the output in f64 and, for every output element,
+    sum_i p_i (|code_i step_i| + |offset_i|), which a rounding of probabilities is relative to: the products
+    may run on codes and offsets apart. Rows of no sequence are NaN."""
     T, Hq, D = q.shape
     group = Hq // cache.heads
     o, a = np.full((T, Hq, D), np.nan), np.zeros((T, Hq, D))
-    K, V = cache.values("k"), cache.values("v")
+    K, V, A = cache.values("k"), cache.values("v"), cache.parts("v")
     for b, n in enumerate(kv_len):
         q0, q1 = q_start[b], q_start[b + 1]
         pages = np.asarray(table[b][:-(-int(n) // cache.page_size)], np.int64)
         for h in range(cache.heads):
             k = K[pages, h].reshape(-1, D)[:n]
-            v = V[pages, h].reshape(-1, D)[:n]
+            v, va = V[pages, h].reshape(-1, D)[:n], A[pages, h].reshape(-1, D)[:n]
             for t in range(q0, q1):
                 seen = max(0, n - (q1 - q0) + (t - q0) + 1) if causal else n
                 rows = slice(h * group, (h + 1) * group)
@@ -113,5 +118,5 @@ def attention(q, cache, table, q_start, kv_len, scale, causal=True):
                     p = np.exp(x - x.max(-1, keepdims=True))
                     p /= p.sum(-1, keepdims=True)
                     o[t, rows] = p @ v[:seen]
-                    a[t, rows] = p @ np.abs(v[:seen])
+                    a[t, rows] = p @ va[:seen]
     return o, a
