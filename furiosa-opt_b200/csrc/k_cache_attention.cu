@@ -13,18 +13,21 @@
 // bytes; the instructions of the expansion (about one per code) come next.
 //   * K operand: lane (g, i) = (lane / 4, lane % 4) takes the 16-byte (D = 128) run of token g that the
 //     layout [D % 32 / 8, D / 32, D % 8] puts at i: word j is 8 channels of group j, which make its operand
-//     registers of two k16 steps; q's fragments are permuted to match. (x & 0x00f000f0) ^ 0x64806480 is
-//     f16 1024 + 16 (code + 8): with q / 16 that is q (code + 72), and the sum starts from -72 sum(q).
+//     registers of two k16 steps; q's fragments are permuted to match. (x & 0x000f000f) ^ 0x00080008 is a
+//     pair of f16 subnormals (code + 8) 2^-24, and (x & 0x00f000f0) ^ 0x00800080 of (code + 8) 2^-20: one
+//     instruction a pair and nothing to subtract, with the powers of two in q's fragments and the 8 in the
+//     group's offset (offset - 8 step).
 //   * V operand (channels as rows, tokens as k): lane (g, i) takes the channels 4 g .. 4 g + 3 of every
-//     group for four tokens; byte permutes pair two tokens' channels, and the codes become exact f16.
-//   * probabilities go from the scores' fragment to the V product's by movmatrix.
+//     group for four tokens; byte permutes pair two tokens' channels.
+//   * probabilities go from the scores' fragment to the V product's by movmatrix, as p step in f16: half a
+//     step of it is 2^-11, an eighth of the output's own rounding. p offset is summed in f32.
 //   * the maximum moves only when a score exceeds it by 2^8 (a warp vote), so the rescaling is rare. Steps of V
 //     are scaled by a power of two that follows them the same way, which keeps p step within f16 at any
 //     magnitude of V.
-// Eight warps take 16 tokens each of a 128-token tile, with their own rings of cp.async stages (no block
-// barrier while keys stream), and merge their (maximum, sum, output) at the end of a segment.
+// Four warps take a run of 16-token tiles each, with their own rings of cp.async stages (no block barrier
+// while keys stream), and merge their (maximum, sum, output) at the end of a segment.
 //
-// Work: all (sequence, row block, key head) of the call, in 128-token tiles, form one line that is cut
+// Work: all (sequence, row block, key head) of the call, in 64-token tiles, form one line that is cut
 // into equal shares, one per resident block, from the lengths on the device: no host knowledge of them, no idle
 // blocks, any mixture of lengths. A segment cut between blocks leaves partial results in a workspace; the
 // last of its blocks to arrive adds them up in order, so results do not depend on timing.
@@ -34,10 +37,13 @@ namespace fopt {
 namespace kv {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTileTokens = 16 * kWarps;
+constexpr int kBlocks = 3;       // resident blocks an SM, where the registers allow (168 a thread)
+constexpr int kSegmentCost = 4;  // beginning and ending a segment takes about as long as this many tiles
 constexpr int kStages = 4;
+constexpr float kNone = -0x1p120f;  // the maximum of a part that has no score; its sum is 0
 constexpr float kLazy = 8.0f;  // log2 by which a score may exceed the running maximum before it moves
 
 struct AttnArgs {
@@ -59,7 +65,8 @@ struct AttnArgs {
 struct Seq {
   int q0, rows;   // first query token; query rows per key head (tokens x group)
   int queries, keys;
-  int tiles;      // 128-token tiles, one at least: a sequence without keys still writes its rows
+  int tiles;      // kTileTokens-token tiles, one at least: a sequence without keys still writes its rows
+  int units;      // of work in one segment (the row block of a key head): its tiles and kSegmentCost
 };
 
 // Sequence b's query range and key count, cut to what the arguments allow.
@@ -72,24 +79,39 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
   s.rows = s.queries * a.group;
   s.keys = (int)min((int64_t)max(n, 0), (int64_t)a.width * a.cache.page_size);
   s.tiles = max(1, (s.keys + kTileTokens - 1) / kTileTokens);
+  s.units = s.tiles + kSegmentCost;
   if (s.q0 != s0 || q1 != s1) atomicExch(a.err, kBadStart);
   if (s.keys != n) atomicExch(a.err, kBadLength);
   return s;
 }
 template <int R>
 __device__ __forceinline__ long long units(const AttnArgs& a, const Seq& s) {
-  return (long long)((s.rows + R - 1) / R) * a.cache.heads * s.tiles;
+  return (long long)((s.rows + R - 1) / R) * a.cache.heads * s.units;
 }
-// Of `total` units on `n` <= total blocks, block c has [first(c), first(c + 1)).
-__device__ __forceinline__ long long first_unit(long long total, int n, int c) { return total * c / n; }
-__device__ __forceinline__ int owner(long long total, int n, long long unit) {
-  return (int)(((unit + 1) * n - 1) / total);
+__device__ __forceinline__ long long quotient(long long a, long long b) {  // both >= 0; a 64-bit division takes long
+  return ((a | b) >> 32) ? a / b : (long long)((uint32_t)a / (uint32_t)b);
 }
+// Of `total` units on n <= total blocks, the first total % n blocks have one more than the others.
+struct Shares {
+  long long each;
+  int more;
+  __device__ __forceinline__ Shares(long long total, int n) : each(quotient(total, n)), more((int)(total - each * n)) {}
+  __device__ __forceinline__ long long first(int c) const { return each * c + min(c, more); }
+  __device__ __forceinline__ int owner(long long unit) const {
+    const long long wide = (each + 1) * more;
+    return unit < wide ? (int)quotient(unit, each + 1) : more + (int)quotient(unit - wide, each);
+  }
+};
 
 // ---- small pieces ----
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {  // bytes 0: zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// A value that the compiler keeps in its register instead of computing it again from the lane number.
+__device__ __forceinline__ int kept(int x) {
+  asm volatile("" : "+r"(x));
+  return x;
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -99,6 +121,31 @@ __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same from zero sums (no registers to clear).
+__device__ __forceinline__ void mma0(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+template <bool FROM_ZERO>
+__device__ __forceinline__ void mma_bf16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (FROM_ZERO)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
@@ -117,19 +164,19 @@ __device__ __forceinline__ float exp2_(float x) {
 }
 __device__ __forceinline__ float step_of(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float offset_of(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-// Two codes (nibbles at bits 4-7 and 20-23) as f16 pairs 1024 + 16 (code + 8).
-__device__ __forceinline__ uint32_t codes_high(uint32_t x) { return (x & 0x00f000f0u) ^ 0x64806480u; }
-// ... as exact f16 codes, from bits 4-7 / 20-23 and from bits 0-3 / 16-19.
-__device__ __forceinline__ uint32_t exact_high(uint32_t x) {
+// Two codes as f16 subnormals: (code + 8) 2^-24 from bits 0-3 and 16-19, (code + 8) 2^-20 from bits 4-7 and 20-23.
+// One lop3 each ((x & mask) ^ constant), the masks in registers: with both constants immediate it takes two
+// instructions (64 more a tile, a quarter of the ALU's work).
+struct Masks {
+  uint32_t low, high;
+};
+__device__ __forceinline__ uint32_t masked(uint32_t x, uint32_t mask, uint32_t flip) {
   uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(codes_high(x)), "r"(0x2c002c00u), "r"(0xd480d480u));  // / 16 - 72
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(x), "r"(mask), "r"(flip));
   return r;
 }
-__device__ __forceinline__ uint32_t exact_low(uint32_t x) {
-  uint32_t r;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((x & 0x000f000fu) ^ 0x64086408u), "r"(0xe408e408u));  // - 1032
-  return r;
-}
+__device__ __forceinline__ uint32_t codes_low(const Masks& m, uint32_t x) { return masked(x, m.low, 0x00080008u); }
+__device__ __forceinline__ uint32_t codes_high(const Masks& m, uint32_t x) { return masked(x, m.high, 0x00800080u); }
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t* w, const uint8_t* p) {
   if constexpr (N == 1) w[0] = *(const uint32_t*)p;
@@ -156,6 +203,7 @@ template <int NG, int NB>
 struct Shared {
   static constexpr int D = NG * kGroup, R = 8 * NB;
   static constexpr int kCodes = 16 * D / 2, kScales = 16 * NG * 4;      // one tile's K or V
+  static constexpr int kScaleLanes = 2 * kScales / 16;                 // lanes that copy both's scales, 16 bytes each
   static constexpr int kStage = 2 * (kCodes + kScales);
   static constexpr int kRing = kStages * kStage;
   static constexpr int kRow = D + 4;                                    // floats; the pad spreads rows over banks
@@ -174,18 +222,24 @@ __device__ __forceinline__ int v_chunk(int token, int chunk) {
 // A warp's state over a segment's keys.
 template <int NG, int NB>
 struct State {
-  float o[NB][NG][2][4];   // [channel 32 j + 4 g + 2 mm (+ 1 for c2, c3)] x [row 2 i, 2 i + 1], in 2^ev
-  float e[NB][NG][2];      // sum of p offset, this lane's tokens
+  // [channel 32 j + 4 g + 2 mm (+ 1 for c2, c3)] x [row 2 i, 2 i + 1]: sum of p step (code + 8), in 2^(ev + 24)
+  // for the even channels (c0, c1) and 2^(ev + 20) for the odd ones
+  float o[NB][NG][2][4];
+  float e[NB][NG][2];      // sum of p (offset - 8 step), this lane's tokens
   float m[NB][2], l[NB][2];
   float vscale;            // 2^-ev
-  uint32_t vlimit;         // bf16 bits of the largest step that p step 2^-ev still holds
+  float vlimit;            // the largest step that p step 2^-ev still holds
 };
 
 template <int NG, int NB>
 struct Query {
-  uint32_t f[NB][2 * NG][2];  // fragments of q 2^(8 - e) / 16
-  float sum[NB][NG][2];       // sums of q 2^(8 - e) over a group, of the lane's rows 2 i and 2 i + 1
-  float scale[NB][2];         // 2^(e - 8) scale log2(e)
+  uint32_t f[NB][2 * NG][2];  // fragments of q 2^(8 - e), times 16 where codes_low() meets them
+  // Fragments that turn a token's scale words, as they are, into sum_groups (offset - 8 step) (sum of q): k runs
+  // over (group, step / offset) of groups 0 .. 3, then (NG = 8) of groups 4 .. 7. The sums are 2^(8 - e - 20) that
+  // of the q in f, split into three bf16 parts, 24 bits together.
+  static constexpr int kLimbs = NG == 8 ? 6 : 3;
+  uint32_t z[NB][kLimbs];
+  float scale[NB][2];         // 2^(e + 12) scale log2(e)
   int limit[NB][2];           // keys that the row sees
 };
 
@@ -213,7 +267,7 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, const Seq& s, int 
     int ex = top > 0.0f ? min(ilogbf(top), 127) : 0;
     // 2^(8 - ex) may pass the f32 range: two factors
     const float up0 = scalbnf(1.0f, (8 - ex) / 2), up1 = scalbnf(1.0f, 8 - ex - (8 - ex) / 2);
-    const float down = scalbnf(a.scale * 1.44269504088896340736f, ex - 8);
+    const float down = scalbnf(a.scale * 1.44269504088896340736f, ex + 12);
     float sum[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
@@ -222,26 +276,39 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, const Seq& s, int 
       sum[j] = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        v[e] = (e & 1 ? offset_of(x[e >> 1]) : step_of(x[e >> 1])) * up0 * up1 * 0.0625f;
+        v[e] = (e & 1 ? offset_of(x[e >> 1]) : step_of(x[e >> 1])) * up0 * up1;
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t h = f16x2(v[e], v[e + 4]);  // the pairs that codes_high() makes of a word
+        // the pairs that codes_low() and codes_high() make of a word
+        const float by = e & 1 ? 1.0f : 16.0f;
+        const uint32_t h = f16x2(v[e] * by, v[e + 4] * by);
         q.f[nb][2 * j + (e >> 1)][e & 1] = h;
         // the sum of what the products take
         float lo, hi;
         asm("{.reg .f16 a, b; mov.b32 {a, b}, %2; cvt.f32.f16 %0, a; cvt.f32.f16 %1, b;}" : "=f"(lo), "=f"(hi) : "r"(h));
-        sum[j] += lo + hi;
+        sum[j] += (lo + hi) / by;
       }
       sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
       sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
+    }
+#pragma unroll
+    for (int h = 0; h < (NG == 8 ? 2 : 1); ++h) {
+      float rest = 0.0f;  // the sum of group 4 h + i
+#pragma unroll
+      for (int j = 0; j < NG; ++j)
+        if (j == 4 * h + i) rest = sum[j] * 0x1p-20f;
+#pragma unroll
+      for (int n = 0; n < 3; ++n) {
+        const float part = __uint_as_float(f32_to_bf16w(__float_as_uint(rest)));
+        rest -= part;
+        q.z[nb][h * 3 + n] = __float_as_uint(-8.0f * part) >> 16 | __float_as_uint(part);
+      }
     }
     // the lane's rows as columns of the scores: 2 i and 2 i + 1, held by the lanes of g = 2 i, 2 i + 1
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int from = 4 * (2 * i + c);
-#pragma unroll
-      for (int j = 0; j < NG; ++j) q.sum[nb][j][c] = 16.0f * __shfl_sync(0xffffffffu, sum[j], from);
       q.scale[nb][c] = __shfl_sync(0xffffffffu, down, from);
       const int rc = row0 + nb * 8 + 2 * i + c;
       // columns past the rows hold q = 0 and no one reads them: they need no mask of their own
@@ -250,47 +317,76 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, const Seq& s, int 
   }
 }
 
+// Where in a stage a lane reads: bytes from the start of its K codes, scales (either's) and V codes.
+struct Places {
+  int k, k_word, scale, v;
+  Masks masks;
+};
+template <int NG>
+__device__ __forceinline__ Places places() {
+  constexpr int D = NG * kGroup;
+  const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3, at = g * NG * 2;
+  return {kept(g * (D / 2) + i * NG * 4), kept(g * NG * 4 + i * 4), kept(g * NG * 4),
+          kept(2 * i * (D / 2) + v_chunk<NG>(2 * i, at >> 4) * 16 + (at & 15)),
+          {(uint32_t)kept(0x000f000f), (uint32_t)kept(0x00f000f0)}};
+}
+
 // One tile of 16 tokens, from its stage; token0 is its first.
 template <int NG, int NB>
-__device__ __forceinline__ void tile(const uint8_t* stage, int token0, int keys, int sure, const Query<NG, NB>& q,
-                                     State<NG, NB>& s) {
+__device__ __forceinline__ void tile(const uint8_t* stage, const Places& at, int token0, int keys, int sure, bool first,
+                                     const Query<NG, NB>& q,                                     State<NG, NB>& s) {
   using S = Shared<NG, NB>;
   const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
   uint32_t kw[2][NG], km[2][NG];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    load_words<NG>(kw[h], stage + (g + 8 * h) * (S::D / 2) + i * NG * 4);
-    load_words<NG>(km[h], stage + 2 * S::kCodes + (g + 8 * h) * NG * 4);
+    load_words<NG>(kw[h], stage + at.k + 8 * h * (S::D / 2));
+    load_words<NG>(km[h], stage + 2 * S::kCodes + at.scale + 8 * h * NG * 4);
   }
   float x[NB][4];
+  {
+    uint32_t w[2][2] = {};  // scale words of tokens g and g + 8, groups i and i + 4
+    const uint8_t* sc = stage + 2 * S::kCodes + at.k_word;
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) x[nb][0] = x[nb][1] = x[nb][2] = x[nb][3] = 0.0f;
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-  for (int j = 0; j < NG; ++j) {
-    uint32_t h0[4], h1[4];
-    h0[0] = codes_high(kw[0][j] << 4), h0[1] = codes_high(kw[0][j]), h0[2] = codes_high(kw[0][j] >> 4), h0[3] = codes_high(kw[0][j] >> 8);
-    h1[0] = codes_high(kw[1][j] << 4), h1[1] = codes_high(kw[1][j]), h1[2] = codes_high(kw[1][j] >> 4), h1[3] = codes_high(kw[1][j] >> 8);
-    const float s0 = step_of(km[0][j]), s1 = step_of(km[1][j]), z0 = offset_of(km[0][j]), z1 = offset_of(km[1][j]);
+      for (int n = 0; n < (NG == 8 ? 2 : 1); ++n)
+        if (NG >= 4 || i < NG) w[h][n] = *(const uint32_t*)(sc + 8 * h * NG * 4 + n * 16);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const float a0 = -72.0f * q.sum[nb][j][0], a1 = -72.0f * q.sum[nb][j][1];
-      float acc[4] = {a0, a1, a0, a1};
-      mma(acc, h0[0], h1[0], h0[1], h1[1], q.f[nb][2 * j][0], q.f[nb][2 * j][1]);
-      mma(acc, h0[2], h1[2], h0[3], h1[3], q.f[nb][2 * j + 1][0], q.f[nb][2 * j + 1][1]);
+      if constexpr (NG == 8) {
+        mma_bf16<true>(x[nb], w[0][0], w[1][0], w[0][1], w[1][1], q.z[nb][0], q.z[nb][3]);
+        mma_bf16<false>(x[nb], w[0][0], w[1][0], w[0][1], w[1][1], q.z[nb][1], q.z[nb][4]);
+        mma_bf16<false>(x[nb], w[0][0], w[1][0], w[0][1], w[1][1], q.z[nb][2], q.z[nb][5]);
+      } else {
+        mma_bf16<true>(x[nb], w[0][0], w[1][0], w[0][0], w[1][0], q.z[nb][0], q.z[nb][1]);
+        mma_bf16<false>(x[nb], w[0][0], w[1][0], 0u, 0u, q.z[nb][2], 0u);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    const uint32_t x0 = kw[0][j], x1 = kw[1][j], y0 = x0 >> 8, y1 = x1 >> 8;
+    const float s0 = step_of(km[0][j]), s1 = step_of(km[1][j]);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float acc[4];
+      mma0(acc, codes_low(at.masks, x0), codes_low(at.masks, x1), codes_high(at.masks, x0), codes_high(at.masks, x1), q.f[nb][2 * j][0], q.f[nb][2 * j][1]);
+      mma(acc, codes_low(at.masks, y0), codes_low(at.masks, y1), codes_high(at.masks, y0), codes_high(at.masks, y1), q.f[nb][2 * j + 1][0], q.f[nb][2 * j + 1][1]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        x[nb][c] = fmaf(s0, acc[c], fmaf(z0, q.sum[nb][j][c], x[nb][c]));
-        x[nb][c + 2] = fmaf(s1, acc[c + 2], fmaf(z1, q.sum[nb][j][c], x[nb][c + 2]));
+        x[nb][c] = fmaf(s0, acc[c], x[nb][c]);
+        x[nb][c + 2] = fmaf(s1, acc[c + 2], x[nb][c + 2]);
       }
     }
   }
   uint32_t vm[2][NG];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) load_words<NG>(vm[h], stage + 2 * S::kCodes + S::kScales + (g + 8 * h) * NG * 4);
+  for (int h = 0; h < 2; ++h) load_words<NG>(vm[h], stage + 2 * S::kCodes + S::kScales + at.scale + 8 * h * NG * 4);
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) x[nb][c] *= q.scale[nb][c & 1];
+    for (int c = 0; c < 4; ++c) x[nb][c] = fmaf(x[nb][c], q.scale[nb][c & 1], -s.m[nb][c & 1]);
   if (token0 + 16 > sure) {  // some row does not see all of it
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -307,33 +403,36 @@ __device__ __forceinline__ void tile(const uint8_t* stage, int token0, int keys,
     }
   }
   // does the maximum, or the power of two of the steps, have to move?
-  uint32_t steps = 0;
+  float step[2][NG], steps = 0.0f, tops = x[0][0];
 #pragma unroll
-  for (int j = 0; j < NG; ++j) steps = __vmaxu2(steps, __vmaxu2(vm[0][j], vm[1][j]));
-  bool move = (steps & 0xffffu) > s.vlimit;
+  for (int j = 0; j < NG; ++j) {
+    step[0][j] = step_of(vm[0][j]);
+    step[1][j] = step_of(vm[1][j]);
+    steps = max3(steps, step[0][j], step[1][j]);
+  }
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
+  for (int nb = 0; nb < NB; ++nb) tops = max3(max3(tops, x[nb][0], x[nb][1]), x[nb][2], x[nb][3]);
+  if (__any_sync(0xffffffffu, first || tops > kLazy || steps > s.vlimit)) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) move |= x[nb][c] > s.m[nb][c & 1] + kLazy;
-  if (__any_sync(0xffffffffu, move)) {
-    uint32_t top = steps & 0x7fffu;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = 1; o < 32; o <<= 1) steps = fmaxf(steps, __shfl_xor_sync(0xffffffffu, steps, o));
     float by = 1.0f;
-    if (top > s.vlimit) {  // the largest step to [2^4, 2^5), and room up to 2^7: p <= 2^8 keeps 2^15
-      const int ev = (int)(top >> 7) - 127 - 4;
-      const float vscale = scalbnf(1.0f, min(-ev, 126));
+    if (steps > s.vlimit) {  // the largest step to [2^4, 2^5), and room up to 2^7: p <= 2^8 keeps 2^15
+      const float vscale = scalbnf(1.0f, min(4 - ilogbf(steps), 126));
       by = s.vscale > 0.0f ? vscale / s.vscale : 0.0f;
       s.vscale = vscale;
-      s.vlimit = min(top + (2u << 7), 0x7f7fu);
+      s.vlimit = fminf(0x1p7f / vscale, 0x1.fep127f);
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float was = s.m[nb][c], now = fmaxf(was, max_over_g(fmaxf(x[nb][c], x[nb][c + 2])));
-        const float f = now == -INFINITY ? 1.0f : exp2_(was - now);
-        s.m[nb][c] = now;
+        // the base moves up by the largest score over it; the first tile's scores set it
+        const float top_score = max_over_g(fmaxf(x[nb][c], x[nb][c + 2]));
+        const float up = first ? (top_score == -INFINITY ? 0.0f : top_score) : fmaxf(0.0f, top_score);
+        const float f = first ? 0.0f : exp2_(-up);
+        s.m[nb][c] += up;
+        x[nb][c] -= up;
+        x[nb][c + 2] -= up;
         s.l[nb][c] *= f;
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
@@ -350,32 +449,32 @@ __device__ __forceinline__ void tile(const uint8_t* stage, int token0, int keys,
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const float m = s.m[nb][c & 1];
-      x[nb][c] = exp2_(x[nb][c] - (m == -INFINITY ? 0.0f : m));
+      x[nb][c] = exp2_(x[nb][c]);
       s.l[nb][c & 1] += x[nb][c];
     }
+  float y[NB][4];  // p 2^-ev
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) y[nb][c] = x[nb][c] * s.vscale;
   // V: words of tokens 2 i, 2 i + 1, 2 i + 8, 2 i + 9
   uint32_t vw[4][NG / 2];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int token = 2 * i + (t & 1) + 8 * (t >> 1), at = g * NG * 2;  // byte of the row
-    load_words<NG / 2>(vw[t], stage + S::kCodes + token * (S::D / 2) + v_chunk<NG>(token, at >> 4) * 16 + (at & 15));
-  }
+  for (int t = 0; t < 4; ++t)  // (2 i + 1) / 2 and (2 i + 8) / 2 mod 4 are i: the chunk is the same
+    load_words<NG / 2>(vw[t], stage + S::kCodes + at.v + ((t & 1) + 8 * (t >> 1)) * (S::D / 2));
 #pragma unroll
   for (int j = 0; j < NG; ++j) {
     const uint32_t sel = j & 1 ? 0x7632u : 0x5410u;
     const uint32_t x01 = __byte_perm(vw[0][j >> 1], vw[1][j >> 1], sel), x23 = __byte_perm(vw[2][j >> 1], vw[3][j >> 1], sel);
     const uint32_t y01 = x01 >> 8, y23 = x23 >> 8;
-    const uint32_t c0 = exact_low(x01), c1 = exact_high(x01), c2 = exact_low(x23), c3 = exact_high(x23);
-    const uint32_t d0 = exact_low(y01), d1 = exact_high(y01), d2 = exact_low(y23), d3 = exact_high(y23);
-    const float s0 = step_of(vm[0][j]) * s.vscale, s1 = step_of(vm[1][j]) * s.vscale;
-    const float z0 = offset_of(vm[0][j]), z1 = offset_of(vm[1][j]);
+    const float s0 = step[0][j], s1 = step[1][j];
+    const float z0 = fmaf(-8.0f, s0, offset_of(vm[0][j])), z1 = fmaf(-8.0f, s1, offset_of(vm[1][j]));
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const uint32_t b0 = transposed(f16x2(x[nb][0] * s0, x[nb][1] * s0));
-      const uint32_t b1 = transposed(f16x2(x[nb][2] * s1, x[nb][3] * s1));
-      mma(s.o[nb][j][0], c0, c1, c2, c3, b0, b1);
-      mma(s.o[nb][j][1], d0, d1, d2, d3, b0, b1);
+      const uint32_t b0 = transposed(f16x2(y[nb][0] * s0, y[nb][1] * s0));
+      const uint32_t b1 = transposed(f16x2(y[nb][2] * s1, y[nb][3] * s1));
+      mma(s.o[nb][j][0], codes_low(at.masks, x01), codes_high(at.masks, x01), codes_low(at.masks, x23), codes_high(at.masks, x23), b0, b1);
+      mma(s.o[nb][j][1], codes_low(at.masks, y01), codes_high(at.masks, y01), codes_low(at.masks, y23), codes_high(at.masks, y23), b0, b1);
 #pragma unroll
       for (int c = 0; c < 2; ++c) s.e[nb][j][c] = fmaf(x[nb][c], z0, fmaf(x[nb][c + 2], z1, s.e[nb][j][c]));
     }
@@ -394,7 +493,7 @@ struct Partial {
 };
 
 template <int NG, int NB>
-__global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? 2 : 1) tokens_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <= 4 ? 2 : 1) tokens_kernel(AttnArgs a) {
   using S = Shared<NG, NB>;
   using P = Partial<NG, NB>;
   constexpr int D = S::D, R = S::R;
@@ -420,8 +519,9 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? 2 : 1) tokens_k
   if (total == 0) return;
   const int blocks = (int)min((long long)gridDim.x, total);
   if (blockIdx.x >= blocks) return;
-  long long unit = first_unit(total, blocks, blockIdx.x);
-  const long long end = first_unit(total, blocks, blockIdx.x + 1);
+  const Shares shares(total, blocks);
+  long long unit = shares.first(blockIdx.x);
+  const long long end = shares.first(blockIdx.x + 1);
   long long before = 0;  // units of the sequences before the chunk
   for (int b0 = 0;; b0 += kThreads) {
     const int b = b0 + tid;
@@ -452,19 +552,34 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? 2 : 1) tokens_k
   long long seq_at = found_at;
   Seq s = sequence(a, b);
 
+  const Places at = places<NG>();
   uint8_t* ring = smem + warp * S::kRing;
-  const uint32_t ring_u32 = smem_u32(ring);
+  const uint32_t ring_u32 = smem_u32(ring) + lane * 16;
+  // what a lane copies of a tile, from where and to where: chunks lane, lane + 32, ... of K and of V, and with
+  // one half of the lanes K's scales, with the other V's
+  constexpr int kHalf = S::kScaleLanes < 32 ? S::kScaleLanes / 2 : 16;
+  const uint8_t* k_lane = a.cache.k + lane * 16;
+  const uint8_t* v_lane = a.cache.v + lane * 16;
+  const uint8_t* scale_lane =
+      lane < kHalf ? (const uint8_t*)a.cache.k_scale + lane * 16 : (const uint8_t*)a.cache.v_scale + (lane - kHalf) * 16;
+  // relative to lane * 16, where the lane's K codes go; a second V chunk is 8 (D = 128: 32 chunks on, the same
+  // place in its row) or 4 (D = 256) tokens on
+  const int scale_to = kept(2 * S::kCodes + (lane < kHalf ? 0 : S::kScales - kHalf * 16));
+  const int v_to0 = kept(S::kCodes + (v_chunk<NG>(lane / NG, lane % NG) - lane % NG) * 16);
+  const int v_to1 = NG == 8 ? kept(S::kCodes + (v_chunk<NG>(lane / NG + 4, lane % NG) - lane % NG) * 16) : v_to0;
   while (unit < end) {
     while (unit >= seq_at + units<R>(a, s)) {
       seq_at += units<R>(a, s);
       s = sequence(a, ++b);
     }
-    const int seg = (int)((unit - seq_at) / s.tiles);
-    const int t0 = (int)(unit - seq_at - (long long)seg * s.tiles);
-    const int t1 = (int)min((long long)s.tiles, t0 + (end - unit));
+    const int seg = (int)quotient(unit - seq_at, s.units);
+    const long long seg_at = seq_at + (long long)seg * s.units;
+    // its cost stands before its first tile; a share that ends within it has no tile here
+    const int u1 = (int)min((long long)s.units, end - seg_at);
+    const int t0 = max(0, (int)(unit - seg_at) - kSegmentCost), t1 = u1 - kSegmentCost;
     const int head = seg % a.cache.heads, row0 = seg / a.cache.heads * R;
-    const long long seg_at = unit - t0;
-    unit += t1 - t0;
+    unit = seg_at + u1;
+    if (t1 <= t0) continue;
 
     Query<NG, NB> q;
     load_query<NG, NB>(a, s, head, row0, q);
@@ -475,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? 2 : 1) tokens_k
     State<NG, NB> st;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      st.m[nb][0] = st.m[nb][1] = -INFINITY;
+      st.m[nb][0] = st.m[nb][1] = 0.0f;
       st.l[nb][0] = st.l[nb][1] = 0.0f;
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
@@ -485,56 +600,70 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? 2 : 1) tokens_k
       }
     }
     st.vscale = 0.0f;
-    st.vlimit = 0;
+    st.vlimit = 0.0f;
 
+    // this warp's run of the segment's 16-token tiles, and where in which page it begins
+    const int tiles16 = max(0, (min(t1 * kTileTokens, most) - t0 * kTileTokens + 15) / 16);
+    int n = t0 * kWarps + tiles16 * warp / kWarps;
+    const int n1 = t0 * kWarps + tiles16 * (warp + 1) / kWarps;
     const int32_t* table = a.table + (int64_t)b * a.width;
-    auto page_of = [&](int t) -> int {
-      const int token = t * kTileTokens + warp * 16;
-      return t < t1 && token < most ? table[fdiv(a.cache.by_page, (uint32_t)token)] : 0;
+    int page_at = (int)fdiv(a.cache.by_page, (uint32_t)n * 16);  // entry of the table that `page` is
+    int in_page = n * 16 - page_at * a.cache.page_size;
+    int page = n < n1 ? table[page_at] : 0;
+    int fetched = n;
+    const uint8_t *k, *v, *sc;
+    bool there;
+    auto enter = [&] {  // the page's rows from in_page on
+      there = page >= 0 && page < a.cache.pages;
+      if (!there && lane == 0) atomicExch(a.err, kBadPage);
+      const int64_t row = there ? ((int64_t)page * a.cache.heads + head) * a.cache.page_size + in_page : 0;
+      k = k_lane + row * (D / 2);
+      v = v_lane + row * (D / 2);
+      sc = scale_lane + row * (NG * 4);
+      ++page_at;
+      page = (int64_t)page_at * a.cache.page_size < n1 * 16 ? table[page_at] : 0;  // for the next time
     };
-    auto fetch = [&](int t, int page, int stage) {
-      const int token = t * kTileTokens + warp * 16;
-      if (t < t1 && token < most) {
-        const bool there = page >= 0 && page < a.cache.pages;
-        if (!there && lane == 0) atomicExch(a.err, kBadPage);
-        const uint32_t bytes = there ? 16 : 0;
-        const int in_page = token - (int)fdiv(a.cache.by_page, (uint32_t)token) * a.cache.page_size;
-        const int64_t row = there ? ((int64_t)page * a.cache.heads + head) * a.cache.page_size + in_page : 0;
-        const uint8_t* k = a.cache.k + row * (D / 2);
-        const uint8_t* v = a.cache.v + row * (D / 2);
-        const uint32_t to = ring_u32 + stage * S::kStage;
-#pragma unroll
-        for (int c = lane; c < S::kCodes / 16; c += 32) {
-          copy16(to + c * 16, k + c * 16, bytes);
-          const int tok = c / NG, chunk = c % NG;
-          copy16(to + S::kCodes + (tok * NG + v_chunk<NG>(tok, chunk)) * 16, v + c * 16, bytes);
+    if (n < n1) enter();
+    uint32_t into = 0, from = 0;  // stages, in bytes
+    auto fetch = [&] {
+      if (fetched < n1) {
+        if (in_page == a.cache.page_size) {
+          in_page = 0;
+          enter();
         }
-        const uint8_t* ks = (const uint8_t*)(a.cache.k_scale + row * NG);
-        const uint8_t* vs = (const uint8_t*)(a.cache.v_scale + row * NG);
+        const uint32_t to = ring_u32 + into;
+        if (there) {
 #pragma unroll
-        for (int c = lane; c < 2 * (S::kScales / 16); c += 32)
-          copy16(to + 2 * S::kCodes + c * 16, c < S::kScales / 16 ? ks + c * 16 : vs + (c - S::kScales / 16) * 16, bytes);
+          for (int c = 0; c * 32 < S::kCodes / 16; ++c) copy16(to + c * 512, k + c * 512);
+#pragma unroll
+          for (int c = 0; c * 32 < S::kCodes / 16; ++c) copy16(to + (c & 1 ? v_to1 : v_to0) + c * 512, v + c * 512);
+#pragma unroll
+          for (int c = 0; c * 32 < S::kScaleLanes; ++c)
+            if (lane < S::kScaleLanes) copy16(to + scale_to + c * 256, sc + c * 256);
+        } else {
+          for (int c = lane; c < S::kStage / 16; c += 32) *(uint4*)(ring + into + c * 16) = make_uint4(0, 0, 0, 0);
+        }
+        k += S::kCodes;
+        v += S::kCodes;
+        sc += S::kScales;
+        in_page += 16;
+        ++fetched;
       }
       copies_commit();
+      into = into + S::kStage == S::kRing ? 0 : into + S::kStage;
     };
-    int page = page_of(t0);
-#pragma unroll
-    for (int n = 0; n < kStages - 1; ++n) {
-      const int next = page_of(t0 + n + 1);
-      fetch(t0 + n, page, n);
-      page = next;
-    }
-    int stage = 0;
-    for (int t = t0; t < t1; ++t) {
-      const int next = page_of(t + kStages);
-      fetch(t + kStages - 1, page, stage ? stage - 1 : kStages - 1);
-      page = next;
+#pragma unroll 1
+    for (int c = 0; c < kStages - 1; ++c) fetch();
+    bool first = true;
+#pragma unroll 1
+    for (; n < n1; ++n) {
+      fetch();
       copies_wait<kStages - 1>();
       __syncwarp();
-      const int token = t * kTileTokens + warp * 16;
-      if (token < most) tile<NG, NB>(ring + stage * S::kStage, token, s.keys, sure, q, st);
+      tile<NG, NB>(ring + from, at, n * 16, s.keys, sure, first, q, st);
+      first = false;
       __syncwarp();  // all lanes have read the stage before the next copies into it
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      from = from + S::kStage == S::kRing ? 0 : from + S::kStage;
     }
     copies_wait<0>();
     __syncthreads();  // every warp's ring is drained: the outputs go over them
@@ -548,15 +677,15 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? 2 : 1) tokens_k
         const int r = nb * 8 + 2 * i + c;
         const float l = sum_over_g(st.l[nb][c]);
         if (g == 0) {
-          ml[0][warp][r] = st.m[nb][c];
+          ml[0][warp][r] = l > 0.0f ? st.m[nb][c] : kNone;
           ml[1][warp][r] = l;
         }
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
           const float e = sum_over_g(st.e[nb][j][c]);
           *(float4*)(out + r * S::kRow + j * kGroup + 4 * g) =
-              make_float4(fmaf(st.o[nb][j][0][c], back, e), fmaf(st.o[nb][j][0][c + 2], back, e),
-                          fmaf(st.o[nb][j][1][c], back, e), fmaf(st.o[nb][j][1][c + 2], back, e));
+              make_float4(fmaf(st.o[nb][j][0][c] * 0x1p24f, back, e), fmaf(st.o[nb][j][0][c + 2] * 0x1p20f, back, e),
+                          fmaf(st.o[nb][j][1][c] * 0x1p24f, back, e), fmaf(st.o[nb][j][1][c + 2] * 0x1p20f, back, e));
         }
       }
     __syncthreads();
@@ -572,13 +701,13 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? 2 : 1) tokens_k
     float* part = P::slot(a.ws, blockIdx.x, t0 == 0);
     for (int k = tid; k < rows * (D / 4); k += kThreads) {
       const int r = k / (D / 4), d = k % (D / 4) * 4;
-      float m = -INFINITY, l = 0.0f;
+      float m = kNone, l = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[0][w][r]);
       float4 sum = make_float4(0, 0, 0, 0);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2_(ml[0][w][r] - (m == -INFINITY ? 0.0f : m));
+        const float f = exp2_(ml[0][w][r] - m);
         const float4 v = *(const float4*)((const float*)smem + (w * R + r) * S::kRow + d);
         l = fmaf(f, ml[1][w][r], l);
         sum.x = fmaf(f, v.x, sum.x), sum.y = fmaf(f, v.y, sum.y), sum.z = fmaf(f, v.z, sum.z), sum.w = fmaf(f, v.w, sum.w);
@@ -594,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? 2 : 1) tokens_k
       }
     }
     if (!whole) {
-      const int c0 = owner(total, blocks, seg_at), c1 = owner(total, blocks, seg_at + s.tiles - 1);
+      const int c0 = shares.owner(seg_at + kSegmentCost), c1 = shares.owner(seg_at + s.units - 1);
       __threadfence();
       __syncthreads();
       if (tid == 0) {
@@ -606,13 +735,13 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? 2 : 1) tokens_k
       if (last) {
         for (int k = tid; k < rows * (D / 4); k += kThreads) {
           const int r = k / (D / 4), d = k % (D / 4) * 4;
-          float m = -INFINITY, l = 0.0f;
+          float m = kNone, l = 0.0f;
           for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(P::slot(a.ws, c, c == c0) + R * D + r));
           float4 sum = make_float4(0, 0, 0, 0);
 #pragma unroll 4
           for (int c = c0; c <= c1; ++c) {
             const float* p = P::slot(a.ws, c, c == c0);
-            const float f = exp2_(__ldcg(p + R * D + r) - (m == -INFINITY ? 0.0f : m));
+            const float f = exp2_(__ldcg(p + R * D + r) - m);
             const float4 v = __ldcg((const float4*)(p + r * D + d));
             l = fmaf(f, __ldcg(p + R * D + R + r), l);
             sum.x = fmaf(f, v.x, sum.x), sum.y = fmaf(f, v.y, sum.y), sum.z = fmaf(f, v.z, sum.z), sum.w = fmaf(f, v.w, sum.w);
@@ -628,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? 2 : 1) tokens_k
 template <int NG, int NB>
 void launch_tokens(fopt_ctx* ctx, AttnArgs a, int sms) {
   using S = Shared<NG, NB>;
-  const int grid = sms * (NG <= 4 && NB == 1 ? 2 : 1);
+  const int grid = sms * (NG <= 4 && NB == 1 ? kBlocks : NG <= 4 ? 2 : 1);
   cuda_check(cudaFuncSetAttribute(tokens_kernel<NG, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes),
              "cache attention shared memory");
   const size_t partials = (size_t)grid * 2 * Partial<NG, NB>::kFloats * sizeof(float);

@@ -80,8 +80,9 @@ class Cache:
         return values(self.codes[n], self.step[n], self.offset[n])
 
     def parts(self, n):
-        """|code * step| + |offset|: the size of what sums to a value, which may cancel in it."""
-        return values(np.abs(self.codes[n]), self.step[n], np.abs(self.offset[n]))
+        """(code + 8) step + |offset - 8 step|: the size of what sums to a value, which may cancel in it."""
+        c, st, of = (a[n].astype(np.float64) for a in (self.codes, self.step, self.offset))
+        return values(c + 8, st, np.abs(of - 8 * st))
 
     def image(self, n):
         """The codes in the order of the cache's image (flat)."""
@@ -95,8 +96,8 @@ class Cache:
 
 def attention(q, cache, table, q_start, kv_len, scale, causal=True):
     """q f32 [T, Hq, D]; table [B, W]. Returns (o, a): the output in f64 and, for every output element,
-    sum_i p_i (|code_i step_i| + |offset_i|), which a rounding of probabilities is relative to: the products
-    may run on codes and offsets apart. Rows of no sequence are NaN."""
+    sum_i p_i ((code_i + 8) step_i + |offset_i - 8 step_i|), which a rounding of probabilities is relative to:
+    the products may run on codes from 0 to 15 and offsets apart. Rows of no sequence are NaN."""
     T, Hq, D = q.shape
     group = Hq // cache.heads
     o, a = np.full((T, Hq, D), np.nan), np.zeros((T, Hq, D))

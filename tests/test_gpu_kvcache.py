@@ -6,11 +6,12 @@ Tolerances, from the roundings alone (half a step of bf16 is 2^-8 of the value, 
     sum: |error| <= (|a| + |b|) m 2^-22 for a pair (a, b) scaled by m; a bf16 result adds 2^-8 |y|;
   * stored codes, steps and offsets: none, every step of the rule is one IEEE operation;
   * attention: each probability carries the f32 error of its score and at most one rounding to 11 bits
-    or more before it multiplies a value's code: with v = code step + offset the two products are rounded
-    apart, sum (p (1 + d)) code step + p offset with |d| <= 2^-11, so the error is relative to w = sum p
-    (|code step| + |offset|), which exceeds sum p |v| where the parts cancel: (2^-10 + 2 s) w with s = 2^-19
-    scale sum |q| |k| + 2^-18 (scores sum D products whose codes may be offset by 72, nine times a code's own
-    size, in f32; the exponential is good to 2^-21), and the output rounds to bf16: 2^-8 |o|."""
+    or more before it multiplies a value's code. A value is (code + 8) step + (offset - 8 step), and the two
+    products may be rounded apart: sum (p (1 + d)) (code + 8) step + p (offset - 8 step), |d| <= 2^-11. The error
+    is then relative to w = sum p ((code + 8) step + |offset - 8 step|), which exceeds sum p |v| where the parts
+    cancel: (2^-10 + 2 s) w with s = 2^-19 scale sum |q| max |k| + 2^-18 (a score's f32 sums, of parts up to
+    (15 + 8) / 8 as large as a code's own; the exponential is good to 2^-21); the output rounds to
+    bf16: 2^-8 |o|."""
 import ctypes as C
 
 import numpy as np
