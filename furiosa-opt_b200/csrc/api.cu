@@ -135,7 +135,9 @@ void* cache_workspace(fopt_ctx* ctx, size_t bytes) {
     cudaError_t e = cudaMemsetAsync(p, 0, n, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     cudaStreamDestroy(s);
+    if (e != cudaSuccess) cudaFree(p);
     cuda_check(e, "cache workspace clear");
+    ctx->cache_ws_live[p] = n;
     return p;
   };
   if (fopt_graph* g = ctx->capture) {
@@ -150,17 +152,22 @@ void* cache_workspace(fopt_ctx* ctx, size_t bytes) {
   }
   auto& ws = ctx->cache_ws[ctx->stream];
   if (bytes > ws.second) {
-    if (ws.first) cuda_check(cudaFree(ws.first), "cache workspace free");  // waits for its last reader
+    void* old = ws.first;
     ws = {nullptr, 0};
+    ctx->cache_ws_live.erase(old);
+    if (old) cuda_check(cudaFree(old), "cache workspace free");  // waits for its last reader
     ws.first = zeroed(bytes);
     ws.second = bytes;
   }
   return ws.first;
 }
 
-static void release_graph_ws(fopt_graph* g) {
-  if (g->cache_ws) cudaFree(g->cache_ws);
-  for (void* p : g->outgrown) cudaFree(p);
+static void release_graph_ws(fopt_ctx* ctx, fopt_graph* g) {
+  if (g->cache_ws) g->outgrown.push_back(g->cache_ws);
+  for (void* p : g->outgrown) {
+    ctx->cache_ws_live.erase(p);
+    cudaFree(p);
+  }
 }
 
 }  // namespace fopt
@@ -228,6 +235,8 @@ static void check_device_error(fopt_ctx* ctx) {
     cuda_check(cudaMemset(ctx->dev_err, 0, sizeof(code)), "error word clear");
     if (code >= kBadIndex) throw Fail{FOPT_ERR_INVALID, bad_index_message(code)};
     ctx->gemm_cnt_dirty = true;
+    // a kernel that gave up may have left arrivals behind
+    for (auto& ws : ctx->cache_ws_live) cuda_check(cudaMemset(ws.first, 0, ws.second), "cache workspace clear");
     throw Fail{FOPT_ERR_TIMEOUT, "a kernel's bounded wait expired (code " + std::to_string(code) + ")"};
   }
 }
@@ -346,7 +355,7 @@ fopt_status fopt_capture_end(fopt_ctx* ctx, fopt_graph** out) {
     ctx->deferred_free.clear();
     if (e != cudaSuccess) {
       if (g->graph) cudaGraphDestroy(g->graph);
-      release_graph_ws(g);
+      release_graph_ws(ctx, g);
       delete g;
       cuda_check(e, "graph capture");
     }
@@ -378,7 +387,7 @@ fopt_status fopt_graph_destroy(fopt_ctx* ctx, fopt_graph* g) {
     cuda_check(cudaStreamSynchronize(ctx->stream), "sync");
     if (g->exec) cudaGraphExecDestroy(g->exec);
     if (g->graph) cudaGraphDestroy(g->graph);
-    release_graph_ws(g);
+    release_graph_ws(ctx, g);
     delete g;
     if (--ctx->graphs_alive == 0) {
       for (void* p : ctx->retired) cudaFree(p);

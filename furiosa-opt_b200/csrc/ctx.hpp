@@ -91,6 +91,7 @@ struct fopt_ctx {
   size_t gemm_cnt_n = 0;
   bool gemm_cnt_dirty = false;
   std::map<cudaStream_t, std::pair<void*, size_t>> cache_ws;  // cache-attention workspace of each stream
+  std::map<void*, size_t> cache_ws_live;  // these and the captured graphs' own, with their sizes
   cudaStream_t copy_in = nullptr, copy_out = nullptr;  // host <-> device pipelines of the host-buffer calls
   void* pinned[2] = {nullptr, nullptr};  // host staging for file -> device streaming
   cudaEvent_t pinned_ev[2] = {nullptr, nullptr};

@@ -27,11 +27,8 @@
 // Four warps take a run of 16-token tiles each, with their own rings of cp.async stages (no block barrier
 // while keys stream), and merge their (maximum, sum, output) at the end of a segment.
 //
-// Work: all (sequence, row block, key head) of the call, in 64-token tiles, form one line that is cut
-// into equal shares, one per resident block, from the lengths on the device: no host knowledge of them, no idle
-// blocks, any mixture of lengths. A segment cut between blocks leaves partial results in a workspace; the
-// last of its blocks to arrive adds them up in order, so results do not depend on timing.
-#include "kvcache.cuh"
+// Segments, of 8 or 16 query rows, are divided between blocks as cache_attention.cuh says.
+#include "cache_attention.cuh"
 
 namespace fopt {
 namespace kv {
@@ -43,75 +40,19 @@ constexpr int kTileTokens = 16 * kWarps;
 constexpr int kBlocks = 3;       // resident blocks an SM, where the registers allow (168 a thread)
 constexpr int kSegmentCost = 4;  // beginning and ending a segment takes about as long as this many tiles
 constexpr int kStages = 4;
-constexpr float kNone = -0x1p120f;  // the maximum of a part that has no score; its sum is 0
-constexpr float kLazy = 8.0f;  // log2 by which a score may exceed the running maximum before it moves
-
-struct AttnArgs {
-  uint16_t* o;
-  const uint16_t* q;
-  Cache cache;
-  const int32_t* table;
-  const int32_t* q_start;
-  const int32_t* kv_len;
-  int32_t* err;
-  float* ws;          // partial results: two slots a block (see slot())
-  uint32_t* counter;  // arrivals at the segment that begins in a block; zero between launches
-  int batch, tokens, width, hq, group;
-  float scale;
-  int causal;
-};
-
-// ---- the division of work ----
-struct Seq {
-  int q0, rows;   // first query token; query rows per key head (tokens x group)
-  int queries, keys;
-  int tiles;      // kTileTokens-token tiles, one at least: a sequence without keys still writes its rows
-  int units;      // of work in one segment (the row block of a key head): its tiles and kSegmentCost
-};
-
-// Sequence b's query range and key count, cut to what the arguments allow.
-__device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
-  const int s0 = a.q_start[b], s1 = a.q_start[b + 1], n = a.kv_len[b];
-  Seq s;
-  s.q0 = min(max(s0, 0), a.tokens);
-  const int q1 = min(max(s1, s.q0), a.tokens);
-  s.queries = q1 - s.q0;
-  s.rows = s.queries * a.group;
-  s.keys = (int)min((int64_t)max(n, 0), (int64_t)a.width * a.cache.page_size);
-  s.tiles = max(1, (s.keys + kTileTokens - 1) / kTileTokens);
-  s.units = s.tiles + kSegmentCost;
-  if (s.q0 != s0 || q1 != s1) atomicExch(a.err, kBadStart);
-  if (s.keys != n) atomicExch(a.err, kBadLength);
-  return s;
-}
+constexpr int kFewRows = 32;     // query rows per key head up to which a sequence is tokens_kernel's
+// The sequence's tiles (one at least: a sequence without keys still writes its rows), and how long its segments
+// and all of them together are in the division of work.
+__device__ __forceinline__ int tiles_of(const Seq& s) { return max(1, (s.keys + kTileTokens - 1) / kTileTokens); }
 template <int R>
 __device__ __forceinline__ long long units(const AttnArgs& a, const Seq& s) {
-  return (long long)((s.rows + R - 1) / R) * a.cache.heads * s.units;
+  return s.rows >= a.long_rows ? 0 : (long long)((s.rows + R - 1) / R) * a.cache.heads * (tiles_of(s) + kSegmentCost);
 }
-__device__ __forceinline__ long long quotient(long long a, long long b) {  // both >= 0; a 64-bit division takes long
-  return ((a | b) >> 32) ? a / b : (long long)((uint32_t)a / (uint32_t)b);
-}
-// Of `total` units on n <= total blocks, the first total % n blocks have one more than the others.
-struct Shares {
-  long long each;
-  int more;
-  __device__ __forceinline__ Shares(long long total, int n) : each(quotient(total, n)), more((int)(total - each * n)) {}
-  __device__ __forceinline__ long long first(int c) const { return each * c + min(c, more); }
-  __device__ __forceinline__ int owner(long long unit) const {
-    const long long wide = (each + 1) * more;
-    return unit < wide ? (int)quotient(unit, each + 1) : more + (int)quotient(unit - wide, each);
-  }
-};
 
 // ---- small pieces ----
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-// A value that the compiler keeps in its register instead of computing it again from the lane number.
-__device__ __forceinline__ int kept(int x) {
-  asm volatile("" : "+r"(x));
-  return x;
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -142,39 +83,12 @@ __device__ __forceinline__ void mma_bf16(float* d, uint32_t a0, uint32_t a1, uin
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float exp2_(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float step_of(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float offset_of(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 // Two codes as f16 subnormals: (code + 8) 2^-24 from bits 0-3 and 16-19, (code + 8) 2^-20 from bits 4-7 and 20-23.
-// One lop3 each ((x & mask) ^ constant), the masks in registers: with both constants immediate it takes two
-// instructions (64 more a tile, a quarter of the ALU's work).
-struct Masks {
-  uint32_t low, high;
-};
-__device__ __forceinline__ uint32_t masked(uint32_t x, uint32_t mask, uint32_t flip) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(x), "r"(mask), "r"(flip));
-  return r;
-}
 __device__ __forceinline__ uint32_t codes_low(const Masks& m, uint32_t x) { return masked(x, m.low, 0x00080008u); }
 __device__ __forceinline__ uint32_t codes_high(const Masks& m, uint32_t x) { return masked(x, m.high, 0x00800080u); }
 template <int N>
@@ -264,10 +178,8 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, const Seq& s, int 
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    int ex = top > 0.0f ? min(ilogbf(top), 127) : 0;
-    // 2^(8 - ex) may pass the f32 range: two factors
-    const float up0 = scalbnf(1.0f, (8 - ex) / 2), up1 = scalbnf(1.0f, 8 - ex - (8 - ex) / 2);
-    const float down = scalbnf(a.scale * 1.44269504088896340736f, ex + 12);
+    const RowScale up(top);
+    const float down = scalbnf(a.scale * 1.44269504088896340736f, up.e + 12);
     float sum[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
@@ -276,7 +188,7 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, const Seq& s, int 
       sum[j] = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        v[e] = (e & 1 ? offset_of(x[e >> 1]) : step_of(x[e >> 1])) * up0 * up1;
+        v[e] = (e & 1 ? offset_of(x[e >> 1]) : step_of(x[e >> 1])) * up.up0 * up.up1;
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -285,9 +197,7 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, const Seq& s, int 
         const uint32_t h = f16x2(v[e] * by, v[e + 4] * by);
         q.f[nb][2 * j + (e >> 1)][e & 1] = h;
         // the sum of what the products take
-        float lo, hi;
-        asm("{.reg .f16 a, b; mov.b32 {a, b}, %2; cvt.f32.f16 %0, a; cvt.f32.f16 %1, b;}" : "=f"(lo), "=f"(hi) : "r"(h));
-        sum[j] += (lo + hi) / by;
+        sum[j] += sum_of(h) / by;
       }
       sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
       sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
@@ -312,7 +222,7 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, const Seq& s, int 
       q.scale[nb][c] = __shfl_sync(0xffffffffu, down, from);
       const int rc = row0 + nb * 8 + 2 * i + c;
       // columns past the rows hold q = 0 and no one reads them: they need no mask of their own
-      q.limit[nb][c] = rc >= s.rows ? s.keys : a.causal ? min(s.keys, s.keys - s.queries + rc / a.group + 1) : s.keys;
+      q.limit[nb][c] = rc >= s.rows ? s.keys : seen(a, s, rc);
     }
   }
 }
@@ -328,7 +238,7 @@ __device__ __forceinline__ Places places() {
   const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3, at = g * NG * 2;
   return {kept(g * (D / 2) + i * NG * 4), kept(g * NG * 4 + i * 4), kept(g * NG * 4),
           kept(2 * i * (D / 2) + v_chunk<NG>(2 * i, at >> 4) * 16 + (at & 15)),
-          {(uint32_t)kept(0x000f000f), (uint32_t)kept(0x00f000f0)}};
+          masks()};
 }
 
 // One tile of 16 tokens, from its stage; token0 is its first.
@@ -498,58 +408,17 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
   using P = Partial<NG, NB>;
   constexpr int D = S::D, R = S::R;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long sums[kWarps];
-  __shared__ long long found_at;
-  __shared__ int found;
   __shared__ float ml[2][kWarps][R];
   __shared__ int last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
 
-  // this block's share of the line: the total, then the sequence in which the share begins
-  long long mine = 0;
-  for (int b = tid; b < a.batch; b += kThreads) mine += units<R>(a, sequence(a, b));
-  long long total = mine;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) sums[warp] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) total += sums[w];
-  if (total == 0) return;
-  const int blocks = (int)min((long long)gridDim.x, total);
-  if (blockIdx.x >= blocks) return;
-  const Shares shares(total, blocks);
+  const Start start = share_start<kThreads>(a.batch, [&](int b) { return units<R>(a, sequence(a, b)); });
+  if ((int)blockIdx.x >= start.blocks) return;
+  const Shares shares(start.total, start.blocks);
   long long unit = shares.first(blockIdx.x);
   const long long end = shares.first(blockIdx.x + 1);
-  long long before = 0;  // units of the sequences before the chunk
-  for (int b0 = 0;; b0 += kThreads) {
-    const int b = b0 + tid;
-    const long long u = b < a.batch ? units<R>(a, sequence(a, b)) : 0;
-    long long upto = u;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    __syncthreads();
-    if (lane == 31) sums[warp] = upto;
-    if (tid == 0) found = -1;
-    __syncthreads();
-    long long here = before;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) here += sums[w];
-      before += sums[w];
-    }
-    if (unit >= here + upto - u && unit < here + upto) {
-      found = b;
-      found_at = here + upto - u;
-    }
-    __syncthreads();
-    if (found >= 0) break;
-  }
-  int b = found;
-  long long seq_at = found_at;
+  int b = start.b;
+  long long seq_at = start.seq_at;
   Seq s = sequence(a, b);
 
   const Places at = places<NG>();
@@ -572,10 +441,11 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
       seq_at += units<R>(a, s);
       s = sequence(a, ++b);
     }
-    const int seg = (int)quotient(unit - seq_at, s.units);
-    const long long seg_at = seq_at + (long long)seg * s.units;
+    const int tiles = tiles_of(s), length = tiles + kSegmentCost;
+    const int seg = (int)quotient(unit - seq_at, length);
+    const long long seg_at = seq_at + (long long)seg * length;
     // its cost stands before its first tile; a share that ends within it has no tile here
-    const int u1 = (int)min((long long)s.units, end - seg_at);
+    const int u1 = (int)min((long long)length, end - seg_at);
     const int t0 = max(0, (int)(unit - seg_at) - kSegmentCost), t1 = u1 - kSegmentCost;
     const int head = seg % a.cache.heads, row0 = seg / a.cache.heads * R;
     unit = seg_at + u1;
@@ -585,8 +455,8 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
     load_query<NG, NB>(a, s, head, row0, q);
     // keys that any row of the block sees, and that every row sees
     const int rows = min(R, s.rows - row0);
-    const int most = a.causal ? min(s.keys, s.keys - s.queries + (row0 + rows - 1) / a.group + 1) : s.keys;
-    const int sure = a.causal ? min(s.keys, s.keys - s.queries + row0 / a.group + 1) : s.keys;
+    const int most = seen(a, s, row0 + rows - 1);
+    const int sure = seen(a, s, row0);
     State<NG, NB> st;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -697,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
       *(uint2*)(a.o + ((int64_t)(s.q0 + token) * a.hq + head * a.group + row - token * a.group) * D + d) =
           make_uint2(bf16x2_rule(v.x * n, v.y * n), bf16x2_rule(v.z * n, v.w * n));
     };
-    const bool whole = t0 == 0 && t1 == s.tiles;
+    const bool whole = t0 == 0 && t1 == tiles;
     float* part = P::slot(a.ws, blockIdx.x, t0 == 0);
     for (int k = tid; k < rows * (D / 4); k += kThreads) {
       const int r = k / (D / 4), d = k % (D / 4) * 4;
@@ -723,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
       }
     }
     if (!whole) {
-      const int c0 = shares.owner(seg_at + kSegmentCost), c1 = shares.owner(seg_at + s.units - 1);
+      const int c0 = shares.owner(seg_at + kSegmentCost), c1 = shares.owner(seg_at + length - 1);
       __threadfence();
       __syncthreads();
       if (tid == 0) {
@@ -754,19 +624,19 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
   }
 }
 
+constexpr int kCounters = 1024;  // of each kernel, one for each block
+
 template <int NG, int NB>
-void launch_tokens(fopt_ctx* ctx, AttnArgs a, int sms) {
+constexpr int tokens_blocks() { return NG <= 4 && NB == 1 ? kBlocks : NG <= 4 ? 2 : 1; }
+template <int NG, int NB>
+size_t tokens_workspace(int sms) { return (size_t)sms * tokens_blocks<NG, NB>() * 2 * Partial<NG, NB>::kFloats * sizeof(float); }
+
+template <int NG, int NB>
+void launch_tokens(fopt_ctx* ctx, const AttnArgs& a, int sms) {
   using S = Shared<NG, NB>;
-  const int grid = sms * (NG <= 4 && NB == 1 ? kBlocks : NG <= 4 ? 2 : 1);
   cuda_check(cudaFuncSetAttribute(tokens_kernel<NG, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes),
              "cache attention shared memory");
-  const size_t partials = (size_t)grid * 2 * Partial<NG, NB>::kFloats * sizeof(float);
-  // the counters first: other variants' partial results must not reach them
-  uint8_t* ws = (uint8_t*)cache_workspace(ctx, 4096 + partials);
-  a.counter = (uint32_t*)ws;
-  a.ws = (float*)(ws + 4096);
-  require(grid <= 1024, "fopt_cache_attention: more resident blocks than counters");
-  tokens_kernel<NG, NB><<<grid, kThreads, S::kBytes, ctx->stream>>>(a);
+  tokens_kernel<NG, NB><<<sms * tokens_blocks<NG, NB>(), kThreads, S::kBytes, ctx->stream>>>(a);
   launched(ctx, "cache attention");
 }
 
@@ -808,12 +678,32 @@ extern "C" fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* 
     a.causal = causal != 0;
     int sms = 0;
     cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, ctx->device), "SM count");
+    require(sms * kv::kBlocks <= kv::kCounters, "fopt_cache_attention: more resident blocks than counters");
+    const int dim = cache->head_dim;
+    // Sequences of more than kv::kFewRows query rows go to rows_kernel, whose tiles of 256 rows take about as long
+    // as that many rows of tokens_kernel (head_dim 256 exceeds its tensor memory). The lengths are the device's,
+    // so both are launched unless no sequence can be that long.
+    const bool rows = dim != 256 && (int64_t)tokens * a.group > kv::kFewRows;
+    a.long_rows = rows ? kv::kFewRows + 1 : INT32_MAX;
     // 16 rows a block where a sequence has that many on average: the codes are expanded once for both halves
     const bool two = (int64_t)tokens * a.group > 8 * (int64_t)batch;
-    switch (cache->head_dim) {
+    const size_t few = dim == 64 ? (two ? kv::tokens_workspace<2, 2>(sms) : kv::tokens_workspace<2, 1>(sms))
+                     : dim == 128 ? (two ? kv::tokens_workspace<4, 2>(sms) : kv::tokens_workspace<4, 1>(sms))
+                                  : kv::tokens_workspace<8, 1>(sms);
+    // the counters first, so that no variant's partial results reach another's
+    const size_t counters = 2 * kv::kCounters * sizeof(uint32_t);
+    uint8_t* ws = (uint8_t*)cache_workspace(ctx, counters + few + (rows ? kv::rows_workspace(dim, sms) : 0));
+    a.counter = (uint32_t*)ws;
+    a.ws = (float*)(ws + counters);
+    switch (dim) {
       case 64: two ? kv::launch_tokens<2, 2>(ctx, a, sms) : kv::launch_tokens<2, 1>(ctx, a, sms); break;
       case 128: two ? kv::launch_tokens<4, 2>(ctx, a, sms) : kv::launch_tokens<4, 1>(ctx, a, sms); break;
       default: kv::launch_tokens<8, 1>(ctx, a, sms); break;
+    }
+    if (rows) {
+      a.counter += kv::kCounters;
+      a.ws = (float*)(ws + counters + few);
+      kv::launch_rows(ctx, a, dim, sms);
     }
   });
 }

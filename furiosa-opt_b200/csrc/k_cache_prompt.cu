@@ -1,0 +1,667 @@
+// Attention over the paged 4-bit cache for sequences with many query rows (prompts and pieces of them), on the
+// fifth-generation tensor cores.
+//
+// The query rows of one key head are (token, query head of its group) pairs; a segment is 256 of them, as two
+// 128-row tiles, against all keys that they see, in tiles of 128 tokens. 384 threads, one block an SM:
+//   warp 0      owns tensor memory and issues, per key tile, S_t = Q_t K^T and O_t += P_t V for t = 0, 1;
+//   warps 1-3   expand codes, in turn 32 tokens each: a lane takes one token, reads its row of K and of V straight
+//               from the cache's pages (64 contiguous bytes at D = 128) ahead of its turn, and writes
+//               value = code * step + offset as f16 into the 128-byte-swizzled tiles;
+//   warps 4-11  softmax: a thread per query row reads its scores from tensor memory, keeps the running maximum and
+//               sum, and writes P as f16 over the first half of its scores.
+// While one tile's softmax runs the tensor cores work on the other. Every wait is bounded (2 s) and reports
+// through the context's error word.
+//
+// K's offsets go in apart: a code times its step has 3 + 8 bits and is exact in f16, where code * step + offset
+// would be rounded (to 2^-12 of K, which sharp scores of a hundred and more turn into percents of P). The offsets'
+// share of a score, sum_groups offset (sum of q), is one more step of the same product, over k = (part, group) with
+// the sums of q in two f16 parts.
+//
+// f16 holds 11 bits of a value where bf16 would hold 8, but not every size of it: every 32
+// tokens' K is scaled by a power of two and V by another, so that the largest is in [2^4, 2^9). K's comes back with the
+// scores. V's, 2^ev, goes into the exponent: with x = score + ev, P = 2^(x - m) and l = sum P 2^-ev, O = sum P V 2^-ev
+// and l share the base m, which follows the largest x as it would the largest score.
+//
+// A 16-byte chunk holds 8 codes in the order that pairs come out of a word (0, 4, 1, 5, 2, 6, 3, 7): for K the
+// queries are stored in the same order, for V the output's columns are put right when they leave.
+//
+// What bounds it: the tensor cores take 32 steps of M 128, N 128, K 16 per key tile (about 3300 cycles); the
+// exponentials take 2048, the expansion about 450 issue slots of each scheduler.
+#include "cache_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace fopt {
+namespace kv {
+namespace {
+
+using namespace attn;
+
+constexpr int kRows = 256, kKeys = 128;  // of a segment and of a tile
+constexpr int kRowThreads = 384;     // 168 registers each
+constexpr int kHalf = 16384;             // 128 rows of 64 f16 (128 bytes), the unit of the swizzled tiles
+constexpr int kOffsets = 128 * 32;        // 128 rows of 16 f16: the sums of a tile's q, or the offsets of a key tile
+constexpr int kCost = 2;                 // key tiles that beginning and ending a segment takes as long as
+constexpr int kUncut = 8;                // segments of fewer tiles are not shared between blocks
+constexpr float kLog2e = 1.44269504088896340736f;
+
+template <int NG>
+struct Tiles {
+  static constexpr int D = NG * kGroup, kHalves = D / 64;
+  static constexpr int kTile = kHalves * kHalf;      // Q_t, K or V
+  // 2 Q, 2 stages of K and of V, the offset steps of Q and K, alignment, barriers and scales; more than half an
+  // SM's, since a second block would only wait for tensor memory
+  static constexpr int kAll = 6 * kTile + 4 * kOffsets + 1024 + 512;
+  static constexpr int kBytes = kAll > 120000 ? kAll : 120000;
+  static constexpr int kSlot = kRows * (D + 2);      // floats of a partial result
+};
+
+__device__ __forceinline__ int blocks_of(const Seq& s) { return (s.rows + kRows - 1) / kRows; }
+// Key tiles of a row block: up to the last key that its last row sees, one at least.
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, const Seq& s, int rb) {
+  return max(1, (max(0, seen(a, s, min(s.rows, (rb + 1) * kRows) - 1)) + kKeys - 1) / kKeys);
+}
+__device__ __forceinline__ long long units(const AttnArgs& a, const Seq& s) {
+  if (s.rows < a.long_rows) return 0;
+  long long n = 0;
+  for (int rb = 0; rb < blocks_of(s); ++rb) n += tiles_of(a, s, rb) + kCost;
+  return n * a.cache.heads;
+}
+
+struct Item {
+  Seq s;
+  int b, head, row0;
+  int t0, t1, tiles;  // this block's key tiles of the segment, and all of them
+  long long at;       // the segment's first unit
+};
+
+// A block's segments in order. Every role of the block walks them by itself.
+struct Walk {
+  const AttnArgs& a;
+  long long pos, end, rb_at;
+  int b, rb;
+  Seq s;
+
+  __device__ __forceinline__ Walk(const AttnArgs& args, const Start& st, const Shares& sh)
+      : a(args), pos(sh.first(blockIdx.x)), end(sh.first(blockIdx.x + 1)), rb_at(st.seq_at), b(st.b), rb(0),
+        s(sequence(args, st.b)) {}
+
+  __device__ bool next(Item& it) {
+    while (pos < end) {
+      int length;
+      for (;;) {  // the row block that holds pos
+        if (s.rows < a.long_rows || rb == blocks_of(s)) {
+          s = sequence(a, ++b);
+          rb = 0;
+          continue;
+        }
+        length = tiles_of(a, s, rb) + kCost;
+        if (pos < rb_at + (long long)length * a.cache.heads) break;
+        rb_at += (long long)length * a.cache.heads;
+        ++rb;
+      }
+      const int head = (int)quotient(pos - rb_at, length);
+      const long long at = rb_at + (long long)head * length;
+      int from = (int)(pos - at), to = (int)min((long long)length, end - at);
+      if (length < kUncut + kCost) {  // whole, to the block on whose side of the cut its middle is
+        if (from > 0) {
+          if (2 * from >= length) {
+            pos = at + length;
+            continue;
+          }
+          from = 0;
+        }
+        if (to < length) {
+          if (2 * to < length) {
+            pos = end;
+            break;
+          }
+          to = length;
+        }
+      }
+      pos = at + to;
+      it.t0 = max(0, from - kCost);
+      it.t1 = to - kCost;
+      if (it.t1 <= it.t0) continue;  // within its cost, which stands before its first tile
+      it.s = s;
+      it.b = b;
+      it.head = head;
+      it.row0 = rb * kRows;
+      it.tiles = length - kCost;
+      it.at = at;
+      return true;
+    }
+    return false;
+  }
+};
+
+// Eight codes of a word as four f16 pairs code * step + offset. The codes are exact first: 1024 + (code + 8) - 1032
+// and (1024 + 16 (code + 8)) / 16 - 72.
+__device__ __forceinline__ uint4 expand(const Masks& m, uint32_t x, uint32_t step, uint32_t offset) {
+  auto value = [&](uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(c), "r"(step), "r"(offset));
+    return r;
+  };
+  auto low = [&](uint32_t w) {
+    uint32_t r;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(masked(w, m.low, 0x64086408u)), "r"(0xe408e408u));
+    return value(r);
+  };
+  auto high = [&](uint32_t w) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(masked(w, m.high, 0x64806480u)), "r"(0x2c002c00u), "r"(0xd480d480u));
+    return value(r);
+  };
+  const uint32_t y = x >> 8;
+  return make_uint4(low(x), high(x), low(y), high(y));
+}
+
+// Where chunk c (16 bytes) of row t of a tile is.
+__device__ __forceinline__ uint32_t place(int t, int c) { return (c >> 3) * kHalf + t * 128 + (((c & 7) ^ (t & 7)) << 4); }
+// ... and chunk c (0, 1) of row t of an offset step: unswizzled 8-row by 16-byte blocks, the two of a row group
+// next to each other.
+__device__ __forceinline__ uint32_t offsets_place(int t, int c) { return (t >> 3) * 256 + c * 128 + (t & 7) * 16; }
+__device__ __forceinline__ uint64_t offsets_desc(uint32_t addr) {
+  uint64_t d = (uint64_t)((addr & 0x3FFFF) >> 4);
+  d |= (uint64_t)(128 >> 4) << 16;  // between the blocks of a row group (along k)
+  d |= (uint64_t)(256 >> 4) << 32;  // between row groups
+  d |= (uint64_t)1 << 46;
+  return d;
+}
+__device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// What a lane that expands has in hand of one token.
+template <int NG>
+struct Row {
+  uint32_t k[4 * NG], v[4 * NG], ks[NG], vs[NG];
+};
+
+template <int N>
+__device__ __forceinline__ void load_row(uint32_t* w, const void* p) {
+  if constexpr (N == 2) *(uint2*)w = __ldg((const uint2*)p);
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) *(uint4*)(w + 4 * i) = __ldg((const uint4*)p + i);
+}
+
+template <int NG>
+__device__ __forceinline__ void load_token(const AttnArgs& a, const Item& it, int token, Row<NG>& r) {
+  bool there = false;
+  int64_t row = 0;
+  if (token < it.s.keys) {
+    const int entry = (int)fdiv(a.cache.by_page, (uint32_t)token);
+    const int page = a.table[(int64_t)it.b * a.width + entry];
+    there = page >= 0 && page < a.cache.pages;
+    if (there) row = ((int64_t)page * a.cache.heads + it.head) * a.cache.page_size + (token - entry * a.cache.page_size);
+    else atomicExch(a.err, kBadPage);
+  }
+  if (there) {
+    load_row<4 * NG>(r.k, a.cache.k + row * (NG * 16));
+    load_row<4 * NG>(r.v, a.cache.v + row * (NG * 16));
+    load_row<NG>(r.ks, a.cache.k_scale + row * NG);
+    load_row<NG>(r.vs, a.cache.v_scale + row * NG);
+  } else {  // past the keys, or of no page: zeros, whatever the slot holds
+#pragma unroll
+    for (int i = 0; i < 4 * NG; ++i) r.k[i] = r.v[i] = 0;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) r.ks[i] = r.vs[i] = 0;
+  }
+}
+
+// The exponent that brings the largest of a warp's values to [2^4, 2^9), from the sizes of their groups.
+template <int NG>
+__device__ __forceinline__ int warp_exponent(const uint32_t* scales) {
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NG; ++j) top = fmaxf(top, fmaf(8.0f, step_of(scales[j]), fabsf(offset_of(scales[j]))));
+  const uint32_t all = __reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu);
+  return all ? min(max((int)(all >> 23) - 127 - 4, -120), 120) : 0;
+}
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // e in -126 .. 127
+
+template <int NG>
+__global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
+  using T = Tiles<NG>;
+  constexpr int D = T::D;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* sQ = smem;                  // tile t at sQ + t * kTile
+  uint8_t* sK = smem + 2 * T::kTile;   // stage n at sK + n * kTile
+  uint8_t* sV = smem + 4 * T::kTile;
+  uint8_t* sQz = smem + 6 * T::kTile;  // the offset steps: of tile t at sQz + t * kOffsets, of stage n at sKz + ...
+  uint8_t* sKz = sQz + 2 * kOffsets;
+  uint64_t* bars = (uint64_t*)(sKz + 2 * kOffsets);
+  uint64_t* k_full = bars;         // [2]
+  uint64_t* k_empty = bars + 2;    // [2]
+  uint64_t* v_full = bars + 4;     // [2]
+  uint64_t* v_empty = bars + 6;    // [2]
+  uint64_t* x_full = bars + 8;     // [4] the exponents of key tile n are in place n % 4
+  uint64_t* q_full = bars + 12;    // [2] of tile t
+  uint64_t* s_full = bars + 14;    // [2]
+  uint64_t* p_ready = bars + 16;   // [2]
+  uint64_t* o_done = bars + 18;    // [2] the segment's last product
+  uint64_t* met = bars + 20;       // [2] the 128 softmax threads of a tile among themselves
+  float* k_back = (float*)(bars + 22);  // [4][4] 2^ek of each 32 tokens of a key tile
+  float* v_up = k_back + 16;            // [4][4] ev
+  uint32_t* tmem_slot = (uint32_t*)(v_up + 16);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  int* last = (int*)(tmem_slot + 2);    // [2]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Start start = share_start<kRowThreads>(a.batch, [&](int b) { return units(a, sequence(a, b)); });
+  if ((int)blockIdx.x >= start.blocks) return;
+  const Shares shares(start.total, start.blocks);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&k_full[i]), 4);
+      mbar_init(smem_u32(&k_empty[i]), 1);
+      mbar_init(smem_u32(&v_full[i]), 4);
+      mbar_init(smem_u32(&v_empty[i]), 1);
+      mbar_init(smem_u32(&q_full[i]), 128);
+      mbar_init(smem_u32(&s_full[i]), 1);
+      mbar_init(smem_u32(&p_ready[i]), 128);
+      mbar_init(smem_u32(&o_done[i]), 1);
+      mbar_init(smem_u32(&met[i]), 128);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&x_full[i]), 4);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;  // S0, S1 (128 columns each), O0, O1 (at 256 and 384)
+  Walk walk(a, start, shares);
+  Item it;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // f16 x f16 -> f32, M = 128
+      const uint32_t base = (1u << 4) | ((uint32_t)(128 >> 4) << 24);
+      const uint32_t qk = base | ((uint32_t)(kKeys >> 3) << 17), pv = base | ((uint32_t)(D >> 3) << 17) | kIdescBMajorMN;
+      auto scores = [&](int t, int n) {  // S_t of key tile n
+        const uint64_t qd = sdesc(smem_u32(sQ + t * T::kTile)), kd = sdesc(smem_u32(sK + (n & 1) * T::kTile));
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (uint32_t)((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+          mma_bf16(tmem + t * 128, qd + off, kd + off, qk, k != 0);
+        }
+        mma_bf16(tmem + t * 128, offsets_desc(smem_u32(sQz + t * kOffsets)),
+                 offsets_desc(smem_u32(sKz + (n & 1) * kOffsets)), qk, 1);
+        commit(smem_u32(&s_full[t]));
+      };
+      int n = 0, seg = 0;  // key tiles and segments so far
+      bool ok = true;
+      for (; ok && walk.next(it); ++seg) {
+        const int n1 = n + it.t1 - it.t0;
+        ok = mbar_wait(smem_u32(&k_full[n & 1]), (n >> 1) & 1, abort_flag, a.err, 401);
+        for (int t = 0; ok && t < 2; ++t) {
+          ok = mbar_wait(smem_u32(&q_full[t]), seg & 1, abort_flag, a.err, 402);
+          if (!ok) break;
+          fence_after();
+          scores(t, n);
+        }
+        if (ok) commit(smem_u32(&k_empty[n & 1]));
+        for (int first = n; ok && n < n1; ++n) {
+          for (int t = 0; ok && t < 2; ++t) {
+            ok = (t || mbar_wait(smem_u32(&v_full[n & 1]), (n >> 1) & 1, abort_flag, a.err, 403)) &&
+                 mbar_wait(smem_u32(&p_ready[t]), n & 1, abort_flag, a.err, 404);
+            if (!ok) break;
+            fence_after();
+            const uint64_t vd = vdesc(smem_u32(sV + (n & 1) * T::kTile));
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+              mma_bf16_ta(tmem + 256 + t * 128, tmem + t * 128 + 8 * k, vd + (uint64_t)(128 * k), pv, (n - first) | k);
+            if (t) commit(smem_u32(&v_empty[n & 1]));
+            if (n + 1 == n1) {
+              commit(smem_u32(&o_done[t]));
+            } else {
+              // behind the product that reads P_t out of the same columns: one thread's MMAs run in order
+              ok = t || mbar_wait(smem_u32(&k_full[(n + 1) & 1]), ((n + 1) >> 1) & 1, abort_flag, a.err, 405);
+              if (!ok) break;
+              fence_after();
+              scores(t, n + 1);
+              if (t) commit(smem_u32(&k_empty[(n + 1) & 1]));
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp <= 3) {
+    const Masks m = masks();
+    Row<NG> r;
+    int low_v = 0;
+    bool fresh = true;  // the segment's first 32 tokens of this warp
+    bool more = walk.next(it), ok = true;
+    int t = more ? it.t0 : 0;
+    int q = warp - 1, n = 0;  // the quarter of its tile, and its tile's number, of the tokens in r
+    if (more) load_token<NG>(a, it, t * kKeys + q * 32 + lane, r);
+    while (more) {
+      const int ek = warp_exponent<NG>(r.ks);
+      int ev = warp_exponent<NG>(r.vs);
+      // V far below the segment's first is not brought up all the way: l would pass the f32 range
+      if (fresh) low_v = ev - 40;
+      ev = max(ev, low_v);
+      const Row<NG> now = r;
+      const int row = q * 32 + lane, tile = n;
+      // this warp's next row is on its way while this one is expanded
+      fresh = false;
+      q += 3;
+      if (q >= 4) {
+        q -= 4;
+        ++n;
+        if (++t == it.t1) {
+          fresh = true;
+          more = walk.next(it);
+          t = it.t0;
+        }
+      }
+      if (more) load_token<NG>(a, it, t * kKeys + q * 32 + lane, r);
+
+      ok = mbar_wait(smem_u32(&k_empty[tile & 1]), ((tile >> 1) & 1) ^ 1, abort_flag, a.err, 411);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) {  // place tile % 4: the softmax of tile - 4 is over, or S of tile - 2 could not be
+        k_back[(tile & 3) * 4 + (row >> 5)] = power(ek);
+        v_up[(tile & 3) * 4 + (row >> 5)] = (float)ev;
+        mbar_arrive(smem_u32(&x_full[tile & 3]));
+      }
+      const float kf = power(-ek), vf = power(-ev);
+      uint8_t* tk = sK + (tile & 1) * T::kTile;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        const float s = step_of(now.ks[j]) * kf;
+        const uint32_t s2 = f16x2(s, s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(uint4*)(tk + place(row, 4 * j + i)) = expand(m, now.k[i * NG + j], s2, 0u);
+      }
+      {  // k = part * NG + group for the two parts of the sums of q, then zeros
+        uint32_t z[8] = {};
+#pragma unroll
+        for (int j = 0; j < NG / 2; ++j)
+          z[j] = z[j + NG / 2] = f16x2(offset_of(now.ks[2 * j]) * kf, offset_of(now.ks[2 * j + 1]) * kf);
+        uint8_t* tz = sKz + (tile & 1) * kOffsets;
+        *(uint4*)(tz + offsets_place(row, 0)) = make_uint4(z[0], z[1], z[2], z[3]);
+        *(uint4*)(tz + offsets_place(row, 1)) = make_uint4(z[4], z[5], z[6], z[7]);
+      }
+      async_fence();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&k_full[tile & 1]));
+
+      ok = mbar_wait(smem_u32(&v_empty[tile & 1]), ((tile >> 1) & 1) ^ 1, abort_flag, a.err, 412);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      uint8_t* tv = sV + (tile & 1) * T::kTile;
+#pragma unroll
+      for (int j = 0; j < NG / 2; ++j) {  // words 2 g + j (NG = 4) of groups 2 j and 2 j + 1
+        const uint32_t s2 = f16x2(step_of(now.vs[2 * j]) * vf, step_of(now.vs[2 * j + 1]) * vf);
+        const uint32_t z2 = f16x2(offset_of(now.vs[2 * j]) * vf, offset_of(now.vs[2 * j + 1]) * vf);
+#pragma unroll
+        for (int g = 0; g < 8; ++g)
+          *(uint4*)(tv + place(row, g * (NG / 2) + j)) = expand(m, now.v[g * (NG / 2) + j], s2, z2);
+      }
+      async_fence();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&v_full[tile & 1]));
+    }
+  } else {
+    const int t = (warp - 4) >> 2, quarter = warp & 3;  // tile, and the tensor-memory lanes that the warp may read
+    const int r = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tS = tmem + t * 128 + lanes, tO = tmem + 256 + t * 128 + lanes;
+    uint8_t* tq = sQ + t * T::kTile;
+
+    // writes the row's query into Q_t; returns the factor of its scores (K's powers of two aside)
+    auto put_query = [&](const Item& x) -> float {
+      const int row = x.row0 + t * 128 + r;
+      uint32_t w[D / 2];
+      float top = 0.0f;
+      if (row < x.s.rows) {
+        const int token = row / a.group;
+        const uint4* p = (const uint4*)(a.q + ((int64_t)(x.s.q0 + token) * a.hq + x.head * a.group + row - token * a.group) * D);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) *(uint4*)(w + 4 * c) = __ldg(p + c);
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 2; ++c) w[c] = 0;
+      }
+#pragma unroll
+      for (int c = 0; c < D / 2; ++c) top = max3(top, fabsf(step_of(w[c])), fabsf(offset_of(w[c])));
+      const RowScale up(top);
+      float sum[NG] = {};  // of q as f16 holds it, by group
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[2 * e] = step_of(w[4 * c + e]) * up.up0 * up.up1;
+          v[2 * e + 1] = offset_of(w[4 * c + e]) * up.up0 * up.up1;
+        }
+        const uint4 h = make_uint4(f16x2(v[0], v[4]), f16x2(v[1], v[5]), f16x2(v[2], v[6]), f16x2(v[3], v[7]));
+        sum[c / 4] += (sum_of(h.x) + sum_of(h.y)) + (sum_of(h.z) + sum_of(h.w));
+        *(uint4*)(tq + place(r, c)) = h;
+      }
+      uint32_t z[8] = {};
+#pragma unroll
+      for (int j = 0; j < NG / 2; ++j) {
+        z[j] = f16x2(sum[2 * j], sum[2 * j + 1]);
+        z[j + NG / 2] = f16x2(sum[2 * j] - low_half(z[j]), sum[2 * j + 1] - high_half(z[j]));
+      }
+      *(uint4*)(sQz + t * kOffsets + offsets_place(r, 0)) = make_uint4(z[0], z[1], z[2], z[3]);
+      *(uint4*)(sQz + t * kOffsets + offsets_place(r, 1)) = make_uint4(z[4], z[5], z[6], z[7]);
+      async_fence();
+      mbar_arrive(smem_u32(&q_full[t]));
+      return scalbnf(a.scale * kLog2e, up.e - 8);
+    };
+
+    uint32_t meetings = 0;
+    auto meet = [&]() -> bool {  // a barrier of the tile's softmax threads whose wait is bounded
+      mbar_arrive(smem_u32(&met[t]));
+      const bool here = mbar_wait(smem_u32(&met[t]), meetings++ & 1, abort_flag, a.err, 424);
+      return __all_sync(0xffffffffu, here);
+    };
+    bool more = walk.next(it), ok = true;
+    float qs = more ? put_query(it) : 0.0f;
+    int n = 0;
+    for (int seg = 0; more; ++seg) {
+      const int row = it.row0 + t * 128 + r;
+      const int limit = row < it.s.rows ? seen(a, it.s, row) : it.s.keys;  // rows past the last are not stored
+      float m = 0.0f, l = 0.0f;
+      for (int kt = it.t0; kt < it.t1; ++kt, ++n) {
+        ok = mbar_wait(smem_u32(&x_full[n & 3]), (n >> 2) & 1, abort_flag, a.err, 421) &&
+             mbar_wait(smem_u32(&s_full[t]), n & 1, abort_flag, a.err, 422);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after();
+        const int left = limit - kt * kKeys;  // keys of the tile that the row sees
+        const bool cut = __any_sync(0xffffffffu, left < kKeys);
+        const float* kb = k_back + (n & 3) * 4;
+        const float* vu = v_up + (n & 3) * 4;
+        uint32_t p[64];
+        float sum, top;
+        auto pass = [&] {  // probabilities against the base m, their sum, and the largest x - m
+          sum = 0.0f;
+          top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t s[32];
+            tld32(tS + 32 * c, s);
+            tld_wait_regs(s);
+            const float f = qs * kb[c], up = vu[c] - m;
+            if (cut) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                s[i] = __float_as_uint(32 * c + i < left ? fmaf(__uint_as_float(s[i]), f, up) : -INFINITY);
+            } else {
+              const uint64_t f2 = pack_f32x2(f, f), up2 = pack_f32x2(up, up);
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float x0, x1;
+                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, up2), x0, x1);
+                s[i] = __float_as_uint(x0);
+                s[i + 1] = __float_as_uint(x1);
+              }
+            }
+            uint64_t part[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float x0 = __uint_as_float(s[i]), x1 = __uint_as_float(s[i + 1]);
+              top = max3(top, x0, x1);
+              const float p0 = exp2_(x0), p1 = exp2_(x1);
+              part[(i >> 1) & 1] = add_f32x2(part[(i >> 1) & 1], pack_f32x2(p0, p1));
+              p[16 * c + (i >> 1)] = f16x2(p0, p1);
+            }
+            float s0, s1, s2, s3;
+            unpack_f32x2(part[0], s0, s1);
+            unpack_f32x2(part[1], s2, s3);
+            sum = fmaf((s0 + s1) + (s2 + s3), exp2_(-vu[c]), sum);
+          }
+        };
+        pass();
+        const bool first = kt == it.t0;
+        if (__any_sync(0xffffffffu, first || top > kLazy)) {
+          const float by = first ? (top == -INFINITY ? 0.0f : top) : top > kLazy ? top : 0.0f;
+          m += by;
+          if (!first) {  // S_t was issued behind the last O_t += P_t V: it is complete
+            const float f = exp2_(-by);
+            l *= f;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tld32(tO + 32 * c, o);
+              tld_wait_regs(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tst32(tO + 32 * c, o);
+            }
+          }
+          pass();
+        }
+        l += sum;
+        tst32(tS, p);
+        tst32(tS + 32, p + 32);
+        tst_wait();
+        fence_before();
+        mbar_arrive(smem_u32(&p_ready[t]));
+      }
+      if (!ok) break;
+      // the last scores are complete, so Q_t is free: the next segment's goes in before this one's output
+      const Item done = it;
+      more = walk.next(it);
+      if (more) qs = put_query(it);
+      ok = mbar_wait(smem_u32(&o_done[t]), seg & 1, abort_flag, a.err, 423);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      fence_after();
+
+      const bool live = row < done.s.rows;
+      const int token = live ? row / a.group : 0;
+      uint16_t* out = a.o + ((int64_t)(done.s.q0 + token) * a.hq + done.head * a.group + (live ? row - token * a.group : 0)) * D;
+      // 32 columns in the order of the codes -> 32 / NG neighbouring channels of each group
+      auto write = [&](int c, const float* o, float scale) {
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+          uint32_t w[16 / NG];
+#pragma unroll
+          for (int i = 0; i < 16 / NG; ++i) {  // channels 2 i, 2 i + 1 of the run: code word 4 c + word, its codes e, e + 1
+            const int g = i / 2, word = g * (NG / 2) + j / 2, e = 2 * (i & 1);
+            w[i] = bf16x2_rule(o[8 * word + 2 * e + (j & 1)] * scale, o[8 * word + 2 * e + 2 + (j & 1)] * scale);
+          }
+#pragma unroll
+          for (int i = 0; i < 16 / NG / 4; ++i)
+            *(uint4*)(out + j * kGroup + c * (32 / NG) + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        }
+      };
+      const float mine = l > 0.0f ? m : l == l ? kNone : m;  // a NaN sum stays one
+      if (done.t0 == 0 && done.t1 == done.tiles) {
+        const float scale = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          tld32(tO + 32 * c, (uint32_t*)o);
+          tld_wait_regs((uint32_t*)o);
+          if (live) write(c, o, scale);
+        }
+      } else {
+        // [D / 4][128] float4, so that a warp's rows are contiguous; then maxima and sums
+        auto slot = [&](int block, bool begins) { return a.ws + ((int64_t)block * 2 + begins) * T::kSlot + t * 128 * (D + 2); };
+        float* part = slot(blockIdx.x, done.t0 == 0);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          tld32(tO + 32 * c, (uint32_t*)o);
+          tld_wait_regs((uint32_t*)o);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ((float4*)part)[(8 * c + i) * 128 + r] = *(float4*)(o + 4 * i);
+        }
+        part[D * 128 + r] = mine;
+        part[D * 128 + 128 + r] = l;
+        const int c0 = shares.owner(done.at + kCost), c1 = shares.owner(done.at + done.tiles + kCost - 1);
+        __threadfence();
+        if (!(ok = meet())) break;
+        if (r == 0) {
+          uint32_t* counter = a.counter + 2 * c0 + t;
+          last[t] = atomicAdd(counter, 1u) == (uint32_t)(c1 - c0);
+          if (last[t]) *counter = 0;
+          __threadfence();
+        }
+        if (!(ok = meet())) break;
+        if (last[t]) {
+          float top = kNone, total = 0.0f;
+          for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(slot(c, c == c0) + D * 128 + r));
+          for (int c = c0; c <= c1; ++c) {
+            const float* q = slot(c, c == c0) + D * 128 + r;
+            total = fmaf(exp2_(__ldcg(q) - top), __ldcg(q + 128), total);
+          }
+          const float scale = total != 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32] = {};
+            for (int b = c0; b <= c1; ++b) {
+              const float* q = slot(b, b == c0);
+              const float f = exp2_(__ldcg(q + D * 128 + r) - top);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 v = __ldcg((const float4*)q + (8 * c + i) * 128 + r);
+                o[4 * i] = fmaf(f, v.x, o[4 * i]), o[4 * i + 1] = fmaf(f, v.y, o[4 * i + 1]);
+                o[4 * i + 2] = fmaf(f, v.z, o[4 * i + 2]), o[4 * i + 3] = fmaf(f, v.w, o[4 * i + 3]);
+              }
+            }
+            if (live) write(c, o, scale);
+          }
+        }
+        if (!(ok = meet())) break;  // last[t] has been read
+      }
+      // O_t may be overwritten: the arrival at p_ready of the next segment's first tile comes after these reads
+      fence_before();
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+}  // namespace
+
+size_t rows_workspace(int head_dim, int sms) {
+  return (size_t)sms * 2 * (head_dim == 64 ? Tiles<2>::kSlot : Tiles<4>::kSlot) * sizeof(float);
+}
+
+void launch_rows(fopt_ctx* ctx, const AttnArgs& a, int head_dim, int sms) {
+  auto go = [&](auto kernel, int smem) {
+    cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cache attention shared memory");
+    kernel<<<sms, kRowThreads, smem, ctx->stream>>>(a);
+    launched(ctx, "cache attention");
+  };
+  if (head_dim == 64) go(rows_kernel<2>, Tiles<2>::kBytes);
+  else go(rows_kernel<4>, Tiles<4>::kBytes);
+}
+
+}  // namespace kv
+}  // namespace fopt
