@@ -165,6 +165,8 @@ class Storage:
     def _will_write(self) -> None:
         """Called before anything writes into this storage in place: lazy storages that read it
         take their values now."""
+        if not len(self._dependents):
+            return
         for d in list(self._dependents):
             d.ptr  # noqa: B018 (materialises)
         self._dependents = weakref.WeakSet()
@@ -694,40 +696,42 @@ class B200:
         return o
 
     # ---- rotary positions and the paged 4-bit cache (see kvcache.py) ----
+    # Called once a layer and token: the checks are plain comparisons and nothing is built per call.
     @staticmethod
-    def _rows(name: str, s: Storage, tokens: int, width: int, offset: int, stride: Optional[int]):
-        """(address, token stride) of `tokens` rows of `width` elements within a storage."""
-        stride = width if stride is None else stride
+    def _rows(name: str, s: Storage, tokens: int, width: int, offset: int, stride: int) -> int:
+        """The address of `tokens` rows of `width` bf16 or f32 elements within a storage."""
+        if s.dtype == "bf16":
+            size = 2
+        elif s.dtype == "f32":
+            size = 4
+        else:
+            raise ValueError(f"{name}: bf16 or f32 values")
         if offset < 0 or stride < width:
             raise ValueError(f"{name}: rows of {width} elements at offset {offset}, stride {stride}")
         if tokens and offset + (tokens - 1) * stride + width > s.n:
             raise ValueError(f"{name}: {tokens} rows of {width} elements exceed the storage's {s.n}")
-        return s.addr + offset * dtypes.BITS[s.dtype] // 8, stride
-
-    @staticmethod
-    def _indices(name: str, s: Storage, n: Optional[int] = None) -> int:
-        if s.dtype != "i32" or (n is not None and s.n != n):
-            raise ValueError(f"{name} must be i32" + (f" with {n} entries" if n is not None else ""))
-        return s.n
+        return s.ptr.value + offset * size
 
     def rotary(self, x: Storage, positions: Storage, rope, heads: int, head_dim: int = 128,
                out: Optional[Storage] = None, x_offset: int = 0, x_stride: Optional[int] = None) -> Storage:
         """Rotates the heads of each token by its position: x holds rows of `heads` x `head_dim` bf16 or
         f32 values (`x_stride` elements apart, from `x_offset` on), positions one i32 a row. The result is
         [tokens, heads, head_dim], in `out` if given; with `out` x itself, the rows are rotated in place."""
-        tokens = self._indices("rotary: positions", positions)
-        if x.dtype not in ("bf16", "f32"):
-            raise ValueError("rotary: bf16 or f32 values")
-        row = heads * head_dim
-        src, stride = self._rows("rotary", x, tokens, row, x_offset, x_stride)
+        if positions.dtype != "i32":
+            raise ValueError("rotary: positions must be i32")
+        tokens, row = positions.n, heads * head_dim
+        stride = row if x_stride is None else x_stride
+        src = self._rows("rotary", x, tokens, row, x_offset, stride)
         if out is None:
             out = Storage(self, x.dtype, tokens * row, zero=False)
         elif out.dtype != x.dtype or (out is not x and out.n != tokens * row):
             raise ValueError("rotary: the output is [tokens, heads, head_dim] of the input's type")
         out._will_write()
-        dst, dst_stride = (src, stride) if out is x else (out.addr, row)
-        check(_lib.lib().fopt_rotary(self.ctx, dst, src, _lib.DTYPES[x.dtype], positions.ptr, rope.handle, tokens,
-                                     heads, head_dim, stride, dst_stride), self.ctx)
+        dst, dst_stride = (src, stride) if out is x else (out.ptr, row)
+        st = _lib.lib().fopt_rotary(self.ctx, dst, src, _lib.DTYPES[x.dtype], positions.ptr, rope.handle, tokens, heads,
+                                    head_dim, stride, dst_stride)
+        if st:
+            check(st, self.ctx)
         return out
 
     def cache_append(self, cache, k: Storage, v: Storage, slots: Storage, positions: Optional[Storage] = None,
@@ -736,33 +740,43 @@ class B200:
         """Stores each token's keys (rotated by its position first when `rope` is given) and values, bf16
         or f32 rows of [cache.heads, cache.head_dim], at its slot (page * page_size + slot of the page;
         negative: no token). Two tokens of one call must not name one slot."""
-        tokens = self._indices("cache_append: slots", slots)
-        if rope is not None:
-            if positions is None:
-                raise ValueError("cache_append: a rotation needs positions")
-            self._indices("cache_append: positions", positions, tokens)
-        if k.dtype != v.dtype or k.dtype not in ("bf16", "f32"):
-            raise ValueError("cache_append: bf16 or f32 keys and values")
-        row = cache.heads * cache.head_dim
-        kp, ks = self._rows("cache_append: keys", k, tokens, row, k_offset, k_stride)
-        vp, vs = self._rows("cache_append: values", v, tokens, row, v_offset, v_stride)
+        tokens, row = slots.n, cache.heads * cache.head_dim
+        if slots.dtype != "i32":
+            raise ValueError("cache_append: slots must be i32")
+        if rope is not None and (positions is None or positions.dtype != "i32" or positions.n != tokens):
+            raise ValueError("cache_append: a rotation needs an i32 position for each token")
+        if k.dtype != v.dtype:
+            raise ValueError("cache_append: keys and values must have one type")
+        ks = row if k_stride is None else k_stride
+        vs = row if v_stride is None else v_stride
+        kp = self._rows("cache_append: keys", k, tokens, row, k_offset, ks)
+        vp = self._rows("cache_append: values", v, tokens, row, v_offset, vs)
         cache._will_write()
-        check(_lib.lib().fopt_cache_append(self.ctx, C.byref(cache.desc()), kp, vp, _lib.DTYPES[k.dtype], ks, vs,
-                                           slots.ptr, positions.ptr if rope is not None else None,
-                                           rope.handle if rope is not None else None, tokens), self.ctx)
+        st = _lib.lib().fopt_cache_append(self.ctx, cache.ref, kp, vp, _lib.DTYPES[k.dtype], ks, vs, slots.ptr,
+                                          None if rope is None else positions.ptr, None if rope is None else rope.handle,
+                                          tokens)
+        if st:
+            check(st, self.ctx)
 
     def cache_read(self, cache, slots: Storage, dtype: str = "bf16", out=None):
         """The keys and values stored at the slots, as two [slots, heads, head_dim] storages of `dtype`
         (or those of the pair `out`); rows of negative slots are left as they were (0 in new storages)."""
-        n = self._indices("cache_read: slots", slots)
+        n = slots.n
+        if slots.dtype != "i32":
+            raise ValueError("cache_read: slots must be i32")
         size = n * cache.heads * cache.head_dim
-        k, v = out if out is not None else (Storage(self, dtype, size), Storage(self, dtype, size))
-        if k.dtype != v.dtype or k.dtype not in ("bf16", "f32") or k.n != size or v.n != size:
+        if out is None:
+            if dtype not in ("bf16", "f32"):
+                raise ValueError("cache_read: bf16 or f32 values")
+            out = Storage(self, dtype, size), Storage(self, dtype, size)
+        k, v = out
+        if k.dtype != v.dtype or k.dtype not in ("bf16", "f32") or k.n != size or v.n != size or k is v:
             raise ValueError("cache_read: two bf16 or f32 outputs of [slots, heads, head_dim]")
         k._will_write()
         v._will_write()
-        check(_lib.lib().fopt_cache_read(self.ctx, k.ptr, v.ptr, _lib.DTYPES[k.dtype], C.byref(cache.desc()),
-                                         slots.ptr, n), self.ctx)
+        st = _lib.lib().fopt_cache_read(self.ctx, k.ptr, v.ptr, _lib.DTYPES[k.dtype], cache.ref, slots.ptr, n)
+        if st:
+            check(st, self.ctx)
         return k, v
 
     def cache_attention(self, q: Storage, cache, table: Storage, q_start: Storage, kv_len: Storage, heads: int,
@@ -771,23 +785,23 @@ class B200:
         the bf16 query rows q_start[b] .. q_start[b + 1] - 1 ([heads, head_dim] each) and kv_len[b] keys in
         the pages of its row of `table`. Causal: its queries are its last tokens. Rows behind the last
         sequence are left as they were (0 in a new output)."""
-        batch = self._indices("cache_attention: kv_len", kv_len)
-        self._indices("cache_attention: q_start", q_start, batch + 1)
-        entries = self._indices("cache_attention: table", table)
-        row = heads * cache.head_dim
+        batch, row = kv_len.n, heads * cache.head_dim
+        if not (kv_len.dtype == q_start.dtype == table.dtype == "i32") or q_start.n != batch + 1:
+            raise ValueError("cache_attention: i32 table, lengths and one more start than lengths")
+        if not batch or table.n % batch:
+            raise ValueError("cache_attention: the table has a row of equal length for each sequence")
         if q.dtype != "bf16" or row <= 0 or q.n % row:
             raise ValueError("cache_attention: bf16 queries of [tokens, heads, head_dim]")
-        if not batch or entries % batch:
-            raise ValueError("cache_attention: the table has a row of equal length for each sequence")
         if out is None:
             out = Storage(self, "bf16", q.n)
         elif out.dtype != "bf16" or out.n != q.n or out is q:
             raise ValueError("cache_attention: the output is another storage laid out as q")
         out._will_write()
-        sc = scale if scale is not None else cache.head_dim ** -0.5
-        check(_lib.lib().fopt_cache_attention(self.ctx, out.ptr, q.ptr, C.byref(cache.desc()), table.ptr, q_start.ptr,
-                                              kv_len.ptr, batch, q.n // row, entries // batch, heads, C.c_float(sc),
-                                              int(causal)), self.ctx)
+        st = _lib.lib().fopt_cache_attention(self.ctx, out.ptr, q.ptr, cache.ref, table.ptr, q_start.ptr, kv_len.ptr,
+                                             batch, q.n // row, table.n // batch, heads,
+                                             cache.head_dim ** -0.5 if scale is None else scale, 1 if causal else 0)
+        if st:
+            check(st, self.ctx)
         return out
 
     # ---- host transfers (backend/mod.rs:220-238) ----

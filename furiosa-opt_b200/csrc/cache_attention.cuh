@@ -25,6 +25,7 @@ struct AttnArgs {
   float* ws;          // partial results: two slots a block
   uint32_t* counter;  // arrivals at the segment that begins in a block; zero between launches
   int batch, tokens, width, hq, group;
+  FastDiv by_group;  // query row -> query token
   int long_rows;      // sequences with this many query rows per key head are rows_kernel's, others tokens_kernel's
   float scale;
   int causal;
@@ -52,8 +53,9 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
   return s;
 }
 // Keys that the sequence's query row sees (at most 0: none).
+__device__ __forceinline__ int token_of(const AttnArgs& a, int row) { return (int)fdiv(a.by_group, (uint32_t)row); }
 __device__ __forceinline__ int seen(const AttnArgs& a, const Seq& s, int row) {
-  return a.causal ? min(s.keys, s.keys - s.queries + row / a.group + 1) : s.keys;
+  return a.causal ? min(s.keys, s.keys - s.queries + token_of(a, row) + 1) : s.keys;
 }
 
 __device__ __forceinline__ long long quotient(long long a, long long b) {  // both >= 0; a 64-bit division takes long

@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -154,6 +155,24 @@ inline const char* bad_index_message(int code) {
     case kBadLength: return "a sequence length below 0 or past its table's pages";
     default: return "query starts that do not ascend within the tokens";
   }
+}
+
+// What a launch needs to know of its device and set for its kernel, once for each device.
+inline int sm_count(const fopt_ctx* ctx) {
+  static std::atomic<int> known[64];
+  int n = ctx->device < 64 ? known[ctx->device].load() : 0;
+  if (!n) {
+    cuda_check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, ctx->device), "SM count");
+    if (ctx->device < 64) known[ctx->device].store(n);
+  }
+  return n;
+}
+// Raises a kernel's dynamic shared memory limit. `done` belongs to the kernel: one bit for each device.
+inline void allow_shared(const fopt_ctx* ctx, std::atomic<uint64_t>& done, const void* kernel, int bytes) {
+  const uint64_t bit = ctx->device < 64 ? 1ull << ctx->device : 0;
+  if (done.load() & bit) return;
+  cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory limit");
+  done.fetch_or(bit);
 }
 
 // Makes the context's device current for a call and puts the caller's back.

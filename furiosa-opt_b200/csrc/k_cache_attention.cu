@@ -165,7 +165,7 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, const Seq& s, int 
   for (int nb = 0; nb < NB; ++nb) {
     const int r = row0 + nb * 8 + g;
     const bool live = r < s.rows;
-    const int token = live ? r / a.group : 0;
+    const int token = live ? token_of(a, r) : 0;
     const uint16_t* p = a.q + ((int64_t)(s.q0 + token) * a.hq + head * a.group + (live ? r - token * a.group : 0)) * D;
     uint4 w[NG];
     float top = 0.0f;
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
     auto write_row = [&](int r, int d, float4 v, float l) {  // channels d .. d + 3 of row r
       const int row = row0 + r;
       const float n = l != 0.0f ? 1.0f / l : 0.0f;  // a row that sees no key is 0
-      const int token = row / a.group;
+      const int token = token_of(a, row);
       *(uint2*)(a.o + ((int64_t)(s.q0 + token) * a.hq + head * a.group + row - token * a.group) * D + d) =
           make_uint2(bf16x2_rule(v.x * n, v.y * n), bf16x2_rule(v.z * n, v.w * n));
     };
@@ -634,8 +634,8 @@ size_t tokens_workspace(int sms) { return (size_t)sms * tokens_blocks<NG, NB>() 
 template <int NG, int NB>
 void launch_tokens(fopt_ctx* ctx, const AttnArgs& a, int sms) {
   using S = Shared<NG, NB>;
-  cuda_check(cudaFuncSetAttribute(tokens_kernel<NG, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes),
-             "cache attention shared memory");
+  static std::atomic<uint64_t> done;
+  allow_shared(ctx, done, (const void*)tokens_kernel<NG, NB>, S::kBytes);
   tokens_kernel<NG, NB><<<sms * tokens_blocks<NG, NB>(), kThreads, S::kBytes, ctx->stream>>>(a);
   launched(ctx, "cache attention");
 }
@@ -657,7 +657,7 @@ extern "C" fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* 
     require(table_width > 0, "fopt_cache_attention: an empty page table");
     require(hq > 0 && hq % cache->heads == 0, "fopt_cache_attention: query heads must be a multiple of the cache's heads");
     require(std::isfinite(scale), "fopt_cache_attention: the scale must be finite");
-    require((int64_t)tokens * (hq / cache->heads) <= INT32_MAX, "fopt_cache_attention: too many query rows");
+    require((int64_t)tokens * hq <= INT32_MAX, "fopt_cache_attention: too many query rows");
     if (ctx && (batch == 0 || tokens == 0)) return;
     require(o && q && table && q_start && kv_len, "fopt_cache_attention: null argument");
     require(((uintptr_t)o | (uintptr_t)q) % 16 == 0, "fopt_cache_attention: q and o must be 16-byte aligned");
@@ -674,10 +674,10 @@ extern "C" fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* 
     a.width = table_width;
     a.hq = hq;
     a.group = hq / cache->heads;
+    a.by_group = make_fastdiv((uint32_t)a.group);
     a.scale = scale;
     a.causal = causal != 0;
-    int sms = 0;
-    cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, ctx->device), "SM count");
+    const int sms = sm_count(ctx);
     require(sms * kv::kBlocks <= kv::kCounters, "fopt_cache_attention: more resident blocks than counters");
     const int dim = cache->head_dim;
     // Sequences of more than kv::kFewRows query rows go to rows_kernel, whose tiles of 256 rows take about as long

@@ -9,6 +9,9 @@
 //               value = code * step + offset as f16 into the 128-byte-swizzled tiles;
 //   warps 4-11  softmax: a thread per query row reads its scores from tensor memory, keeps the running maximum and
 //               sum, and writes P as f16 over the first half of its scores.
+// The roles' loops are short on purpose. They run side by side, and unrolled over a tile (500 to 600 instructions each)
+// they missed the instruction cache so often that an instruction took 10 cycles a warp; 16 softmax and 7 expanding
+// warps made it worse (a tile's softmax 1.75 -> 2.5 us).
 // While one tile's softmax runs the tensor cores work on the other. Every wait is bounded (2 s) and reports
 // through the context's error word.
 //
@@ -50,7 +53,8 @@ struct Tiles {
   static constexpr int kTile = kHalves * kHalf;      // Q_t, K or V
   // 2 Q, 2 stages of K and of V, the offset steps of Q and K, alignment, barriers and scales; more than half an
   // SM's, since a second block would only wait for tensor memory
-  static constexpr int kAll = 6 * kTile + 4 * kOffsets + 1024 + 512;
+  static constexpr int kRaw = 32 * (NG * 32 + NG * 8);  // what a warp holds of 32 tokens
+  static constexpr int kAll = 6 * kTile + 4 * kOffsets + 3 * kRaw + 1024 + 512;
   static constexpr int kBytes = kAll > 120000 ? kAll : 120000;
   static constexpr int kSlot = kRows * (D + 2);      // floats of a partial result
 };
@@ -156,6 +160,24 @@ __device__ __forceinline__ uint4 expand(const Masks& m, uint32_t x, uint32_t ste
   return make_uint4(low(x), high(x), low(y), high(y));
 }
 
+// Scores of keys from `left` on become -inf.
+__device__ __forceinline__ void hide(uint32_t* s, int left) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (i >= left) s[i] = 0xff800000u;
+}
+
+// Two outputs times `by` as bf16 under the library's rule (half to even, subnormals to signed zero, one NaN).
+__device__ __forceinline__ uint32_t rounded(float lo, float hi, float by) {
+  float x, y;
+  asm("mul.ftz.f32 %0, %1, %2;" : "=f"(x) : "f"(lo), "f"(by));
+  asm("mul.ftz.f32 %0, %1, %2;" : "=f"(y) : "f"(hi), "f"(by));
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+  // an output is NaN where its row's sum is, the whole row
+  return by == by ? r : 0x7fc07fc0u;
+}
+
 // Where chunk c (16 bytes) of row t of a tile is.
 __device__ __forceinline__ uint32_t place(int t, int c) { return (c >> 3) * kHalf + t * 128 + (((c & 7) ^ (t & 7)) << 4); }
 // ... and chunk c (0, 1) of row t of an offset step: unswizzled 8-row by 16-byte blocks, the two of a row group
@@ -170,41 +192,36 @@ __device__ __forceinline__ uint64_t offsets_desc(uint32_t addr) {
 }
 __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// What a lane that expands has in hand of one token.
-template <int NG>
-struct Row {
-  uint32_t k[4 * NG], v[4 * NG], ks[NG], vs[NG];
-};
-
 template <int N>
-__device__ __forceinline__ void load_row(uint32_t* w, const void* p) {
+__device__ __forceinline__ void load_row(uint32_t* w, const void* p, bool there) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = 0;
+  if (!there) return;
   if constexpr (N == 2) *(uint2*)w = __ldg((const uint2*)p);
 #pragma unroll
   for (int i = 0; i < N / 4; ++i) *(uint4*)(w + 4 * i) = __ldg((const uint4*)p + i);
 }
 
-template <int NG>
-__device__ __forceinline__ void load_token(const AttnArgs& a, const Item& it, int token, Row<NG>& r) {
-  bool there = false;
-  int64_t row = 0;
-  if (token < it.s.keys) {
+// A token's place: its page (looked up ahead of its row) and the row's number in the images. Past the keys, or of no
+// page: none, and zeros are what is read, whatever the slot holds.
+struct Spot {
+  int page, in_page;
+  bool inside;
+};
+__device__ __forceinline__ Spot spot_of(const AttnArgs& a, const Item& it, int token) {
+  Spot p{-1, 0, token < it.s.keys};
+  if (p.inside) {
     const int entry = (int)fdiv(a.cache.by_page, (uint32_t)token);
-    const int page = a.table[(int64_t)it.b * a.width + entry];
-    there = page >= 0 && page < a.cache.pages;
-    if (there) row = ((int64_t)page * a.cache.heads + it.head) * a.cache.page_size + (token - entry * a.cache.page_size);
-    else atomicExch(a.err, kBadPage);
+    p.page = a.table[(int64_t)it.b * a.width + entry];
+    p.in_page = token - entry * a.cache.page_size;
   }
-  if (there) {
-    load_row<4 * NG>(r.k, a.cache.k + row * (NG * 16));
-    load_row<4 * NG>(r.v, a.cache.v + row * (NG * 16));
-    load_row<NG>(r.ks, a.cache.k_scale + row * NG);
-    load_row<NG>(r.vs, a.cache.v_scale + row * NG);
-  } else {  // past the keys, or of no page: zeros, whatever the slot holds
-#pragma unroll
-    for (int i = 0; i < 4 * NG; ++i) r.k[i] = r.v[i] = 0;
-#pragma unroll
-    for (int i = 0; i < NG; ++i) r.ks[i] = r.vs[i] = 0;
-  }
+  return p;
+}
+__device__ __forceinline__ bool row_at(const AttnArgs& a, const Item& it, const Spot& p, int64_t& row) {
+  const bool there = p.page >= 0 && p.page < a.cache.pages;
+  if (p.inside && !there) atomicExch(a.err, kBadPage);
+  row = there ? ((int64_t)p.page * a.cache.heads + it.head) * a.cache.page_size + p.in_page : 0;
+  return there;
 }
 
 // The exponent that brings the largest of a warp's values to [2^4, 2^9), from the sizes of their groups.
@@ -229,7 +246,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
   uint8_t* sV = smem + 4 * T::kTile;
   uint8_t* sQz = smem + 6 * T::kTile;  // the offset steps: of tile t at sQz + t * kOffsets, of stage n at sKz + ...
   uint8_t* sKz = sQz + 2 * kOffsets;
-  uint64_t* bars = (uint64_t*)(sKz + 2 * kOffsets);
+  uint8_t* raw = sKz + 2 * kOffsets;   // rows as they are in the cache, of warps 1-3
+  uint64_t* bars = (uint64_t*)(raw + 3 * T::kRaw);
   uint64_t* k_full = bars;         // [2]
   uint64_t* k_empty = bars + 2;    // [2]
   uint64_t* v_full = bars + 4;     // [2]
@@ -296,7 +314,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       };
       int n = 0, seg = 0;  // key tiles and segments so far
       bool ok = true;
-      for (; ok && walk.next(it); ++seg) {
+      bool more = walk.next(it);
+      for (; ok && more; ++seg) {
         const int n1 = n + it.t1 - it.t0;
         ok = mbar_wait(smem_u32(&k_full[n & 1]), (n >> 1) & 1, abort_flag, a.err, 401);
         for (int t = 0; ok && t < 2; ++t) {
@@ -306,6 +325,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
           scores(t, n);
         }
         if (ok) commit(smem_u32(&k_empty[n & 1]));
+        more = walk.next(it);  // the next segment, while this one's scores are on their way
         for (int first = n; ok && n < n1; ++n) {
           for (int t = 0; ok && t < 2; ++t) {
             ok = (t || mbar_wait(smem_u32(&v_full[n & 1]), (n >> 1) & 1, abort_flag, a.err, 403)) &&
@@ -334,22 +354,52 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
     __syncwarp();
   } else if (warp <= 3) {
     const Masks m = masks();
-    Row<NG> r;
+    // The next row is on its way in registers while the current one is expanded from shared memory, where a loop can
+    // index it: [K's pieces of 16 bytes, then V's][lane]. A lane reads back what it wrote itself.
+    constexpr int kPieces = NG;
+    uint4* mine = (uint4*)(raw + (warp - 1) * T::kRaw) + lane;
+    uint4 next_codes[2 * kPieces];
+    uint32_t ks[NG], vs[NG];
+    auto load = [&](const Item& of, const Spot& at) {
+      int64_t row;
+      const bool there = row_at(a, of, at, row);
+      load_row<4 * NG>((uint32_t*)next_codes, a.cache.k + row * (NG * 16), there);
+      load_row<4 * NG>((uint32_t*)(next_codes + kPieces), a.cache.v + row * (NG * 16), there);
+      load_row<NG>(ks, a.cache.k_scale + row * NG, there);
+      load_row<NG>(vs, a.cache.v_scale + row * NG, there);
+    };
     int low_v = 0;
     bool fresh = true;  // the segment's first 32 tokens of this warp
     bool more = walk.next(it), ok = true;
     int t = more ? it.t0 : 0;
-    int q = warp - 1, n = 0;  // the quarter of its tile, and its tile's number, of the tokens in r
-    if (more) load_token<NG>(a, it, t * kKeys + q * 32 + lane, r);
+    int q = warp - 1, n = 0;  // the quarter of its tile, and its tile's number, of the tokens in hand
+    if (more) load(it, spot_of(a, it, t * kKeys + q * 32 + lane));
     while (more) {
-      const int ek = warp_exponent<NG>(r.ks);
-      int ev = warp_exponent<NG>(r.vs);
+      const int ek = warp_exponent<NG>(ks);
+      int ev = warp_exponent<NG>(vs);
       // V far below the segment's first is not brought up all the way: l would pass the f32 range
       if (fresh) low_v = ev - 40;
       ev = max(ev, low_v);
-      const Row<NG> now = r;
-      const int row = q * 32 + lane, tile = n;
-      // this warp's next row is on its way while this one is expanded
+      const int quarter = q, row = q * 32 + lane, tile = n;
+      // by code word of a piece: steps and offsets of what its pairs of codes are (see the loop)
+      uint32_t step[2][4], offset[2][4], z[8] = {};
+      const float kf = power(-ek), vf = power(-ev);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int g = NG == 4 ? w : w & 1, h = NG == 4 ? w & 1 : 0;
+        const float s = step_of(ks[g]) * kf;
+        step[0][w] = f16x2(s, s);
+        offset[0][w] = 0;
+        step[1][w] = f16x2(step_of(vs[2 * h]) * vf, step_of(vs[2 * h + 1]) * vf);
+        offset[1][w] = f16x2(offset_of(vs[2 * h]) * vf, offset_of(vs[2 * h + 1]) * vf);
+      }
+      // K's offsets: k = part * NG + group for the two parts of the sums of q, then zeros
+#pragma unroll
+      for (int j = 0; j < NG / 2; ++j)
+        z[j] = z[j + NG / 2] = f16x2(offset_of(ks[2 * j]) * kf, offset_of(ks[2 * j + 1]) * kf);
+#pragma unroll
+      for (int i = 0; i < 2 * kPieces; ++i) mine[i * 32] = next_codes[i];
+      // this warp's next tokens
       fresh = false;
       q += 3;
       if (q >= 4) {
@@ -361,53 +411,47 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
           t = it.t0;
         }
       }
-      if (more) load_token<NG>(a, it, t * kKeys + q * 32 + lane, r);
+      Spot next{-1, 0, false};
+      if (more) next = spot_of(a, it, t * kKeys + q * 32 + lane);
 
-      ok = mbar_wait(smem_u32(&k_empty[tile & 1]), ((tile >> 1) & 1) ^ 1, abort_flag, a.err, 411);
-      ok = __all_sync(0xffffffffu, ok);
+#pragma unroll 1
+      for (int v = 0; v < 2; ++v) {  // K, then V
+        uint64_t* empty = v ? &v_empty[tile & 1] : &k_empty[tile & 1];
+        ok = mbar_wait(smem_u32(empty), ((tile >> 1) & 1) ^ 1, abort_flag, a.err, 411);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (v == 0) {
+          if (lane == 0) {  // place tile % 4: the softmax of tile - 4 is over, or S of tile - 2 could not be
+            k_back[(tile & 3) * 4 + quarter] = power(ek);
+            v_up[(tile & 3) * 4 + quarter] = (float)ev;
+            mbar_arrive(smem_u32(&x_full[tile & 3]));
+          }
+          uint8_t* tz = sKz + (tile & 1) * kOffsets;
+          *(uint4*)(tz + offsets_place(row, 0)) = make_uint4(z[0], z[1], z[2], z[3]);
+          *(uint4*)(tz + offsets_place(row, 1)) = make_uint4(z[4], z[5], z[6], z[7]);
+        }
+        uint8_t* to = (v ? sV : sK) + (tile & 1) * T::kTile + row * 128;
+        const uint32_t s0 = step[v][0], s1 = step[v][1], s2 = step[v][2], s3 = step[v][3];
+        const uint32_t z0 = offset[v][0], z1 = offset[v][1], z2 = offset[v][2], z3 = offset[v][3];
+        // Word w of piece i is chunk: of K (words in the order of [D % 32 / 8, D / 32]) 4 group + run, of V its number.
+        const int by_piece = v ? 4 : NG == 4 ? 1 : 2;
+        const int c1 = v ? 1 : 4, c2 = v ? 2 : NG == 4 ? 8 : 1, c3 = v ? 3 : NG == 4 ? 12 : 5;
+        auto chunk_at = [&](int c) { return (uint4*)(to + (c >> 3) * kHalf + (((c & 7) ^ (row & 7)) << 4)); };
+#pragma unroll 1
+        for (int i = 0; i < kPieces; ++i) {
+          const uint4 w = mine[(v * kPieces + i) * 32];
+          const int c = i * by_piece;
+          *chunk_at(c) = expand(m, w.x, s0, z0);
+          *chunk_at(c + c1) = expand(m, w.y, s1, z1);
+          *chunk_at(c + c2) = expand(m, w.z, s2, z2);
+          *chunk_at(c + c3) = expand(m, w.w, s3, z3);
+        }
+        async_fence();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(v ? &v_full[tile & 1] : &k_full[tile & 1]));
+        if (v == 0) load(it, next);  // its page has come by now
+      }
       if (!ok) break;
-      if (lane == 0) {  // place tile % 4: the softmax of tile - 4 is over, or S of tile - 2 could not be
-        k_back[(tile & 3) * 4 + (row >> 5)] = power(ek);
-        v_up[(tile & 3) * 4 + (row >> 5)] = (float)ev;
-        mbar_arrive(smem_u32(&x_full[tile & 3]));
-      }
-      const float kf = power(-ek), vf = power(-ev);
-      uint8_t* tk = sK + (tile & 1) * T::kTile;
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        const float s = step_of(now.ks[j]) * kf;
-        const uint32_t s2 = f16x2(s, s);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *(uint4*)(tk + place(row, 4 * j + i)) = expand(m, now.k[i * NG + j], s2, 0u);
-      }
-      {  // k = part * NG + group for the two parts of the sums of q, then zeros
-        uint32_t z[8] = {};
-#pragma unroll
-        for (int j = 0; j < NG / 2; ++j)
-          z[j] = z[j + NG / 2] = f16x2(offset_of(now.ks[2 * j]) * kf, offset_of(now.ks[2 * j + 1]) * kf);
-        uint8_t* tz = sKz + (tile & 1) * kOffsets;
-        *(uint4*)(tz + offsets_place(row, 0)) = make_uint4(z[0], z[1], z[2], z[3]);
-        *(uint4*)(tz + offsets_place(row, 1)) = make_uint4(z[4], z[5], z[6], z[7]);
-      }
-      async_fence();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&k_full[tile & 1]));
-
-      ok = mbar_wait(smem_u32(&v_empty[tile & 1]), ((tile >> 1) & 1) ^ 1, abort_flag, a.err, 412);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      uint8_t* tv = sV + (tile & 1) * T::kTile;
-#pragma unroll
-      for (int j = 0; j < NG / 2; ++j) {  // words 2 g + j (NG = 4) of groups 2 j and 2 j + 1
-        const uint32_t s2 = f16x2(step_of(now.vs[2 * j]) * vf, step_of(now.vs[2 * j + 1]) * vf);
-        const uint32_t z2 = f16x2(offset_of(now.vs[2 * j]) * vf, offset_of(now.vs[2 * j + 1]) * vf);
-#pragma unroll
-        for (int g = 0; g < 8; ++g)
-          *(uint4*)(tv + place(row, g * (NG / 2) + j)) = expand(m, now.v[g * (NG / 2) + j], s2, z2);
-      }
-      async_fence();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&v_full[tile & 1]));
     }
   } else {
     const int t = (warp - 4) >> 2, quarter = warp & 3;  // tile, and the tensor-memory lanes that the warp may read
@@ -416,47 +460,66 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
     const uint32_t tS = tmem + t * 128 + lanes, tO = tmem + 256 + t * 128 + lanes;
     uint8_t* tq = sQ + t * T::kTile;
 
-    // writes the row's query into Q_t; returns the factor of its scores (K's powers of two aside)
+    // Rows of q and o (16 bytes a lane) start at their number * D.
+    auto number = [&](const Item& x, int row) -> int {
+      const int token = token_of(a, row);
+      return (x.s.q0 + token) * a.hq + x.head * a.group + row - token * a.group;
+    };
+    // Puts the warp's 32 queries into Q_t, NG * 4 lanes to a row: each chunk as f16 in its place, and the sums of its
+    // groups. Returns the factor of this thread's row's scores (K's powers of two aside).
+    constexpr int kPer = NG * 4, kAtOnce = 32 / kPer;  // lanes a row, rows at a time
     auto put_query = [&](const Item& x) -> float {
-      const int row = x.row0 + t * 128 + r;
-      uint32_t w[D / 2];
-      float top = 0.0f;
-      if (row < x.s.rows) {
-        const int token = row / a.group;
-        const uint4* p = (const uint4*)(a.q + ((int64_t)(x.s.q0 + token) * a.hq + x.head * a.group + row - token * a.group) * D);
+      const int chunk = lane % kPer, first = quarter * 32 + lane / kPer;
+      int exponent = 0;
+#pragma unroll 1
+      for (int k0 = 0; k0 < kPer; k0 += 4) {
+        uint4 w[4];
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) *(uint4*)(w + 4 * c) = __ldg(p + c);
-      } else {
-#pragma unroll
-        for (int c = 0; c < D / 2; ++c) w[c] = 0;
-      }
-#pragma unroll
-      for (int c = 0; c < D / 2; ++c) top = max3(top, fabsf(step_of(w[c])), fabsf(offset_of(w[c])));
-      const RowScale up(top);
-      float sum[NG] = {};  // of q as f16 holds it, by group
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[2 * e] = step_of(w[4 * c + e]) * up.up0 * up.up1;
-          v[2 * e + 1] = offset_of(w[4 * c + e]) * up.up0 * up.up1;
+        for (int k = 0; k < 4; ++k) {
+          const int row = x.row0 + t * 128 + first + (k0 + k) * kAtOnce;
+          w[k] = make_uint4(0, 0, 0, 0);
+          if (row < x.s.rows) w[k] = __ldg((const uint4*)(a.q + (int64_t)number(x, row) * D) + chunk);
         }
-        const uint4 h = make_uint4(f16x2(v[0], v[4]), f16x2(v[1], v[5]), f16x2(v[2], v[6]), f16x2(v[3], v[7]));
-        sum[c / 4] += (sum_of(h.x) + sum_of(h.y)) + (sum_of(h.z) + sum_of(h.w));
-        *(uint4*)(tq + place(r, c)) = h;
-      }
-      uint32_t z[8] = {};
 #pragma unroll
-      for (int j = 0; j < NG / 2; ++j) {
-        z[j] = f16x2(sum[2 * j], sum[2 * j + 1]);
-        z[j + NG / 2] = f16x2(sum[2 * j] - low_half(z[j]), sum[2 * j + 1] - high_half(z[j]));
+        for (int k = 0; k < 4; ++k) {
+          const int row = first + (k0 + k) * kAtOnce;
+          const uint32_t y[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+          uint32_t top = 0;  // of the magnitudes, as bf16 bits
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = __vmaxu2(top, y[e] & 0x7fff7fffu);
+          top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+          for (int o = 1; o < kPer; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const int e = max((int)(top >> 7) - 127, -118);  // largest in [2^e, 2^(e + 1)); below 2^-118 it stays smaller
+          // the scale's sign goes into q, so that the largest score is the largest product
+          const float up = a.scale < 0.0f ? -power(8 - e) : a.scale > 0.0f ? power(8 - e) : 0.0f;
+          float v[8];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            v[2 * c] = step_of(y[c]) * up;
+            v[2 * c + 1] = offset_of(y[c]) * up;
+          }
+          const uint4 h = make_uint4(f16x2(v[0], v[4]), f16x2(v[1], v[5]), f16x2(v[2], v[6]), f16x2(v[3], v[7]));
+          *(uint4*)(tq + place(row, chunk)) = h;
+          float sum = (sum_of(h.x) + sum_of(h.y)) + (sum_of(h.z) + sum_of(h.w));
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          // the sum's two f16 parts from the first two lanes of the group, zeros from the others: k = part * NG + group
+          const uint32_t one = f16x2(sum, 0.0f);
+          const uint32_t parts = chunk & 1 ? f16x2(sum - low_half(one), 0.0f) : one;
+          uint16_t* z = (uint16_t*)(sQz + t * kOffsets + offsets_place(row, 0));
+          const int at = (chunk & 3) * NG + (chunk >> 2);  // 0 .. 4 NG - 1
+          z[at < 8 ? at : 64 + at - 8] = (uint16_t)((chunk & 3) < 2 ? parts : 0u);
+          if (NG == 2) z[64 + at] = 0;
+          // row r's exponent goes to thread r
+          const int es = __shfl_sync(0xffffffffu, e, lane % kAtOnce * kPer);
+          if (lane / kAtOnce == k0 + k) exponent = es;
+        }
       }
-      *(uint4*)(sQz + t * kOffsets + offsets_place(r, 0)) = make_uint4(z[0], z[1], z[2], z[3]);
-      *(uint4*)(sQz + t * kOffsets + offsets_place(r, 1)) = make_uint4(z[4], z[5], z[6], z[7]);
       async_fence();
       mbar_arrive(smem_u32(&q_full[t]));
-      return scalbnf(a.scale * kLog2e, up.e - 8);
+      // not 0, so that a hidden key stays at -inf
+      return fmaxf(scalbnf(fabsf(a.scale) * kLog2e, exponent - 8), 0x1p-126f);
     };
 
     uint32_t meetings = 0;
@@ -466,179 +529,188 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       return __all_sync(0xffffffffu, here);
     };
     bool more = walk.next(it), ok = true;
-    float qs = more ? put_query(it) : 0.0f;
+    Item done;  // the segment whose output is still in O_t
+    float qs = 0.0f, m = 0.0f, l = 0.0f;
     int n = 0;
-    for (int seg = 0; more; ++seg) {
-      const int row = it.row0 + t * 128 + r;
-      const int limit = row < it.s.rows ? seen(a, it.s, row) : it.s.keys;  // rows past the last are not stored
-      float m = 0.0f, l = 0.0f;
-      for (int kt = it.t0; kt < it.t1; ++kt, ++n) {
+    // Each part stands here once, in one place: the roles' code together has to stay in the instruction cache.
+    for (int seg = 0; more || seg; ++seg) {
+      if (seg) {
+        ok = mbar_wait(smem_u32(&o_done[t]), (seg - 1) & 1, abort_flag, a.err, 423);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after();
+        const bool whole = done.t0 == 0 && done.t1 == done.tiles;
+        // partial results: [D / 4][128] float4, so that a warp's rows are contiguous, then maxima and sums
+        auto slot = [&](int block, bool begins) { return a.ws + ((int64_t)block * 2 + begins) * T::kSlot + t * 128 * (D + 2); };
+        int c0 = 0, c1 = 0;
+        float top = 0.0f, total = l;
+        bool output = true;
+        if (!whole) {
+          float* part = slot(blockIdx.x, done.t0 == 0);
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            tld32(tO + 32 * c, (uint32_t*)o);
+            tld_wait_regs((uint32_t*)o);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ((float4*)part)[(8 * c + i) * 128 + r] = *(float4*)(o + 4 * i);
+          }
+          part[D * 128 + r] = l > 0.0f ? m : l == l ? kNone : m;  // a NaN sum stays one
+          part[D * 128 + 128 + r] = l;
+          c0 = shares.owner(done.at + kCost);
+          c1 = shares.owner(done.at + done.tiles + kCost - 1);
+          __threadfence();
+          if (!(ok = meet())) break;
+          if (r == 0) {
+            uint32_t* counter = a.counter + 2 * c0 + t;
+            last[t] = atomicAdd(counter, 1u) == (uint32_t)(c1 - c0);
+            if (last[t]) *counter = 0;
+            __threadfence();
+          }
+          if (!(ok = meet())) break;
+          output = last[t];
+          if (!(ok = meet())) break;  // last[t] has been read
+          if (output) {
+            top = kNone;
+            total = 0.0f;
+#pragma unroll 4
+            for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(slot(c, c == c0) + D * 128 + r));
+#pragma unroll 4
+            for (int c = c0; c <= c1; ++c) {
+              const float* q = slot(c, c == c0) + D * 128 + r;
+              total = fmaf(exp2_(__ldcg(q) - top), __ldcg(q + 128), total);
+            }
+          }
+        }
+        if (output) {
+          // through the warp's rows of Q_t, whose scores are complete, so that it leaves in whole rows
+          const float scale = total != 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            if (whole) {
+              tld32(tO + 32 * c, (uint32_t*)o);
+              tld_wait_regs((uint32_t*)o);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+#pragma unroll 1
+              for (int b = c0; b <= c1; ++b) {
+                const float* q = slot(b, b == c0);
+                const float f = exp2_(__ldcg(q + D * 128 + r) - top);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const float4 v = __ldcg((const float4*)q + (8 * c + i) * 128 + r);
+                  o[4 * i] = fmaf(f, v.x, o[4 * i]), o[4 * i + 1] = fmaf(f, v.y, o[4 * i + 1]);
+                  o[4 * i + 2] = fmaf(f, v.z, o[4 * i + 2]), o[4 * i + 3] = fmaf(f, v.w, o[4 * i + 3]);
+                }
+              }
+            }
+            // 32 columns in the order of the codes -> 32 / NG neighbouring channels of each group
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+              uint32_t y[16 / NG];
+#pragma unroll
+              for (int i = 0; i < 16 / NG; ++i) {  // channels 2 i, 2 i + 1 of the run: code word 4 c + word, its codes e, e + 1
+                const int g = i / 2, word = g * (NG / 2) + j / 2, e = 2 * (i & 1);
+                y[i] = rounded(o[8 * word + 2 * e + (j & 1)], o[8 * word + 2 * e + 2 + (j & 1)], scale);
+              }
+#pragma unroll
+              for (int i = 0; i < 16 / NG / 4; ++i)
+                *(uint4*)(tq + place(r, j * 4 + c * (4 / NG) + i)) = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+            }
+          }
+          const int mine = done.row0 + t * 128 + r < done.s.rows ? number(done, done.row0 + t * 128 + r) : -1;
+          __syncwarp();
+#pragma unroll 4
+          for (int k = 0; k < kPer; ++k) {
+            const int row = k * kAtOnce + lane / kPer, chunk = lane % kPer;
+            const int to = __shfl_sync(0xffffffffu, mine, row);
+            if (to >= 0) ((uint4*)(a.o + (int64_t)to * D))[chunk] = *(const uint4*)(tq + place(quarter * 32 + row, chunk));
+          }
+          __syncwarp();
+        }
+        // O_t may be overwritten: the arrival at p_ready of the next segment's first tile comes after these reads
+        fence_before();
+      }
+      if (!more) break;
+      qs = put_query(it);
+      done = it;
+      more = walk.next(it);  // while the first scores are on their way
+      const int row = done.row0 + t * 128 + r;
+      const int limit = row < done.s.rows ? seen(a, done.s, row) : done.s.keys;  // rows past the last are not stored
+      m = l = 0.0f;
+      for (int kt = done.t0; kt < done.t1; ++kt, ++n) {
         ok = mbar_wait(smem_u32(&x_full[n & 3]), (n >> 2) & 1, abort_flag, a.err, 421) &&
              mbar_wait(smem_u32(&s_full[t]), n & 1, abort_flag, a.err, 422);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_after();
         const int left = limit - kt * kKeys;  // keys of the tile that the row sees
-        const bool cut = __any_sync(0xffffffffu, left < kKeys);
+        const bool cut = __any_sync(0xffffffffu, left < kKeys), first = kt == done.t0;
         const float* kb = k_back + (n & 3) * 4;
         const float* vu = v_up + (n & 3) * 4;
-        uint32_t p[64];
-        float sum, top;
-        auto pass = [&] {  // probabilities against the base m, their sum, and the largest x - m
-          sum = 0.0f;
-          top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t s[32];
-            tld32(tS + 32 * c, s);
-            tld_wait_regs(s);
-            const float f = qs * kb[c], up = vu[c] - m;
-            if (cut) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                s[i] = __float_as_uint(32 * c + i < left ? fmaf(__uint_as_float(s[i]), f, up) : -INFINITY);
-            } else {
-              const uint64_t f2 = pack_f32x2(f, f), up2 = pack_f32x2(up, up);
-#pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                float x0, x1;
-                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, up2), x0, x1);
-                s[i] = __float_as_uint(x0);
-                s[i + 1] = __float_as_uint(x1);
-              }
-            }
-            uint64_t part[2] = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float x0 = __uint_as_float(s[i]), x1 = __uint_as_float(s[i + 1]);
-              top = max3(top, x0, x1);
-              const float p0 = exp2_(x0), p1 = exp2_(x1);
-              part[(i >> 1) & 1] = add_f32x2(part[(i >> 1) & 1], pack_f32x2(p0, p1));
-              p[16 * c + (i >> 1)] = f16x2(p0, p1);
-            }
-            float s0, s1, s2, s3;
-            unpack_f32x2(part[0], s0, s1);
-            unpack_f32x2(part[1], s2, s3);
-            sum = fmaf((s0 + s1) + (s2 + s3), exp2_(-vu[c]), sum);
-          }
-        };
-        pass();
-        const bool first = kt == it.t0;
-        if (__any_sync(0xffffffffu, first || top > kLazy)) {
-          const float by = first ? (top == -INFINITY ? 0.0f : top) : top > kLazy ? top : 0.0f;
-          m += by;
-          if (!first) {  // S_t was issued behind the last O_t += P_t V: it is complete
-            const float f = exp2_(-by);
-            l *= f;
+        // the largest x, then the base: it moves when x exceeds it by 2^8
+        float top = -INFINITY;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tld32(tO + 32 * c, o);
-              tld_wait_regs(o);
+        for (int c = 0; c < 4; ++c) {
+          uint32_t s[32];
+          tld32(tS + 32 * c, s);
+          tld_wait_regs(s);
+          if (cut) hide(s, left - 32 * c);
+          float high[2] = {__uint_as_float(s[0]), __uint_as_float(s[1])};
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tst32(tO + 32 * c, o);
-            }
+          for (int i = 2; i < 30; i += 4) {
+            high[0] = max3(high[0], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+            high[1] = max3(high[1], __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
           }
-          pass();
+          high[0] = max3(high[0], __uint_as_float(s[30]), __uint_as_float(s[31]));
+          top = fmaxf(top, fmaf(fmaxf(high[0], high[1]), qs * kb[c], vu[c]));
         }
-        l += sum;
-        tst32(tS, p);
-        tst32(tS + 32, p + 32);
+        const float base = first ? (top == -INFINITY ? 0.0f : top) : top > m + kLazy ? top : m;
+        if (!first && __any_sync(0xffffffffu, base != m)) {
+          // S_t was issued behind the last O_t += P_t V: it is complete
+          const float f = exp2_(m - base);
+          l *= f;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tld32(tO + 32 * c, o);
+            tld_wait_regs(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tst32(tO + 32 * c, o);
+          }
+        }
+        m = base;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {  // P goes over columns whose scores have been read: 16 c .. 16 c + 15
+          uint32_t s[32], p[16];
+          tld32(tS + 32 * c, s);
+          tld_wait_regs(s);
+          if (cut) hide(s, left - 32 * c);
+          const float f = qs * kb[c], up = vu[c] - m;
+          const uint64_t f2 = pack_f32x2(f, f), up2 = pack_f32x2(up, up);
+          uint64_t part[2] = {0, 0};
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x0, x1;
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, up2), x0, x1);
+            const float p0 = exp2_(x0), p1 = exp2_(x1);
+            part[(i >> 1) & 1] = add_f32x2(part[(i >> 1) & 1], pack_f32x2(p0, p1));
+            p[i >> 1] = f16x2(p0, p1);
+          }
+          tst16(tS + 16 * c, p);
+          float s0, s1, s2, s3;
+          unpack_f32x2(part[0], s0, s1);
+          unpack_f32x2(part[1], s2, s3);
+          l = fmaf((s0 + s1) + (s2 + s3), exp2_(-vu[c]), l);
+        }
         tst_wait();
         fence_before();
         mbar_arrive(smem_u32(&p_ready[t]));
       }
       if (!ok) break;
-      // the last scores are complete, so Q_t is free: the next segment's goes in before this one's output
-      const Item done = it;
-      more = walk.next(it);
-      if (more) qs = put_query(it);
-      ok = mbar_wait(smem_u32(&o_done[t]), seg & 1, abort_flag, a.err, 423);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      fence_after();
-
-      const bool live = row < done.s.rows;
-      const int token = live ? row / a.group : 0;
-      uint16_t* out = a.o + ((int64_t)(done.s.q0 + token) * a.hq + done.head * a.group + (live ? row - token * a.group : 0)) * D;
-      // 32 columns in the order of the codes -> 32 / NG neighbouring channels of each group
-      auto write = [&](int c, const float* o, float scale) {
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          uint32_t w[16 / NG];
-#pragma unroll
-          for (int i = 0; i < 16 / NG; ++i) {  // channels 2 i, 2 i + 1 of the run: code word 4 c + word, its codes e, e + 1
-            const int g = i / 2, word = g * (NG / 2) + j / 2, e = 2 * (i & 1);
-            w[i] = bf16x2_rule(o[8 * word + 2 * e + (j & 1)] * scale, o[8 * word + 2 * e + 2 + (j & 1)] * scale);
-          }
-#pragma unroll
-          for (int i = 0; i < 16 / NG / 4; ++i)
-            *(uint4*)(out + j * kGroup + c * (32 / NG) + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        }
-      };
-      const float mine = l > 0.0f ? m : l == l ? kNone : m;  // a NaN sum stays one
-      if (done.t0 == 0 && done.t1 == done.tiles) {
-        const float scale = l != 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          float o[32];
-          tld32(tO + 32 * c, (uint32_t*)o);
-          tld_wait_regs((uint32_t*)o);
-          if (live) write(c, o, scale);
-        }
-      } else {
-        // [D / 4][128] float4, so that a warp's rows are contiguous; then maxima and sums
-        auto slot = [&](int block, bool begins) { return a.ws + ((int64_t)block * 2 + begins) * T::kSlot + t * 128 * (D + 2); };
-        float* part = slot(blockIdx.x, done.t0 == 0);
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          float o[32];
-          tld32(tO + 32 * c, (uint32_t*)o);
-          tld_wait_regs((uint32_t*)o);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) ((float4*)part)[(8 * c + i) * 128 + r] = *(float4*)(o + 4 * i);
-        }
-        part[D * 128 + r] = mine;
-        part[D * 128 + 128 + r] = l;
-        const int c0 = shares.owner(done.at + kCost), c1 = shares.owner(done.at + done.tiles + kCost - 1);
-        __threadfence();
-        if (!(ok = meet())) break;
-        if (r == 0) {
-          uint32_t* counter = a.counter + 2 * c0 + t;
-          last[t] = atomicAdd(counter, 1u) == (uint32_t)(c1 - c0);
-          if (last[t]) *counter = 0;
-          __threadfence();
-        }
-        if (!(ok = meet())) break;
-        if (last[t]) {
-          float top = kNone, total = 0.0f;
-          for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(slot(c, c == c0) + D * 128 + r));
-          for (int c = c0; c <= c1; ++c) {
-            const float* q = slot(c, c == c0) + D * 128 + r;
-            total = fmaf(exp2_(__ldcg(q) - top), __ldcg(q + 128), total);
-          }
-          const float scale = total != 0.0f ? 1.0f / total : 0.0f;
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            float o[32] = {};
-            for (int b = c0; b <= c1; ++b) {
-              const float* q = slot(b, b == c0);
-              const float f = exp2_(__ldcg(q + D * 128 + r) - top);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 v = __ldcg((const float4*)q + (8 * c + i) * 128 + r);
-                o[4 * i] = fmaf(f, v.x, o[4 * i]), o[4 * i + 1] = fmaf(f, v.y, o[4 * i + 1]);
-                o[4 * i + 2] = fmaf(f, v.z, o[4 * i + 2]), o[4 * i + 3] = fmaf(f, v.w, o[4 * i + 3]);
-              }
-            }
-            if (live) write(c, o, scale);
-          }
-        }
-        if (!(ok = meet())) break;  // last[t] has been read
-      }
-      // O_t may be overwritten: the arrival at p_ready of the next segment's first tile comes after these reads
-      fence_before();
     }
   }
   fence_before();
@@ -654,8 +726,9 @@ size_t rows_workspace(int head_dim, int sms) {
 }
 
 void launch_rows(fopt_ctx* ctx, const AttnArgs& a, int head_dim, int sms) {
+  static std::atomic<uint64_t> done[2];
   auto go = [&](auto kernel, int smem) {
-    cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cache attention shared memory");
+    allow_shared(ctx, done[head_dim == 64], (const void*)kernel, smem);
     kernel<<<sms, kRowThreads, smem, ctx->stream>>>(a);
     launched(ctx, "cache attention");
   };

@@ -156,6 +156,25 @@ __device__ __forceinline__ void tld_wait_regs(uint32_t* r) {
                : "memory");
 }
 #undef T32
+// 16 columns, and the wait for them.
+#define R16(i) "=r"(r[i])
+__device__ __forceinline__ void tld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : R16(0), R16(1), R16(2), R16(3), R16(4), R16(5), R16(6), R16(7), R16(8), R16(9), R16(10), R16(11), R16(12),
+        R16(13), R16(14), R16(15)
+      : "r"(taddr));
+}
+#undef R16
+#define T16(i) "+r"(r[i])
+__device__ __forceinline__ void tld_wait_regs16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : T16(0), T16(1), T16(2), T16(3), T16(4), T16(5), T16(6), T16(7), T16(8), T16(9), T16(10), T16(11),
+                 T16(12), T16(13), T16(14), T16(15)
+               :
+               : "memory");
+}
+#undef T16
 __device__ __forceinline__ void tld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tst_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void mma_bf16_ta(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {

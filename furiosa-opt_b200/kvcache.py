@@ -101,16 +101,16 @@ class PagedCache:
         self.k, self.v = Storage(be, "i4", n), Storage(be, "i4", n)
         self.k_scale, self.v_scale = Storage(be, "bf16", n // GROUP * 2), Storage(be, "bf16", n // GROUP * 2)
 
+        self._images = self.k, self.v, self.k_scale, self.v_scale
+        self._desc = _lib.PagedCacheDesc(*(s.addr for s in self._images), pages, page_size, heads, head_dim)
+        self.ref = C.byref(self._desc)  # what the entry points take
+
     @property
     def slots(self) -> int:
         return self.pages * self.page_size
 
-    def desc(self) -> _lib.PagedCacheDesc:
-        return _lib.PagedCacheDesc(self.k.addr, self.v.addr, self.k_scale.addr, self.v_scale.addr, self.pages,
-                                   self.page_size, self.heads, self.head_dim)
-
     def _will_write(self) -> None:
-        for s in (self.k, self.v, self.k_scale, self.v_scale):
+        for s in self._images:
             s._will_write()
 
 
