@@ -660,7 +660,8 @@ extern "C" fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* 
     require((int64_t)tokens * hq <= INT32_MAX, "fopt_cache_attention: too many query rows");
     if (ctx && (batch == 0 || tokens == 0)) return;
     require(o && q && table && q_start && kv_len, "fopt_cache_attention: null argument");
-    require(((uintptr_t)o | (uintptr_t)q) % 16 == 0, "fopt_cache_attention: q and o must be 16-byte aligned");
+    require((uintptr_t)o % 32 == 0 && (uintptr_t)q % 16 == 0,
+            "fopt_cache_attention: q must be 16-byte and o 32-byte aligned");
     require(ctx != nullptr, "null context");
     DeviceGuard guard(ctx);
     a.o = (uint16_t*)o;

@@ -2,16 +2,15 @@
 // fifth-generation tensor cores.
 //
 // The query rows of one key head are (token, query head of its group) pairs; a segment is 256 of them, as two
-// 128-row tiles, against all keys that they see, in tiles of 128 tokens. 384 threads, one block an SM:
+// 128-row tiles, against all keys that they see, in tiles of 128 tokens. 512 threads, one block an SM:
 //   warp 0      owns tensor memory and issues, per key tile, S_t = Q_t K^T and O_t += P_t V for t = 0, 1;
-//   warps 1-3   expand codes, in turn 32 tokens each: a lane takes one token, reads its row of K and of V straight
-//               from the cache's pages (64 contiguous bytes at D = 128) ahead of its turn, and writes
-//               value = code * step + offset as f16 into the 128-byte-swizzled tiles;
-//   warps 4-11  softmax: a thread per query row reads its scores from tensor memory, keeps the running maximum and
+//   warps 1-7   expand codes, in turn K or V of 32 tokens: a lane takes one token, reads its row straight from the
+//               cache's pages (64 contiguous bytes at D = 128) ahead of its turn, and writes it as f16 into the
+//               128-byte-swizzled tile (three warps took longer than a tile's products);
+//   warps 8-15  softmax: a thread per query row reads its scores from tensor memory, keeps the running maximum and
 //               sum, and writes P as f16 over the first half of its scores.
 // The roles' loops are short on purpose. They run side by side, and unrolled over a tile (500 to 600 instructions each)
-// they missed the instruction cache so often that an instruction took 10 cycles a warp; 16 softmax and 7 expanding
-// warps made it worse (a tile's softmax 1.75 -> 2.5 us).
+// they missed the instruction cache so often that an instruction took 10 cycles a warp, the more the more warps.
 // While one tile's softmax runs the tensor cores work on the other. Every wait is bounded (2 s) and reports
 // through the context's error word.
 //
@@ -40,7 +39,7 @@ namespace {
 using namespace attn;
 
 constexpr int kRows = 256, kKeys = 128;  // of a segment and of a tile
-constexpr int kRowThreads = 384;     // 168 registers each
+constexpr int kExpand = 7, kRowThreads = 32 * (1 + kExpand + 8);  // warps that expand codes; 128 registers a thread
 constexpr int kHalf = 16384;             // 128 rows of 64 f16 (128 bytes), the unit of the swizzled tiles
 constexpr int kOffsets = 128 * 32;        // 128 rows of 16 f16: the sums of a tile's q, or the offsets of a key tile
 constexpr int kCost = 2;                 // key tiles that beginning and ending a segment takes as long as
@@ -53,8 +52,8 @@ struct Tiles {
   static constexpr int kTile = kHalves * kHalf;      // Q_t, K or V
   // 2 Q, 2 stages of K and of V, the offset steps of Q and K, alignment, barriers and scales; more than half an
   // SM's, since a second block would only wait for tensor memory
-  static constexpr int kRaw = 32 * (NG * 32 + NG * 8);  // what a warp holds of 32 tokens
-  static constexpr int kAll = 6 * kTile + 4 * kOffsets + 3 * kRaw + 1024 + 512;
+  static constexpr int kRaw = 32 * NG * 16;  // what a warp holds of 32 tokens' K or V
+  static constexpr int kAll = 6 * kTile + 4 * kOffsets + kExpand * kRaw + 1024 + 512;
   static constexpr int kBytes = kAll > 120000 ? kAll : 120000;
   static constexpr int kSlot = kRows * (D + 2);      // floats of a partial result
 };
@@ -178,6 +177,12 @@ __device__ __forceinline__ uint32_t rounded(float lo, float hi, float by) {
   return by == by ? r : 0x7fc07fc0u;
 }
 
+__device__ __forceinline__ void store32(void* p, const uint32_t* y) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]),
+               "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7])
+               : "memory");
+}
+
 // Where chunk c (16 bytes) of row t of a tile is.
 __device__ __forceinline__ uint32_t place(int t, int c) { return (c >> 3) * kHalf + t * 128 + (((c & 7) ^ (t & 7)) << 4); }
 // ... and chunk c (0, 1) of row t of an offset step: unswizzled 8-row by 16-byte blocks, the two of a row group
@@ -246,8 +251,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
   uint8_t* sV = smem + 4 * T::kTile;
   uint8_t* sQz = smem + 6 * T::kTile;  // the offset steps: of tile t at sQz + t * kOffsets, of stage n at sKz + ...
   uint8_t* sKz = sQz + 2 * kOffsets;
-  uint8_t* raw = sKz + 2 * kOffsets;   // rows as they are in the cache, of warps 1-3
-  uint64_t* bars = (uint64_t*)(raw + 3 * T::kRaw);
+  uint8_t* raw = sKz + 2 * kOffsets;   // rows as they are in the cache, of warps 1-7
+  uint64_t* bars = (uint64_t*)(raw + kExpand * T::kRaw);
   uint64_t* k_full = bars;         // [2]
   uint64_t* k_empty = bars + 2;    // [2]
   uint64_t* v_full = bars + 4;     // [2]
@@ -281,7 +286,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       mbar_init(smem_u32(&o_done[i]), 1);
       mbar_init(smem_u32(&met[i]), 128);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&x_full[i]), 4);
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&x_full[i]), 8);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -352,58 +357,57 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       }
     }
     __syncwarp();
-  } else if (warp <= 3) {
+  } else if (warp <= kExpand) {
     const Masks m = masks();
     // The next row is on its way in registers while the current one is expanded from shared memory, where a loop can
-    // index it: [K's pieces of 16 bytes, then V's][lane]. A lane reads back what it wrote itself.
-    constexpr int kPieces = NG;
+    // index it: [piece of 16 bytes][lane]. A lane reads back what it wrote itself.
     uint4* mine = (uint4*)(raw + (warp - 1) * T::kRaw) + lane;
-    uint4 next_codes[2 * kPieces];
-    uint32_t ks[NG], vs[NG];
-    auto load = [&](const Item& of, const Spot& at) {
-      int64_t row;
-      const bool there = row_at(a, of, at, row);
-      load_row<4 * NG>((uint32_t*)next_codes, a.cache.k + row * (NG * 16), there);
-      load_row<4 * NG>((uint32_t*)(next_codes + kPieces), a.cache.v + row * (NG * 16), there);
-      load_row<NG>(ks, a.cache.k_scale + row * NG, there);
-      load_row<NG>(vs, a.cache.v_scale + row * NG, there);
-    };
+    uint4 codes[NG];
+    uint32_t scales[NG];
     int low_v = 0;
-    bool fresh = true;  // the segment's first 32 tokens of this warp
+    bool fresh = true;  // the segment's first V of this warp
     bool more = walk.next(it), ok = true;
     int t = more ? it.t0 : 0;
-    int q = warp - 1, n = 0;  // the quarter of its tile, and its tile's number, of the tokens in hand
-    if (more) load(it, spot_of(a, it, t * kKeys + q * 32 + lane));
+    int u = warp - 1, n = 0;  // which of a tile's eight turns (K of its quarters, then V), and the tile's number
+    auto load = [&](const Spot& at) {
+      int64_t row;
+      const bool there = row_at(a, it, at, row);
+      load_row<4 * NG>((uint32_t*)codes, (u < 4 ? a.cache.k : a.cache.v) + row * (NG * 16), there);
+      load_row<NG>(scales, (u < 4 ? a.cache.k_scale : a.cache.v_scale) + row * NG, there);
+    };
+    if (more) load(spot_of(a, it, t * kKeys + (u & 3) * 32 + lane));
     while (more) {
-      const int ek = warp_exponent<NG>(ks);
-      int ev = warp_exponent<NG>(vs);
-      // V far below the segment's first is not brought up all the way: l would pass the f32 range
-      if (fresh) low_v = ev - 40;
-      ev = max(ev, low_v);
-      const int quarter = q, row = q * 32 + lane, tile = n;
+      const bool is_v = u >= 4;
+      const int quarter = u & 3, row = quarter * 32 + lane, stage = n & 1, at4 = (n & 3) * 4 + quarter;
+      const uint32_t full = smem_u32(is_v ? &v_full[stage] : &k_full[stage]);
+      const uint32_t empty = smem_u32(is_v ? &v_empty[stage] : &k_empty[stage]), parity = ((n >> 1) & 1) ^ 1;
+      const uint32_t known = smem_u32(&x_full[n & 3]);
+      int e = warp_exponent<NG>(scales);
+      if (is_v) {  // V far below the segment's first is not brought up all the way: l would pass the f32 range
+        if (fresh) low_v = e - 40;
+        fresh = false;
+        e = max(e, low_v);
+      }
+      const float f = power(-e);
       // by code word of a piece: steps and offsets of what its pairs of codes are (see the loop)
-      uint32_t step[2][4], offset[2][4], z[8] = {};
-      const float kf = power(-ek), vf = power(-ev);
+      uint32_t step[4], offset[4], z[8] = {};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const int g = NG == 4 ? w : w & 1, h = NG == 4 ? w & 1 : 0;
-        const float s = step_of(ks[g]) * kf;
-        step[0][w] = f16x2(s, s);
-        offset[0][w] = 0;
-        step[1][w] = f16x2(step_of(vs[2 * h]) * vf, step_of(vs[2 * h + 1]) * vf);
-        offset[1][w] = f16x2(offset_of(vs[2 * h]) * vf, offset_of(vs[2 * h + 1]) * vf);
+        const float s = step_of(scales[g]) * f;
+        step[w] = is_v ? f16x2(step_of(scales[2 * h]) * f, step_of(scales[2 * h + 1]) * f) : f16x2(s, s);
+        offset[w] = is_v ? f16x2(offset_of(scales[2 * h]) * f, offset_of(scales[2 * h + 1]) * f) : 0;
       }
       // K's offsets: k = part * NG + group for the two parts of the sums of q, then zeros
 #pragma unroll
       for (int j = 0; j < NG / 2; ++j)
-        z[j] = z[j + NG / 2] = f16x2(offset_of(ks[2 * j]) * kf, offset_of(ks[2 * j + 1]) * kf);
+        z[j] = z[j + NG / 2] = f16x2(offset_of(scales[2 * j]) * f, offset_of(scales[2 * j + 1]) * f);
 #pragma unroll
-      for (int i = 0; i < 2 * kPieces; ++i) mine[i * 32] = next_codes[i];
-      // this warp's next tokens
-      fresh = false;
-      q += 3;
-      if (q >= 4) {
-        q -= 4;
+      for (int i = 0; i < NG; ++i) mine[i * 32] = codes[i];
+      // the next turn: its page is looked up while this one's row is expanded
+      u += kExpand;
+      if (u >= 8) {
+        u -= 8;
         ++n;
         if (++t == it.t1) {
           fresh = true;
@@ -412,49 +416,42 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         }
       }
       Spot next{-1, 0, false};
-      if (more) next = spot_of(a, it, t * kKeys + q * 32 + lane);
+      if (more) next = spot_of(a, it, t * kKeys + (u & 3) * 32 + lane);
 
-#pragma unroll 1
-      for (int v = 0; v < 2; ++v) {  // K, then V
-        uint64_t* empty = v ? &v_empty[tile & 1] : &k_empty[tile & 1];
-        ok = mbar_wait(smem_u32(empty), ((tile >> 1) & 1) ^ 1, abort_flag, a.err, 411);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (v == 0) {
-          if (lane == 0) {  // place tile % 4: the softmax of tile - 4 is over, or S of tile - 2 could not be
-            k_back[(tile & 3) * 4 + quarter] = power(ek);
-            v_up[(tile & 3) * 4 + quarter] = (float)ev;
-            mbar_arrive(smem_u32(&x_full[tile & 3]));
-          }
-          uint8_t* tz = sKz + (tile & 1) * kOffsets;
-          *(uint4*)(tz + offsets_place(row, 0)) = make_uint4(z[0], z[1], z[2], z[3]);
-          *(uint4*)(tz + offsets_place(row, 1)) = make_uint4(z[4], z[5], z[6], z[7]);
-        }
-        uint8_t* to = (v ? sV : sK) + (tile & 1) * T::kTile + row * 128;
-        const uint32_t s0 = step[v][0], s1 = step[v][1], s2 = step[v][2], s3 = step[v][3];
-        const uint32_t z0 = offset[v][0], z1 = offset[v][1], z2 = offset[v][2], z3 = offset[v][3];
-        // Word w of piece i is chunk: of K (words in the order of [D % 32 / 8, D / 32]) 4 group + run, of V its number.
-        const int by_piece = v ? 4 : NG == 4 ? 1 : 2;
-        const int c1 = v ? 1 : 4, c2 = v ? 2 : NG == 4 ? 8 : 1, c3 = v ? 3 : NG == 4 ? 12 : 5;
-        auto chunk_at = [&](int c) { return (uint4*)(to + (c >> 3) * kHalf + (((c & 7) ^ (row & 7)) << 4)); };
-#pragma unroll 1
-        for (int i = 0; i < kPieces; ++i) {
-          const uint4 w = mine[(v * kPieces + i) * 32];
-          const int c = i * by_piece;
-          *chunk_at(c) = expand(m, w.x, s0, z0);
-          *chunk_at(c + c1) = expand(m, w.y, s1, z1);
-          *chunk_at(c + c2) = expand(m, w.z, s2, z2);
-          *chunk_at(c + c3) = expand(m, w.w, s3, z3);
-        }
-        async_fence();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(v ? &v_full[tile & 1] : &k_full[tile & 1]));
-        if (v == 0) load(it, next);  // its page has come by now
-      }
+      ok = mbar_wait(empty, parity, abort_flag, a.err, 411);
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      if (lane == 0) {  // place n % 4: the softmax of tile n - 4 is over, or the product of n - 2 could not be
+        if (is_v) v_up[at4] = (float)e;
+        else k_back[at4] = power(e);
+        mbar_arrive(known);
+      }
+      if (!is_v) {
+        uint8_t* tz = sKz + stage * kOffsets;
+        *(uint4*)(tz + offsets_place(row, 0)) = make_uint4(z[0], z[1], z[2], z[3]);
+        *(uint4*)(tz + offsets_place(row, 1)) = make_uint4(z[4], z[5], z[6], z[7]);
+      }
+      uint8_t* to = (is_v ? sV : sK) + stage * T::kTile + row * 128;
+      // Word w of piece i is chunk: of K (words in the order of [D % 32 / 8, D / 32]) 4 group + run, of V its number.
+      const int by_piece = is_v ? 4 : NG == 4 ? 1 : 2;
+      const int c1 = is_v ? 1 : 4, c2 = is_v ? 2 : NG == 4 ? 8 : 1, c3 = is_v ? 3 : NG == 4 ? 12 : 5;
+      auto chunk_at = [&](int c) { return (uint4*)(to + (c >> 3) * kHalf + (((c & 7) ^ (row & 7)) << 4)); };
+#pragma unroll 1
+      for (int i = 0; i < NG; ++i) {
+        const uint4 w = mine[i * 32];
+        const int c = i * by_piece;
+        *chunk_at(c) = expand(m, w.x, step[0], offset[0]);
+        *chunk_at(c + c1) = expand(m, w.y, step[1], offset[1]);
+        *chunk_at(c + c2) = expand(m, w.z, step[2], offset[2]);
+        *chunk_at(c + c3) = expand(m, w.w, step[3], offset[3]);
+      }
+      load(next);
+      async_fence();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full);
     }
   } else {
-    const int t = (warp - 4) >> 2, quarter = warp & 3;  // tile, and the tensor-memory lanes that the warp may read
+    const int t = (warp - 8) >> 2, quarter = warp & 3;  // tile, and the tensor-memory lanes that the warp may read
     const int r = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem + t * 128 + lanes, tO = tmem + 256 + t * 128 + lanes;
@@ -465,61 +462,67 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       const int token = token_of(a, row);
       return (x.s.q0 + token) * a.hq + x.head * a.group + row - token * a.group;
     };
-    // Puts the warp's 32 queries into Q_t, NG * 4 lanes to a row: each chunk as f16 in its place, and the sums of its
-    // groups. Returns the factor of this thread's row's scores (K's powers of two aside).
     constexpr int kPer = NG * 4, kAtOnce = 32 / kPer;  // lanes a row, rows at a time
-    auto put_query = [&](const Item& x) -> float {
-      const int chunk = lane % kPer, first = quarter * 32 + lane / kPer;
-      int exponent = 0;
-#pragma unroll 1
-      for (int k0 = 0; k0 < kPer; k0 += 4) {
-        uint4 w[4];
+    // Copies the warp's 32 queries as they are to their places in Q_t, kPer lanes to a row ...
+    auto fetch_query = [&](const Item& x) {
+      const int row = x.row0 + t * 128 + r, mine = row < x.s.rows ? number(x, row) : -1;
+      const int chunk = lane % kPer;
+#pragma unroll 4
+      for (int k = 0; k < kPer; ++k) {
+        const int in_warp = k * kAtOnce + lane / kPer, from = __shfl_sync(0xffffffffu, mine, in_warp);
+        uint8_t* to = tq + place(quarter * 32 + in_warp, chunk);
+        if (from >= 0)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(a.q + (int64_t)from * D + chunk * 8) : "memory");
+        else
+          *(uint4*)to = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // ... where each thread turns its row into f16, chunk by chunk, and sums its groups. Returns the factor of the row's
+    // scores (K's powers of two aside).
+    auto put_query = [&]() -> float {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncwarp();
+      uint32_t top = 0;  // of the magnitudes, as bf16 bits
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 w = *(const uint4*)(tq + place(r, c));
+        top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+      }
+      top = max(top & 0xffffu, top >> 16);
+      const int e = max((int)(top >> 7) - 127, -118);  // largest in [2^e, 2^(e + 1)); below 2^-118 it stays smaller
+      // the scale's sign goes into q, so that the largest score is the largest product
+      const float up = a.scale < 0.0f ? -power(8 - e) : a.scale > 0.0f ? power(8 - e) : 0.0f;
+      uint32_t z[8] = {};  // k = part * NG + group: the groups' sums in two f16 parts
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int row = x.row0 + t * 128 + first + (k0 + k) * kAtOnce;
-          w[k] = make_uint4(0, 0, 0, 0);
-          if (row < x.s.rows) w[k] = __ldg((const uint4*)(a.q + (int64_t)number(x, row) * D) + chunk);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int row = first + (k0 + k) * kAtOnce;
-          const uint32_t y[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-          uint32_t top = 0;  // of the magnitudes, as bf16 bits
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = __vmaxu2(top, y[e] & 0x7fff7fffu);
-          top = max(top & 0xffffu, top >> 16);
-#pragma unroll
-          for (int o = 1; o < kPer; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int e = max((int)(top >> 7) - 127, -118);  // largest in [2^e, 2^(e + 1)); below 2^-118 it stays smaller
-          // the scale's sign goes into q, so that the largest score is the largest product
-          const float up = a.scale < 0.0f ? -power(8 - e) : a.scale > 0.0f ? power(8 - e) : 0.0f;
+      for (int j = 0; j < NG; ++j) {
+        float sum = 0.0f;
+#pragma unroll 2
+        for (int i = 0; i < 4; ++i) {
+          uint4* at = (uint4*)(tq + place(r, 4 * j + i));
+          const uint4 w = *at;
+          const uint32_t y[4] = {w.x, w.y, w.z, w.w};
           float v[8];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             v[2 * c] = step_of(y[c]) * up;
             v[2 * c + 1] = offset_of(y[c]) * up;
           }
-          const uint4 h = make_uint4(f16x2(v[0], v[4]), f16x2(v[1], v[5]), f16x2(v[2], v[6]), f16x2(v[3], v[7]));
-          *(uint4*)(tq + place(row, chunk)) = h;
-          float sum = (sum_of(h.x) + sum_of(h.y)) + (sum_of(h.z) + sum_of(h.w));
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          // the sum's two f16 parts from the first two lanes of the group, zeros from the others: k = part * NG + group
-          const uint32_t one = f16x2(sum, 0.0f);
-          const uint32_t parts = chunk & 1 ? f16x2(sum - low_half(one), 0.0f) : one;
-          uint16_t* z = (uint16_t*)(sQz + t * kOffsets + offsets_place(row, 0));
-          const int at = (chunk & 3) * NG + (chunk >> 2);  // 0 .. 4 NG - 1
-          z[at < 8 ? at : 64 + at - 8] = (uint16_t)((chunk & 3) < 2 ? parts : 0u);
-          if (NG == 2) z[64 + at] = 0;
-          // row r's exponent goes to thread r
-          const int es = __shfl_sync(0xffffffffu, e, lane % kAtOnce * kPer);
-          if (lane / kAtOnce == k0 + k) exponent = es;
+          // 8 bits fit f16's 11 but for values below 2^-22 of the row's largest: the sum is that of what is stored
+          sum += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+          *at = make_uint4(f16x2(v[0], v[4]), f16x2(v[1], v[5]), f16x2(v[2], v[6]), f16x2(v[3], v[7]));
         }
+        const uint32_t one = f16x2(sum, 0.0f), two = f16x2(sum - low_half(one), 0.0f);
+        z[j >> 1] |= j & 1 ? one << 16 : one & 0xffffu;
+        z[(j + NG) >> 1] |= j & 1 ? two << 16 : two & 0xffffu;
       }
+      uint8_t* tz = sQz + t * kOffsets;
+      *(uint4*)(tz + offsets_place(r, 0)) = make_uint4(z[0], z[1], z[2], z[3]);
+      *(uint4*)(tz + offsets_place(r, 1)) = make_uint4(z[4], z[5], z[6], z[7]);
       async_fence();
       mbar_arrive(smem_u32(&q_full[t]));
       // not 0, so that a hidden key stays at -inf
-      return fmaxf(scalbnf(fabsf(a.scale) * kLog2e, exponent - 8), 0x1p-126f);
+      return fmaxf(scalbnf(fabsf(a.scale) * kLog2e, e - 8), 0x1p-126f);
     };
 
     uint32_t meetings = 0;
@@ -534,6 +537,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
     int n = 0;
     // Each part stands here once, in one place: the roles' code together has to stay in the instruction cache.
     for (int seg = 0; more || seg; ++seg) {
+      // the scores of the segment before are complete, so Q_t is free: this one's query goes in before that one's
+      // output leaves
+      if (more) {
+        fetch_query(it);
+        qs = put_query();
+      }
       if (seg) {
         ok = mbar_wait(smem_u32(&o_done[t]), (seg - 1) & 1, abort_flag, a.err, 423);
         ok = __all_sync(0xffffffffu, ok);
@@ -583,58 +592,52 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
           }
         }
         if (output) {
-          // through the warp's rows of Q_t, whose scores are complete, so that it leaves in whole rows
           const float scale = total != 0.0f ? 1.0f / total : 0.0f;
+          const int row = done.row0 + t * 128 + r, mine = row < done.s.rows ? number(done, row) : -1;
+          uint16_t* out = a.o + (int64_t)max(mine, 0) * D;
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            float o[32];
+          for (int c = 0; c < D / 64; ++c) {
+            float o[64];
             if (whole) {
-              tld32(tO + 32 * c, (uint32_t*)o);
+              tld32(tO + 64 * c, (uint32_t*)o);
+              tld32(tO + 64 * c + 32, (uint32_t*)o + 32);
               tld_wait_regs((uint32_t*)o);
+              tld_wait_regs((uint32_t*)o + 32);
             } else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+              for (int i = 0; i < 64; ++i) o[i] = 0.0f;
 #pragma unroll 1
               for (int b = c0; b <= c1; ++b) {
                 const float* q = slot(b, b == c0);
                 const float f = exp2_(__ldcg(q + D * 128 + r) - top);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  const float4 v = __ldcg((const float4*)q + (8 * c + i) * 128 + r);
+                for (int i = 0; i < 16; ++i) {
+                  const float4 v = __ldcg((const float4*)q + (16 * c + i) * 128 + r);
                   o[4 * i] = fmaf(f, v.x, o[4 * i]), o[4 * i + 1] = fmaf(f, v.y, o[4 * i + 1]);
                   o[4 * i + 2] = fmaf(f, v.z, o[4 * i + 2]), o[4 * i + 3] = fmaf(f, v.w, o[4 * i + 3]);
                 }
               }
             }
-            // 32 columns in the order of the codes -> 32 / NG neighbouring channels of each group
+            if (mine < 0) continue;
+            // 64 columns in the order of the codes -> 64 / NG neighbouring channels of each group, whole sectors
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
-              uint32_t y[16 / NG];
+              uint32_t y[32 / NG];
 #pragma unroll
-              for (int i = 0; i < 16 / NG; ++i) {  // channels 2 i, 2 i + 1 of the run: code word 4 c + word, its codes e, e + 1
+              for (int i = 0; i < 32 / NG; ++i) {  // channels 2 i, 2 i + 1 of the run: code word `word`, its codes e, e + 1
                 const int g = i / 2, word = g * (NG / 2) + j / 2, e = 2 * (i & 1);
                 y[i] = rounded(o[8 * word + 2 * e + (j & 1)], o[8 * word + 2 * e + 2 + (j & 1)], scale);
               }
 #pragma unroll
-              for (int i = 0; i < 16 / NG / 4; ++i)
-                *(uint4*)(tq + place(r, j * 4 + c * (4 / NG) + i)) = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+              for (int i = 0; i < 32 / NG / 8; ++i)
+                store32(out + j * kGroup + c * (64 / NG) + 16 * i, y + 8 * i);
             }
           }
-          const int mine = done.row0 + t * 128 + r < done.s.rows ? number(done, done.row0 + t * 128 + r) : -1;
-          __syncwarp();
-#pragma unroll 4
-          for (int k = 0; k < kPer; ++k) {
-            const int row = k * kAtOnce + lane / kPer, chunk = lane % kPer;
-            const int to = __shfl_sync(0xffffffffu, mine, row);
-            if (to >= 0) ((uint4*)(a.o + (int64_t)to * D))[chunk] = *(const uint4*)(tq + place(quarter * 32 + row, chunk));
-          }
-          __syncwarp();
         }
         // O_t may be overwritten: the arrival at p_ready of the next segment's first tile comes after these reads
         fence_before();
       }
       if (!more) break;
-      qs = put_query(it);
       done = it;
       more = walk.next(it);  // while the first scores are on their way
       const int row = done.row0 + t * 128 + r;

@@ -420,7 +420,7 @@ fopt_status fopt_cache_read(fopt_ctx* ctx, void* out_k, void* out_v, fopt_dtype 
  * entries) and the kv_len[b] keys whose key i lies in page table[b * table_width + i / page_size], slot i %
  * page_size. Causal: the queries are the sequence's last tokens, so query j of n sees keys 0 ..
  * kv_len[b] - n + j; otherwise every query sees all kv_len[b]. Query head h reads key head h / (hq / H).
- * o [tokens, hq, D] bf16: a row that sees no key is 0; rows of tokens past q_start[batch] are left
+ * o [tokens, hq, D] bf16 (32-byte aligned, q 16): a row that sees no key is 0; rows of tokens past q_start[batch] are left
  * as they were. Scores, maxima, sums and the output accumulate in f32. Reads nothing but the keys in
  * range: table entries and cache slots past kv_len may hold anything. A page number outside the cache
  * (its keys count as zeros), a length past table_width pages (cut) or a q_start that is not ascending
