@@ -32,7 +32,6 @@ struct AttnArgs {
 };
 
 constexpr float kNone = -0x1p120f;  // the maximum of a part that has no score; its sum is 0
-constexpr float kLazy = 8.0f;       // log2 by which a score may exceed the running maximum before it moves
 
 struct Seq {
   int q0, rows;  // first query token; query rows per key head (tokens x group)
@@ -75,13 +74,14 @@ struct Shares {
 
 // Where a block's share begins: the line's length, the blocks that have a share, and the sequence in which this
 // one's begins with the position of that sequence's first unit. For all threads of the block, with `units(b)`
-// the length of sequence b; blocks without a share get blocks <= blockIdx.x.
+// the length of sequence b and shares of at least `least` units (adding up parts costs, too); blocks without a
+// share get blocks <= blockIdx.x.
 struct Start {
   long long total, seq_at;
   int blocks, b;
 };
 template <int THREADS, typename Units>
-__device__ __forceinline__ Start share_start(int batch, Units units) {
+__device__ __forceinline__ Start share_start(int batch, int least, Units units) {
   constexpr int kW = THREADS / 32;
   __shared__ long long sums[kW];
   __shared__ long long found_at;
@@ -97,7 +97,7 @@ __device__ __forceinline__ Start share_start(int batch, Units units) {
   total = 0;
 #pragma unroll
   for (int w = 0; w < kW; ++w) total += sums[w];
-  Start st{total, 0, (int)min((long long)gridDim.x, total), 0};
+  Start st{total, 0, (int)min((long long)gridDim.x, (total + least - 1) / least), 0};
   if ((int)blockIdx.x >= st.blocks) return st;
   const long long unit = Shares(total, st.blocks).first(blockIdx.x);
   long long before = 0;  // units of the sequences before the chunk

@@ -39,7 +39,9 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kTileTokens = 16 * kWarps;
 constexpr int kBlocks = 3;       // resident blocks an SM, where the registers allow (168 a thread)
 constexpr int kSegmentCost = 4;  // beginning and ending a segment takes about as long as this many tiles
+constexpr int kLeast = 2;        // tiles of a share: a part more to add up takes about as long as one
 constexpr int kStages = 4;
+constexpr float kLazy = 8.0f;    // log2 by which a score may exceed the running maximum before it moves
 constexpr int kFewRows = 32;     // query rows per key head up to which a sequence is tokens_kernel's
 // The sequence's tiles (one at least: a sequence without keys still writes its rows), and how long its segments
 // and all of them together are in the division of work.
@@ -412,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
   __shared__ int last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
 
-  const Start start = share_start<kThreads>(a.batch, [&](int b) { return units<R>(a, sequence(a, b)); });
+  const Start start = share_start<kThreads>(a.batch, kLeast, [&](int b) { return units<R>(a, sequence(a, b)); });
   if ((int)blockIdx.x >= start.blocks) return;
   const Shares shares(start.total, start.blocks);
   long long unit = shares.first(blockIdx.x);
@@ -683,8 +685,9 @@ extern "C" fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* 
     const int dim = cache->head_dim;
     // Sequences of more than kv::kFewRows query rows go to rows_kernel, whose tiles of 256 rows take about as long
     // as that many rows of tokens_kernel (head_dim 256 exceeds its tensor memory). The lengths are the device's,
-    // so both are launched unless no sequence can be that long.
-    const bool rows = dim != 256 && (int64_t)tokens * a.group > kv::kFewRows;
+    // so both are launched, unless no sequence can be that long or the call has no more tokens than sequences:
+    // then it is single tokens, for which rows_kernel would only begin and end (4 us).
+    const bool rows = dim != 256 && tokens > batch && (int64_t)tokens * a.group > kv::kFewRows;
     a.long_rows = rows ? kv::kFewRows + 1 : INT32_MAX;
     // 16 rows a block where a sequence has that many on average: the codes are expanded once for both halves
     const bool two = (int64_t)tokens * a.group > 8 * (int64_t)batch;

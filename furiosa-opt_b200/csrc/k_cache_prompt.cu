@@ -43,7 +43,9 @@ constexpr int kExpand = 7, kRowThreads = 32 * (1 + kExpand + 8);  // warps that 
 constexpr int kHalf = 16384;             // 128 rows of 64 f16 (128 bytes), the unit of the swizzled tiles
 constexpr int kOffsets = 128 * 32;        // 128 rows of 16 f16: the sums of a tile's q, or the offsets of a key tile
 constexpr int kCost = 2;                 // key tiles that beginning and ending a segment takes as long as
+constexpr int kLeast = 4;                // units of a share: a part more to add up takes about as long as a tile
 constexpr int kUncut = 8;                // segments of fewer tiles are not shared between blocks
+constexpr float kLazyRows = 14.0f;        // log2 by which x may exceed its base: P stays within f16, the base moves rarely
 constexpr float kLog2e = 1.44269504088896340736f;
 
 template <int NG>
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
   int* last = (int*)(tmem_slot + 2);    // [2]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Start start = share_start<kRowThreads>(a.batch, [&](int b) { return units(a, sequence(a, b)); });
+  const Start start = share_start<kRowThreads>(a.batch, kLeast, [&](int b) { return units(a, sequence(a, b)); });
   if ((int)blockIdx.x >= start.blocks) return;
   const Shares shares(start.total, start.blocks);
 
@@ -552,7 +554,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         // partial results: [D / 4][128] float4, so that a warp's rows are contiguous, then maxima and sums
         auto slot = [&](int block, bool begins) { return a.ws + ((int64_t)block * 2 + begins) * T::kSlot + t * 128 * (D + 2); };
         int c0 = 0, c1 = 0;
-        float top = 0.0f, total = l;
         bool output = true;
         if (!whole) {
           float* part = slot(blockIdx.x, done.t0 == 0);
@@ -579,45 +580,48 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
           if (!(ok = meet())) break;
           output = last[t];
           if (!(ok = meet())) break;  // last[t] has been read
-          if (output) {
-            top = kNone;
-            total = 0.0f;
+          if (output) {  // the parts' sum goes into O_t
+            float top = kNone;
+            l = 0.0f;
 #pragma unroll 4
             for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(slot(c, c == c0) + D * 128 + r));
 #pragma unroll 4
             for (int c = c0; c <= c1; ++c) {
               const float* q = slot(c, c == c0) + D * 128 + r;
-              total = fmaf(exp2_(__ldcg(q) - top), __ldcg(q + 128), total);
+              l = fmaf(exp2_(__ldcg(q) - top), __ldcg(q + 128), l);
             }
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+#pragma unroll 2
+              for (int b = c0; b <= c1; ++b) {
+                const float* q = slot(b, b == c0);
+                const float f = exp2_(__ldcg(q + D * 128 + r) - top);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const float4 v = __ldcg((const float4*)q + (8 * c + i) * 128 + r);
+                  o[4 * i] = fmaf(f, v.x, o[4 * i]), o[4 * i + 1] = fmaf(f, v.y, o[4 * i + 1]);
+                  o[4 * i + 2] = fmaf(f, v.z, o[4 * i + 2]), o[4 * i + 3] = fmaf(f, v.w, o[4 * i + 3]);
+                }
+              }
+              tst32(tO + 32 * c, (const uint32_t*)o);
+            }
+            tst_wait();
           }
         }
         if (output) {
-          const float scale = total != 0.0f ? 1.0f / total : 0.0f;
+          const float scale = l != 0.0f ? 1.0f / l : 0.0f;
           const int row = done.row0 + t * 128 + r, mine = row < done.s.rows ? number(done, row) : -1;
           uint16_t* out = a.o + (int64_t)max(mine, 0) * D;
 #pragma unroll 1
           for (int c = 0; c < D / 64; ++c) {
             float o[64];
-            if (whole) {
-              tld32(tO + 64 * c, (uint32_t*)o);
-              tld32(tO + 64 * c + 32, (uint32_t*)o + 32);
-              tld_wait_regs((uint32_t*)o);
-              tld_wait_regs((uint32_t*)o + 32);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 64; ++i) o[i] = 0.0f;
-#pragma unroll 1
-              for (int b = c0; b <= c1; ++b) {
-                const float* q = slot(b, b == c0);
-                const float f = exp2_(__ldcg(q + D * 128 + r) - top);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const float4 v = __ldcg((const float4*)q + (16 * c + i) * 128 + r);
-                  o[4 * i] = fmaf(f, v.x, o[4 * i]), o[4 * i + 1] = fmaf(f, v.y, o[4 * i + 1]);
-                  o[4 * i + 2] = fmaf(f, v.z, o[4 * i + 2]), o[4 * i + 3] = fmaf(f, v.w, o[4 * i + 3]);
-                }
-              }
-            }
+            tld32(tO + 64 * c, (uint32_t*)o);
+            tld32(tO + 64 * c + 32, (uint32_t*)o + 32);
+            tld_wait_regs((uint32_t*)o);
+            tld_wait_regs((uint32_t*)o + 32);
             if (mine < 0) continue;
             // 64 columns in the order of the codes -> 64 / NG neighbouring channels of each group, whole sectors
 #pragma unroll
@@ -653,24 +657,33 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         const bool cut = __any_sync(0xffffffffu, left < kKeys), first = kt == done.t0;
         const float* kb = k_back + (n & 3) * 4;
         const float* vu = v_up + (n & 3) * 4;
-        // the largest x, then the base: it moves when x exceeds it by 2^8
+        // the largest x, then the base
         float top = -INFINITY;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t s[32];
-          tld32(tS + 32 * c, s);
+        for (int h = 0; h < 2; ++h) {  // two loads at a time on their way
+          uint32_t s[64];
+          tld32(tS + 64 * h, s);
+          tld32(tS + 64 * h + 32, s + 32);
           tld_wait_regs(s);
-          if (cut) hide(s, left - 32 * c);
-          float high[2] = {__uint_as_float(s[0]), __uint_as_float(s[1])};
-#pragma unroll
-          for (int i = 2; i < 30; i += 4) {
-            high[0] = max3(high[0], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-            high[1] = max3(high[1], __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+          tld_wait_regs(s + 32);
+          if (cut) {
+            hide(s, left - 64 * h);
+            hide(s + 32, left - 64 * h - 32);
           }
-          high[0] = max3(high[0], __uint_as_float(s[30]), __uint_as_float(s[31]));
-          top = fmaxf(top, fmaf(fmaxf(high[0], high[1]), qs * kb[c], vu[c]));
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t* y = s + 32 * c;
+            float high[2] = {__uint_as_float(y[0]), __uint_as_float(y[1])};
+#pragma unroll
+            for (int i = 2; i < 30; i += 4) {
+              high[0] = max3(high[0], __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
+              high[1] = max3(high[1], __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
+            }
+            high[0] = max3(high[0], __uint_as_float(y[30]), __uint_as_float(y[31]));
+            top = fmaxf(top, fmaf(fmaxf(high[0], high[1]), qs * kb[2 * h + c], vu[2 * h + c]));
+          }
         }
-        const float base = first ? (top == -INFINITY ? 0.0f : top) : top > m + kLazy ? top : m;
+        const float base = first ? (top == -INFINITY ? 0.0f : top) : top > m + kLazyRows ? top : m;
         if (!first && __any_sync(0xffffffffu, base != m)) {
           // S_t was issued behind the last O_t += P_t V: it is complete
           const float f = exp2_(m - base);
@@ -687,27 +700,36 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         }
         m = base;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {  // P goes over columns whose scores have been read: 16 c .. 16 c + 15
-          uint32_t s[32], p[16];
-          tld32(tS + 32 * c, s);
+        for (int h = 0; h < 2; ++h) {  // P goes over columns whose scores have been read: 16 c .. 16 c + 15
+          uint32_t s[64];
+          tld32(tS + 64 * h, s);
+          tld32(tS + 64 * h + 32, s + 32);
           tld_wait_regs(s);
-          if (cut) hide(s, left - 32 * c);
-          const float f = qs * kb[c], up = vu[c] - m;
-          const uint64_t f2 = pack_f32x2(f, f), up2 = pack_f32x2(up, up);
-          uint64_t part[2] = {0, 0};
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float x0, x1;
-            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, up2), x0, x1);
-            const float p0 = exp2_(x0), p1 = exp2_(x1);
-            part[(i >> 1) & 1] = add_f32x2(part[(i >> 1) & 1], pack_f32x2(p0, p1));
-            p[i >> 1] = f16x2(p0, p1);
+          tld_wait_regs(s + 32);
+          if (cut) {
+            hide(s, left - 64 * h);
+            hide(s + 32, left - 64 * h - 32);
           }
-          tst16(tS + 16 * c, p);
-          float s0, s1, s2, s3;
-          unpack_f32x2(part[0], s0, s1);
-          unpack_f32x2(part[1], s2, s3);
-          l = fmaf((s0 + s1) + (s2 + s3), exp2_(-vu[c]), l);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float v_e = vu[2 * h + c], f = qs * kb[2 * h + c], up = v_e - m;
+            const uint64_t f2 = pack_f32x2(f, f), up2 = pack_f32x2(up, up);
+            uint64_t part[2] = {0, 0};
+            uint32_t p[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float x0, x1;
+              unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[32 * c + i]), __uint_as_float(s[32 * c + i + 1])), f2, up2), x0, x1);
+              const float p0 = exp2_(x0), p1 = exp2_(x1);
+              part[(i >> 1) & 1] = add_f32x2(part[(i >> 1) & 1], pack_f32x2(p0, p1));
+              p[i >> 1] = f16x2(p0, p1);
+            }
+            tst16(tS + 32 * h + 16 * c, p);
+            float s0, s1, s2, s3;
+            unpack_f32x2(part[0], s0, s1);
+            unpack_f32x2(part[1], s2, s3);
+            l = fmaf((s0 + s1) + (s2 + s3), exp2_(-v_e), l);
+          }
         }
         tst_wait();
         fence_before();
