@@ -138,13 +138,15 @@ __device__ __forceinline__ int v_chunk(int token, int chunk) {
 // A warp's state over a segment's keys.
 template <int NG, int NB>
 struct State {
-  // [channel 32 j + 4 g + 2 mm (+ 1 for c2, c3)] x [row 2 i, 2 i + 1]: sum of p step (code + 8), in 2^(ev + 24)
-  // for the even channels (c0, c1) and 2^(ev + 20) for the odd ones
+  // [channel 32 j + 4 g + 2 mm (+ 1 for c2, c3)] x [row 2 i, 2 i + 1]: sum of p step (code + 8), in 2^24 for the
+  // even channels (c0, c1) and 2^20 for the odd ones
   float o[NB][NG][2][4];
   float e[NB][NG][2];      // sum of p (offset - 8 step), this lane's tokens
+  // p = 2^(score - m). The base m is that of p 2^-ev, so that p step fits f16 at any magnitude of V: it is the score's
+  // maximum (lagging by up to 2^kLazy) plus ev
   float m[NB][2], l[NB][2];
-  float vscale;            // 2^-ev
-  float vlimit;            // the largest step that p step 2^-ev still holds
+  float ev;
+  float vlimit;            // the largest step that p step still holds
 };
 
 template <int NG, int NB>
@@ -243,19 +245,17 @@ __device__ __forceinline__ Places places() {
           masks()};
 }
 
-// One tile of 16 tokens, from its stage; token0 is its first.
+// The raw scores q . k of one tile of 16 tokens, from its stage.
 template <int NG, int NB>
-__device__ __forceinline__ void tile(const uint8_t* stage, const Places& at, int token0, int keys, int sure, bool first,
-                                     const Query<NG, NB>& q,                                     State<NG, NB>& s) {
+__device__ __forceinline__ void scores(const uint8_t* stage, const Places& at, const Query<NG, NB>& q, float (*x)[4]) {
   using S = Shared<NG, NB>;
-  const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
+  const int i = threadIdx.x & 3;
   uint32_t kw[2][NG], km[2][NG];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     load_words<NG>(kw[h], stage + at.k + 8 * h * (S::D / 2));
     load_words<NG>(km[h], stage + 2 * S::kCodes + at.scale + 8 * h * NG * 4);
   }
-  float x[NB][4];
   {
     uint32_t w[2][2] = {};  // scale words of tokens g and g + 8, groups i and i + 4
     const uint8_t* sc = stage + 2 * S::kCodes + at.k_word;
@@ -292,6 +292,14 @@ __device__ __forceinline__ void tile(const uint8_t* stage, const Places& at, int
       }
     }
   }
+}
+
+// The tile's softmax and its share of the output; token0 is its first.
+template <int NG, int NB>
+__device__ __forceinline__ void values(const uint8_t* stage, const Places& at, int token0, int keys, int sure, bool first,
+                                       const Query<NG, NB>& q, State<NG, NB>& s, float (*x)[4]) {
+  using S = Shared<NG, NB>;
+  const int lane = threadIdx.x & 31, g = lane >> 2;
   uint32_t vm[2][NG];
 #pragma unroll
   for (int h = 0; h < 2; ++h) load_words<NG>(vm[h], stage + 2 * S::kCodes + S::kScales + at.scale + 8 * h * NG * 4);
@@ -324,23 +332,25 @@ __device__ __forceinline__ void tile(const uint8_t* stage, const Places& at, int
   }
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) tops = max3(max3(tops, x[nb][0], x[nb][1]), x[nb][2], x[nb][3]);
-  if (__any_sync(0xffffffffu, first || tops > kLazy || steps > s.vlimit)) {
+  if (__any_sync(0xffffffffu, first || tops > kLazy - s.ev || steps > s.vlimit)) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) steps = fmaxf(steps, __shfl_xor_sync(0xffffffffu, steps, o));
-    float by = 1.0f;
-    if (steps > s.vlimit) {  // the largest step to [2^4, 2^5), and room up to 2^7: p <= 2^8 keeps 2^15
-      const float vscale = scalbnf(1.0f, min(4 - ilogbf(steps), 126));
-      by = s.vscale > 0.0f ? vscale / s.vscale : 0.0f;
-      s.vscale = vscale;
-      s.vlimit = fminf(0x1p7f / vscale, 0x1.fep127f);
+    float lift = 0.0f;  // of ev: the largest step to 2^ev [2^4, 2^5), and room up to 2^7: p <= 2^8 keeps 2^15
+    if (steps > s.vlimit) {
+      const float ev = (float)max(ilogbf(steps) - 4, -100);  // further down p 2^-ev would pass the f32 range
+      lift = first ? 0.0f : ev - s.ev;
+      s.ev = ev;
+      s.vlimit = fminf(exp2f(ev) * 0x1p7f, 0x1.fep127f);
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        // the base moves up by the largest score over it; the first tile's scores set it
+        // the base moves up by the largest score over it, and with ev; the first tile's scores set it
         const float top_score = max_over_g(fmaxf(x[nb][c], x[nb][c + 2]));
-        const float up = first ? (top_score == -INFINITY ? 0.0f : top_score) : fmaxf(0.0f, top_score);
+        float up;
+        if (first) up = top_score == -INFINITY ? 0.0f : top_score + s.ev;
+        else up = (top_score > kLazy - (s.ev - lift) ? top_score + (s.ev - lift) : 0.0f) + lift;
         const float f = first ? 0.0f : exp2_(-up);
         s.m[nb][c] += up;
         x[nb][c] -= up;
@@ -351,8 +361,8 @@ __device__ __forceinline__ void tile(const uint8_t* stage, const Places& at, int
           s.e[nb][j][c] *= f;
 #pragma unroll
           for (int mm = 0; mm < 2; ++mm) {
-            s.o[nb][j][mm][c] *= f * by;
-            s.o[nb][j][mm][c + 2] *= f * by;
+            s.o[nb][j][mm][c] *= f;
+            s.o[nb][j][mm][c + 2] *= f;
           }
         }
       }
@@ -364,11 +374,6 @@ __device__ __forceinline__ void tile(const uint8_t* stage, const Places& at, int
       x[nb][c] = exp2_(x[nb][c]);
       s.l[nb][c & 1] += x[nb][c];
     }
-  float y[NB][4];  // p 2^-ev
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) y[nb][c] = x[nb][c] * s.vscale;
   // V: words of tokens 2 i, 2 i + 1, 2 i + 8, 2 i + 9
   uint32_t vw[4][NG / 2];
 #pragma unroll
@@ -383,8 +388,8 @@ __device__ __forceinline__ void tile(const uint8_t* stage, const Places& at, int
     const float z0 = fmaf(-8.0f, s0, offset_of(vm[0][j])), z1 = fmaf(-8.0f, s1, offset_of(vm[1][j]));
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const uint32_t b0 = transposed(f16x2(y[nb][0] * s0, y[nb][1] * s0));
-      const uint32_t b1 = transposed(f16x2(y[nb][2] * s1, y[nb][3] * s1));
+      const uint32_t b0 = transposed(f16x2(x[nb][0] * s0, x[nb][1] * s0));
+      const uint32_t b1 = transposed(f16x2(x[nb][2] * s1, x[nb][3] * s1));
       mma(s.o[nb][j][0], codes_low(at.masks, x01), codes_high(at.masks, x01), codes_low(at.masks, x23), codes_high(at.masks, x23), b0, b1);
       mma(s.o[nb][j][1], codes_low(at.masks, y01), codes_high(at.masks, y01), codes_low(at.masks, y23), codes_high(at.masks, y23), b0, b1);
 #pragma unroll
@@ -430,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
   // one half of the lanes K's scales, with the other V's
   constexpr int kHalf = S::kScaleLanes < 32 ? S::kScaleLanes / 2 : 16;
   const uint8_t* k_lane = a.cache.k + lane * 16;
-  const uint8_t* v_lane = a.cache.v + lane * 16;
+  const int64_t v_from_k = a.cache.v - a.cache.k;
   const uint8_t* scale_lane =
       lane < kHalf ? (const uint8_t*)a.cache.k_scale + lane * 16 : (const uint8_t*)a.cache.v_scale + (lane - kHalf) * 16;
   // relative to lane * 16, where the lane's K codes go; a second V chunk is 8 (D = 128: 32 chunks on, the same
@@ -471,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
         for (int c = 0; c < 4; ++c) st.o[nb][j][0][c] = st.o[nb][j][1][c] = 0.0f;
       }
     }
-    st.vscale = 0.0f;
+    st.ev = 0.0f;
     st.vlimit = 0.0f;
 
     // this warp's run of the segment's 16-token tiles, and where in which page it begins
@@ -480,27 +485,35 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
     const int n1 = t0 * kWarps + tiles16 * (warp + 1) / kWarps;
     const int32_t* table = a.table + (int64_t)b * a.width;
     int page_at = (int)fdiv(a.cache.by_page, (uint32_t)n * 16);  // entry of the table that `page` is
-    int in_page = n * 16 - page_at * a.cache.page_size;
+    const int page_end = (n1 * 16 + a.cache.page_size - 1) / a.cache.page_size;
+    const int begin = n * 16 - page_at * a.cache.page_size;  // within the first page
+    int left = (a.cache.page_size - begin) / 16;             // tiles of the page not yet fetched
     int page = n < n1 ? table[page_at] : 0;
     int fetched = n;
-    const uint8_t *k, *v, *sc;
+    // a page of all heads is less than 2^32 bytes: its number times that is one instruction
+    const uint32_t page_codes = (uint32_t)a.cache.heads * a.cache.page_size * (D / 2);
+    const uint32_t page_scales = (uint32_t)a.cache.heads * a.cache.page_size * (NG * 4);
+    const uint8_t* k_head = k_lane + (int64_t)head * a.cache.page_size * (D / 2);
+    const uint8_t* sc_head = scale_lane + (int64_t)head * a.cache.page_size * (NG * 4);
+    const uint8_t *k, *sc;
     bool there;
-    auto enter = [&] {  // the page's rows from in_page on
-      there = page >= 0 && page < a.cache.pages;
+    auto enter = [&] {  // the page's first rows
+      there = (uint32_t)page < (uint32_t)a.cache.pages;
       if (!there && lane == 0) atomicExch(a.err, kBadPage);
-      const int64_t row = there ? ((int64_t)page * a.cache.heads + head) * a.cache.page_size + in_page : 0;
-      k = k_lane + row * (D / 2);
-      v = v_lane + row * (D / 2);
-      sc = scale_lane + row * (NG * 4);
-      ++page_at;
-      page = (int64_t)page_at * a.cache.page_size < n1 * 16 ? table[page_at] : 0;  // for the next time
+      k = k_head + (uint64_t)(uint32_t)page * page_codes;
+      sc = sc_head + (uint64_t)(uint32_t)page * page_scales;
+      page = ++page_at < page_end ? table[page_at] : 0;  // for the next time
     };
-    if (n < n1) enter();
+    if (n < n1) {
+      enter();
+      k += begin * (D / 2);
+      sc += begin * (NG * 4);
+    }
     uint32_t into = 0, from = 0;  // stages, in bytes
     auto fetch = [&] {
       if (fetched < n1) {
-        if (in_page == a.cache.page_size) {
-          in_page = 0;
+        if (left == 0) {
+          left = a.cache.page_size / 16;
           enter();
         }
         const uint32_t to = ring_u32 + into;
@@ -508,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
 #pragma unroll
           for (int c = 0; c * 32 < S::kCodes / 16; ++c) copy16(to + c * 512, k + c * 512);
 #pragma unroll
-          for (int c = 0; c * 32 < S::kCodes / 16; ++c) copy16(to + (c & 1 ? v_to1 : v_to0) + c * 512, v + c * 512);
+          for (int c = 0; c * 32 < S::kCodes / 16; ++c) copy16(to + (c & 1 ? v_to1 : v_to0) + c * 512, k + v_from_k + c * 512);
 #pragma unroll
           for (int c = 0; c * 32 < S::kScaleLanes; ++c)
             if (lane < S::kScaleLanes) copy16(to + scale_to + c * 256, sc + c * 256);
@@ -516,9 +529,8 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
           for (int c = lane; c < S::kStage / 16; c += 32) *(uint4*)(ring + into + c * 16) = make_uint4(0, 0, 0, 0);
         }
         k += S::kCodes;
-        v += S::kCodes;
         sc += S::kScales;
-        in_page += 16;
+        --left;
         ++fetched;
       }
       copies_commit();
@@ -526,22 +538,36 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
     };
 #pragma unroll 1
     for (int c = 0; c < kStages - 1; ++c) fetch();
+    // A tile's scores are computed while the tile before is finished: two independent chains of instructions.
+    auto next_stage = [](uint32_t at) { return at + S::kStage == S::kRing ? 0 : at + S::kStage; };
+    float x[NB][4];
+    if (n < n1) {
+      copies_wait<kStages - 2>();
+      __syncwarp();
+      scores<NG, NB>(ring, at, q, x);
+    }
     bool first = true;
 #pragma unroll 1
     for (; n < n1; ++n) {
       fetch();
-      copies_wait<kStages - 1>();
+      copies_wait<kStages - 2>();
       __syncwarp();
-      tile<NG, NB>(ring + from, at, n * 16, s.keys, sure, first, q, st);
+      const uint32_t then = next_stage(from);
+      float ahead[NB][4];
+      scores<NG, NB>(ring + then, at, q, ahead);  // behind the last tile: of what the stage holds, and not used
+      values<NG, NB>(ring + from, at, n * 16, s.keys, sure, first, q, st, x);
       first = false;
       __syncwarp();  // all lanes have read the stage before the next copies into it
-      from = from + S::kStage == S::kRing ? 0 : from + S::kStage;
+      from = then;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[nb][c] = ahead[nb][c];
     }
     copies_wait<0>();
     __syncthreads();  // every warp's ring is drained: the outputs go over them
 
     float* out = (float*)smem + warp * R * S::kRow;
-    const float back = st.vscale > 0.0f ? 1.0f / st.vscale : 0.0f;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -556,8 +582,8 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
         for (int j = 0; j < NG; ++j) {
           const float e = sum_over_g(st.e[nb][j][c]);
           *(float4*)(out + r * S::kRow + j * kGroup + 4 * g) =
-              make_float4(fmaf(st.o[nb][j][0][c] * 0x1p24f, back, e), fmaf(st.o[nb][j][0][c + 2] * 0x1p20f, back, e),
-                          fmaf(st.o[nb][j][1][c] * 0x1p24f, back, e), fmaf(st.o[nb][j][1][c + 2] * 0x1p20f, back, e));
+              make_float4(fmaf(st.o[nb][j][0][c], 0x1p24f, e), fmaf(st.o[nb][j][0][c + 2], 0x1p20f, e),
+                          fmaf(st.o[nb][j][1][c], 0x1p24f, e), fmaf(st.o[nb][j][1][c + 2], 0x1p20f, e));
         }
       }
     __syncthreads();

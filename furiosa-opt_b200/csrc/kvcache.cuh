@@ -43,6 +43,7 @@ inline Cache checked(const fopt_paged_cache* c, const char* who) {
   require(c->page_size > 0 && c->page_size % kSlots == 0 && c->page_size <= 65536,
           w + "page_size must be a multiple of 16, at most 65536");
   require((int64_t)c->pages * c->page_size <= INT32_MAX, w + "slots past 2^31");
+  require((int64_t)c->heads * c->page_size * c->head_dim <= UINT32_MAX, w + "a page past 2^32 elements");
   Cache k{(uint8_t*)c->k, (uint8_t*)c->v, (uint32_t*)c->k_scale, (uint32_t*)c->v_scale, c->pages, c->page_size,
           c->heads, make_fastdiv((uint32_t)c->page_size)};
   return k;

@@ -387,7 +387,7 @@ fopt_status fopt_rotary(fopt_ctx* ctx, void* out, const void* x, fopt_dtype dtyp
                         const fopt_rope* rope, int32_t tokens, int32_t heads, int32_t head_dim, int64_t x_stride,
                         int64_t out_stride);
 
-/* The cache: `pages` pages of `page_size` slots (a multiple of 16) for `heads` key / value heads of
+/* The cache: `pages` pages of `page_size` slots (a multiple of 16, 65536 at most) for `heads` key / value heads of
  * head_dim 64, 128 or 256 channels D. Mappings of the four 16-byte aligned images (P page, H head, S
  * slot of the page):
  *   k        i4    [P, H, S, D % 32 / 8, D / 32, D % 8]
