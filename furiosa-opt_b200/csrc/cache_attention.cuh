@@ -178,17 +178,10 @@ __device__ __forceinline__ uint32_t masked(uint32_t x, uint32_t mask, uint32_t f
   return r;
 }
 
-// 2^(8 - e) for rows of queries whose largest magnitude is in [2^e, 2^(e + 1)), as two factors (it may pass
-// the f32 range), which brings them to f16 with full precision.
-struct RowScale {
-  float up0, up1;
-  int e;
-  __device__ __forceinline__ explicit RowScale(float top) {
-    e = top > 0.0f ? min(ilogbf(top), 127) : 0;
-    up0 = scalbnf(1.0f, (8 - e) / 2);
-    up1 = scalbnf(1.0f, 8 - e - (8 - e) / 2);
-  }
-};
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // e in -126 .. 127
+// A row of queries whose largest magnitude, as bf16 bits, is `top` in [2^e, 2^(e + 1)) times 2^(8 - e) is f16 with full
+// precision. Below 2^-118 rows stay smaller.
+__device__ __forceinline__ int row_exponent(uint32_t top) { return max((int)(top >> 7) - 127, -118); }
 
 // Launches rows_kernel for the sequences of at least a.long_rows rows (head_dim 64 or 128). `ws` holds
 // rows_workspace() bytes; `counter` two counters per SM.

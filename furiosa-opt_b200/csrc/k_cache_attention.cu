@@ -172,18 +172,20 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, const Seq& s, int 
     const int token = live ? token_of(a, r) : 0;
     const uint16_t* p = a.q + ((int64_t)(s.q0 + token) * a.hq + head * a.group + (live ? r - token * a.group : 0)) * D;
     uint4 w[NG];
-    float top = 0.0f;
+    uint32_t top = 0;  // of the magnitudes, as bf16 bits
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       w[j] = live ? *(const uint4*)(p + j * kGroup + i * 8) : make_uint4(0, 0, 0, 0);
       const uint32_t* x = (const uint32_t*)&w[j];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(fabsf(step_of(x[e])), fabsf(offset_of(x[e]))));
+      for (int e = 0; e < 4; ++e) top = __vmaxu2(top, x[e] & 0x7fff7fffu);
     }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const RowScale up(top);
-    const float down = scalbnf(a.scale * 1.44269504088896340736f, up.e + 12);
+    top = max(top & 0xffffu, top >> 16);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int ex = row_exponent(top);
+    const float up = power(8 - ex);
+    const float down = scalbnf(a.scale * 1.44269504088896340736f, ex + 12);
     float sum[NG];
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
@@ -192,7 +194,7 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, const Seq& s, int 
       sum[j] = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        v[e] = (e & 1 ? offset_of(x[e >> 1]) : step_of(x[e >> 1])) * up.up0 * up.up1;
+        v[e] = (e & 1 ? offset_of(x[e >> 1]) : step_of(x[e >> 1])) * up;
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -458,8 +460,6 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
     unit = seg_at + u1;
     if (t1 <= t0) continue;
 
-    Query<NG, NB> q;
-    load_query<NG, NB>(a, s, head, row0, q);
     // keys that any row of the block sees, and that every row sees
     const int rows = min(R, s.rows - row0);
     const int most = seen(a, s, row0 + rows - 1);
@@ -538,6 +538,8 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
     };
 #pragma unroll 1
     for (int c = 0; c < kStages - 1; ++c) fetch();
+    Query<NG, NB> q;
+    load_query<NG, NB>(a, s, head, row0, q);  // while the first keys are on their way
     // A tile's scores are computed while the tile before is finished: two independent chains of instructions.
     auto next_stage = [](uint32_t at) { return at + S::kStage == S::kRing ? 0 : at + S::kStage; };
     float x[NB][4];
@@ -622,9 +624,9 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
     }
     if (!whole) {
       const int c0 = shares.owner(seg_at + kSegmentCost), c1 = shares.owner(seg_at + length - 1);
-      __threadfence();
-      __syncthreads();
+      __syncthreads();  // one thread's fence below covers what the barrier has ordered before it
       if (tid == 0) {
+        __threadfence();
         last = atomicAdd(a.counter + c0, 1u) == (uint32_t)(c1 - c0);
         if (last) a.counter[c0] = 0;
         __threadfence();

@@ -240,7 +240,6 @@ __device__ __forceinline__ int warp_exponent(const uint32_t* scales) {
   const uint32_t all = __reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu);
   return all ? min(max((int)(all >> 23) - 127 - 4, -120), 120) : 0;
 }
-__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // e in -126 .. 127
 
 template <int NG>
 __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
@@ -492,7 +491,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
       }
       top = max(top & 0xffffu, top >> 16);
-      const int e = max((int)(top >> 7) - 127, -118);  // largest in [2^e, 2^(e + 1)); below 2^-118 it stays smaller
+      const int e = row_exponent(top);
       // the scale's sign goes into q, so that the largest score is the largest product
       const float up = a.scale < 0.0f ? -power(8 - e) : a.scale > 0.0f ? power(8 - e) : 0.0f;
       uint32_t z[8] = {};  // k = part * NG + group: the groups' sums in two f16 parts
@@ -569,9 +568,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
           part[D * 128 + 128 + r] = l;
           c0 = shares.owner(done.at + kCost);
           c1 = shares.owner(done.at + done.tiles + kCost - 1);
-          __threadfence();
           if (!(ok = meet())) break;
           if (r == 0) {
+            __threadfence();  // covers what the meeting has ordered before it
             uint32_t* counter = a.counter + 2 * c0 + t;
             last[t] = atomicAdd(counter, 1u) == (uint32_t)(c1 - c0);
             if (last[t]) *counter = 0;
