@@ -219,6 +219,51 @@ def test_append_of_what_no_code_says(b200, dtype):
     assert np.isfinite(k.to_numpy()).all() and np.isfinite(v.to_numpy()).all()
 
 
+@pytest.mark.parametrize("rot", [0, 48])  # 24 pairs: a half ends inside the channels of one thread
+@pytest.mark.parametrize("power", [-140, -126, -104, -97, -60, 0, 60, 97, 124])
+def test_append_on_and_beside_the_borders_between_codes(b200, power, rot):
+    """Values at the middle of two codes, which go to the even one, and their neighbours, in steps of all sizes."""
+    T, H, D = 64, 2, 64
+    rng = np.random.default_rng(power % 97)
+    n = (T, H, D // 32)
+    step = _bf(np.exp2(rng.uniform(0, 1, n)))
+    at = rng.integers(0, 31, n + (32,)) * F(0.5)
+    at[..., 0], at[..., 1] = 0, 15
+    with np.errstate(over="ignore", under="ignore"):
+        x = (at * step[..., None] + rng.integers(-2, 3, n)[..., None] * step[..., None]).astype(F)
+        x = np.where(rng.random(x.shape) < 0.5, x, np.nextafter(x, F(np.inf) * rng.choice([-1, 1], x.shape).astype(F)))
+        x = np.ldexp(x.astype(F), power).astype(F).reshape(T, H, D)
+    pos = rng.integers(0, 50, T)
+    f = _freqs(48)
+    for dtype in ("f32", "bf16"):
+        a = _bf(x) if dtype == "bf16" else x
+        ref, cache = R.Cache(4, 16, H, D), fb.PagedCache(b200, 4, 16, H, D)
+        ref.append(R.rotate(a, pos, f) if rot else a, a, np.arange(T))
+        b200.cache_append(cache, _up(b200, a, dtype), _up(b200, a, dtype), _up(b200, np.arange(T), "i32"),
+                          positions=_up(b200, pos, "i32") if rot else None, rope=fb.Rope(f) if rot else None)
+        b200.sync()
+        _assert_cache(cache, ref)
+
+
+@pytest.mark.parametrize("rot,layout", [(64, "half"), (64, "interleaved"), (48, "half"), (26, "half")])
+def test_rotary_of_what_bf16_says_specially(b200, rot, layout):
+    """NaN, infinities, the largest, the smallest and subnormal values: rounded under the bf16 rule, and only
+    their own pairs touched."""
+    T, H, D = 40, 2, 64
+    rng = np.random.default_rng(rot)
+    x = _bf(rng.standard_normal((T, H, D)))
+    for v in (np.nan, np.inf, -np.inf, 3.3e38, -3.3e38, 1.2e-38, 1e-39, -1e-40, 0.0, -0.0):
+        x[rng.integers(0, T, 12), rng.integers(0, H, 12), rng.integers(0, D, 12)] = _bf(v)
+    pos, f = np.arange(T), _freqs(rot)
+    got = b200.rotary(_up(b200, x, "bf16"), _up(b200, pos, "i32"), fb.Rope(f, layout=layout), H, D).to_numpy()
+    y = R.rotate(x, pos, f, layout)
+    want = dtypes.f32_to_bf16_bits(R.bf16_round(y)).reshape(T, H, D)
+    got = np.asarray(got).reshape(T, H, D)
+    want[np.isnan(y)] = 0x7FC0
+    want[..., rot:] = dtypes.f32_to_bf16_bits(x[..., rot:])  # copied, not rounded
+    assert np.array_equal(got, want)
+
+
 def test_append_leaves_other_slots_and_reports_slots_past_the_cache(b200):
     T, H, D, page, pages = 6, 2, 128, 16, 3
     rng = np.random.default_rng(3)
