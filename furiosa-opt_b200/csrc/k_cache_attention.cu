@@ -421,6 +421,8 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
   __shared__ int last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
 
+  // rows_kernel, if it is launched behind, may begin: it works on other sequences, in memory of its own
+  asm volatile("griddepcontrol.launch_dependents;");
   const Start start = share_start<kThreads>(a.batch, kLeast, [&](int b) { return units<R>(a, sequence(a, b)); });
   if ((int)blockIdx.x >= start.blocks) return;
   const Shares shares(start.total, start.blocks);

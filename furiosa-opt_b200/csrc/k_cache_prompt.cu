@@ -272,7 +272,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Start start = share_start<kRowThreads>(a.batch, kLeast, [&](int b) { return units(a, sequence(a, b)); });
-  if ((int)blockIdx.x >= start.blocks) return;
+  // The launch does not wait for tokens_kernel's end (they share nothing); this kernel's end does, for what follows.
+  if ((int)blockIdx.x >= start.blocks) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const Shares shares(start.total, start.blocks);
 
   if (threadIdx.x == 0) {
@@ -741,6 +745,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
   __syncthreads();
   fence_after();
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace
@@ -753,7 +758,20 @@ void launch_rows(fopt_ctx* ctx, const AttnArgs& a, int head_dim, int sms) {
   static std::atomic<uint64_t> done[2];
   auto go = [&](auto kernel, int smem) {
     allow_shared(ctx, done[head_dim == 64], (const void*)kernel, smem);
-    kernel<<<sms, kRowThreads, smem, ctx->stream>>>(a);
+    // Beside tokens_kernel and not behind it: a batch of both kinds (6 sequences, 1999 keys the longest, 7 query heads
+    // to a key head of 64) takes 32 us instead of 43, and where there are prompts alone tokens_kernel's empty launch
+    // is hidden.
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = sms;
+    cfg.blockDim = kRowThreads;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    cuda_check(cudaLaunchKernelEx(&cfg, kernel, a), "cache attention launch");
     launched(ctx, "cache attention");
   };
   if (head_dim == 64) go(rows_kernel<2>, Tiles<2>::kBytes);
