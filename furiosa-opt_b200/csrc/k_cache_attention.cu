@@ -418,6 +418,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
   constexpr int D = S::D, R = S::R;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float ml[2][kWarps][R];
+  __shared__ float4 shares_of[kThreads];
   __shared__ int last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
 
@@ -635,20 +636,71 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
       }
       __syncthreads();
       if (last) {
-        for (int k = tid; k < rows * (D / 4); k += kThreads) {
-          const int r = k / (D / 4), d = k % (D / 4) * 4;
-          float m = kNone, l = 0.0f;
-          for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(P::slot(a.ws, c, c == c0) + R * D + r));
-          float4 sum = make_float4(0, 0, 0, 0);
+        // Each part's weight of each row first, by all threads at once; then the sums over the parts, with the parts
+        // of a column divided between threads where there are more threads than columns. (Every thread looking at
+        // all maxima by itself, a long context of two key heads took 25 us, against 9 when cut into fewer parts.)
+        const int parts = c1 - c0 + 1, mr = lane % R;
+        constexpr int kEach = 32 / R, kStep = kWarps * kEach;
+        const int from = c0 + warp * kEach + lane / R;
+        float* weight = (float*)smem;  // [part][row]
+        auto across = [&](float v, auto f) {
+#pragma unroll
+          for (int o = R; o < 32; o <<= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+          return v;
+        };
+        float top = kNone;
+        if (mr < rows) {
 #pragma unroll 4
-          for (int c = c0; c <= c1; ++c) {
-            const float* p = P::slot(a.ws, c, c == c0);
-            const float f = exp2_(__ldcg(p + R * D + r) - m);
-            const float4 v = __ldcg((const float4*)(p + r * D + d));
-            l = fmaf(f, __ldcg(p + R * D + R + r), l);
+          for (int c = from; c <= c1; c += kStep) top = fmaxf(top, __ldcg(P::slot(a.ws, c, c == c0) + R * D + mr));
+        }
+        top = across(top, [](float x, float y) { return fmaxf(x, y); });
+        if (lane < R) ml[0][warp][mr] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[0][w][mr]);
+        float l = 0.0f;
+        if (mr < rows) {
+#pragma unroll 4
+          for (int c = from; c <= c1; c += kStep) {
+            const float* p = P::slot(a.ws, c, c == c0) + R * D + mr;
+            const float f = exp2_(__ldcg(p) - top);
+            weight[(c - c0) * R + mr] = f;
+            l = fmaf(f, __ldcg(p + R), l);
+          }
+        }
+        l = across(l, [](float x, float y) { return x + y; });
+        if (lane < R) ml[1][warp][mr] = l;
+        __syncthreads();
+        auto row_sum = [&](int r) {
+          float t = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) t += ml[1][w][r];
+          return t;
+        };
+        const int columns = rows * (D / 4), split = max(1, kThreads / columns);
+        for (int k = tid; k < columns * split; k += kThreads) {
+          const int of = split > 1 ? k / columns : 0, column = k - of * columns;
+          const int r = column / (D / 4), d = column % (D / 4) * 4;
+          float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+          for (int c = of; c < parts; c += split) {
+            const float f = weight[c * R + r];
+            const float4 v = __ldcg((const float4*)(P::slot(a.ws, c0 + c, c == 0) + r * D + d));
             sum.x = fmaf(f, v.x, sum.x), sum.y = fmaf(f, v.y, sum.y), sum.z = fmaf(f, v.z, sum.z), sum.w = fmaf(f, v.w, sum.w);
           }
-          write_row(r, d, sum, l);
+          if (split == 1) write_row(r, d, sum, row_sum(r));
+          else shares_of[k] = sum;
+        }
+        if (split > 1) {
+          __syncthreads();
+          if (tid < columns) {
+            float4 sum = shares_of[tid];
+            for (int of = 1; of < split; ++of) {
+              const float4 v = shares_of[of * columns + tid];
+              sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            }
+            write_row(tid / (D / 4), tid % (D / 4) * 4, sum, row_sum(tid / (D / 4)));
+          }
         }
       }
     }
@@ -667,6 +719,7 @@ template <int NG, int NB>
 void launch_tokens(fopt_ctx* ctx, const AttnArgs& a, int sms) {
   using S = Shared<NG, NB>;
   static std::atomic<uint64_t> done;
+  require(sms * tokens_blocks<NG, NB>() * S::R * 4 <= S::kBytes, "fopt_cache_attention: more resident blocks than a block adds up");
   allow_shared(ctx, done, (const void*)tokens_kernel<NG, NB>, S::kBytes);
   tokens_kernel<NG, NB><<<sms * tokens_blocks<NG, NB>(), kThreads, S::kBytes, ctx->stream>>>(a);
   launched(ctx, "cache attention");
