@@ -74,29 +74,44 @@ struct Shares {
 
 // Where a block's share begins: the line's length, the blocks that have a share, and the sequence in which this
 // one's begins with the position of that sequence's first unit. For all threads of the block, with `units(b)`
-// the length of sequence b and shares of at least `least` units (adding up parts costs, too); blocks without a
-// share get blocks <= blockIdx.x.
+// the length of sequence b, and `segment(b)` that of its longest segment. Shares have at least `least` units, and
+// `by_root` sqrt(the longest segment): one block adds up a segment's parts one after the other, so n units in shares
+// of u take u + (n / u) times what a part costs, least at u ~ sqrt(n). Blocks without a share get
+// blocks <= blockIdx.x.
 struct Start {
   long long total, seq_at;
   int blocks, b;
 };
-template <int THREADS, typename Units>
-__device__ __forceinline__ Start share_start(int batch, int least, Units units) {
+template <int THREADS, typename Units, typename Segment>
+__device__ __forceinline__ Start share_start(int batch, int least, float by_root, Units units, Segment segment) {
   constexpr int kW = THREADS / 32;
   __shared__ long long sums[kW];
+  __shared__ int tops[kW];
   __shared__ long long found_at;
   __shared__ int found;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long first = tid < batch ? units(tid) : 0;
   long long total = first;
-  for (int b = tid + THREADS; b < batch; b += THREADS) total += units(b);
+  int top = tid < batch ? segment(tid) : 0;
+  for (int b = tid + THREADS; b < batch; b += THREADS) {
+    total += units(b);
+    top = max(top, segment(b));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) sums[warp] = total;
+  if (lane == 0) {
+    sums[warp] = total;
+    tops[warp] = top;
+  }
   __syncthreads();
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kW; ++w) total += sums[w];
+  for (int w = 0; w < kW; ++w) {
+    total += sums[w];
+    top = max(top, tops[w]);
+  }
+  least = max(least, (int)(by_root * sqrtf((float)top)));
   Start st{total, 0, (int)min((long long)gridDim.x, (total + least - 1) / least), 0};
   if ((int)blockIdx.x >= st.blocks) return st;
   const long long unit = Shares(total, st.blocks).first(blockIdx.x);

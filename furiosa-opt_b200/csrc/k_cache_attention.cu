@@ -39,7 +39,10 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kTileTokens = 16 * kWarps;
 constexpr int kBlocks = 3;       // resident blocks an SM, where the registers allow (168 a thread)
 constexpr int kSegmentCost = 4;  // beginning and ending a segment takes about as long as this many tiles
-constexpr int kLeast = 2;        // tiles of a share: a part more to add up takes about as long as one
+constexpr int kLeast = 2;        // tiles of a share
+// A part more to add up takes about a sixth of a tile. Shares of 2 tiles were best at 777 tokens of 8 heads
+// (12.4 us; 14.0 with 4), of 8 at 15179 of two heads (20.6; 29.3 with 2), of 8 to 16 at 131072 of one (24.8; 26.8 with 5).
+constexpr float kByRoot = 0.4f;
 constexpr int kStages = 4;
 constexpr float kLazy = 8.0f;    // log2 by which a score may exceed the running maximum before it moves
 constexpr int kFewRows = 32;     // query rows per key head up to which a sequence is tokens_kernel's
@@ -424,7 +427,12 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
 
   // rows_kernel, if it is launched behind, may begin: it works on other sequences, in memory of its own
   asm volatile("griddepcontrol.launch_dependents;");
-  const Start start = share_start<kThreads>(a.batch, kLeast, [&](int b) { return units<R>(a, sequence(a, b)); });
+  const Start start = share_start<kThreads>(
+      a.batch, kLeast, kByRoot, [&](int b) { return units<R>(a, sequence(a, b)); },
+      [&](int b) {
+        const Seq s = sequence(a, b);
+        return s.rows >= a.long_rows ? 0 : tiles_of(s);
+      });
   if ((int)blockIdx.x >= start.blocks) return;
   const Shares shares(start.total, start.blocks);
   long long unit = shares.first(blockIdx.x);

@@ -43,7 +43,10 @@ constexpr int kExpand = 7, kRowThreads = 32 * (1 + kExpand + 8);  // warps that 
 constexpr int kHalf = 16384;             // 128 rows of 64 f16 (128 bytes), the unit of the swizzled tiles
 constexpr int kOffsets = 128 * 32;        // 128 rows of 16 f16: the sums of a tile's q, or the offsets of a key tile
 constexpr int kCost = 2;                 // key tiles that beginning and ending a segment takes as long as
-constexpr int kLeast = 4;                // units of a share: a part more to add up takes about as long as a tile
+constexpr int kLeast = 4;                // units of a share
+// A part more to add up (66 KB for each of two tiles, by one SM) takes about as long as a unit. Of 16 tokens at 131072
+// keys of one head of 8 query heads: 159 us; 347 without this rule, in shares of 7 units.
+constexpr float kByRoot = 1.0f;
 constexpr int kUncut = 8;                // segments of fewer tiles are not shared between blocks
 constexpr float kLazyRows = 14.0f;        // log2 by which x may exceed its base: P stays within f16, the base moves rarely
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -271,7 +274,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
   int* last = (int*)(tmem_slot + 2);    // [2]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Start start = share_start<kRowThreads>(a.batch, kLeast, [&](int b) { return units(a, sequence(a, b)); });
+  const Start start = share_start<kRowThreads>(
+      a.batch, kLeast, kByRoot, [&](int b) { return units(a, sequence(a, b)); },
+      [&](int b) {
+        const Seq s = sequence(a, b);
+        return s.rows < a.long_rows ? 0 : tiles_of(a, s, blocks_of(s) - 1);
+      });
   // The launch does not wait for tokens_kernel's end (they share nothing); this kernel's end does, for what follows.
   if ((int)blockIdx.x >= start.blocks) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -553,12 +561,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_after();
-        const bool whole = done.t0 == 0 && done.t1 == done.tiles;
+        const bool whole = done.t0 == 0 && done.t1 == done.tiles, rows = done.row0 + t * 128 < done.s.rows;
         // partial results: [D / 4][128] float4, so that a warp's rows are contiguous, then maxima and sums
         auto slot = [&](int block, bool begins) { return a.ws + ((int64_t)block * 2 + begins) * T::kSlot + t * 128 * (D + 2); };
         int c0 = 0, c1 = 0;
-        bool output = true;
-        if (!whole) {
+        bool output = rows;
+        if (!whole && rows) {
           float* part = slot(blockIdx.x, done.t0 == 0);
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
