@@ -139,81 +139,32 @@ struct RotaryArgs {
   const int32_t* positions;
   int64_t x_stride, out_stride;
   int tokens, heads, dim;
+  int each;          // tokens a block
   int units;         // per head: 8-channel chunks (pairs of them for HALF) when vectorised, pairs or channels if not
-  FastDiv by_units;
+  FastDiv by_units, by_heads;
 };
 
-// TB tokens a block, a thread with the same unit of each. The first units' values are on their way while the
-// angles are computed (the sines take about as long as the loads).
-template <bool F32, bool VEC, int TB>
+// A block has `each` tokens. With vectors their units are one range, of which a thread has AHEAD at a time, a block's
+// threads apart, on their way while the angles are computed (the sines take about as long as the loads). Without,
+// most time goes into addresses, so a thread takes the same unit of each token (as one range, 45 us where this
+// takes 35: 5878 tokens of 21 heads of 97 in bf16).
+template <bool F32, bool VEC, int AHEAD>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, const __grid_constant__ Rope r) {
   using E = Elem<F32>;
+  using T = typename E::T;
   extern __shared__ float2 cs[];
-  const int t0 = blockIdx.x * TB, n = min(TB, a.tokens - t0);
-  const int per_token = a.heads * a.units;
-  bool turned = false;
-  for (int k = threadIdx.x; !turned || k < per_token; k += kThreads) {
-    const bool live = k < per_token;
-    const int h = live ? (int)fdiv(a.by_units, (uint32_t)k) : 0, u = live ? k - h * a.units : 0;
-    const auto* x = (const typename E::T*)a.x + (int64_t)t0 * a.x_stride + (int64_t)h * a.dim;
-    auto* o = (typename E::T*)a.out + (int64_t)t0 * a.out_stride + (int64_t)h * a.dim;
-    if constexpr (VEC) {
-      const bool rotated = r.interleaved ? 4 * u < r.pairs : 8 * u < r.pairs;
-      // past the rotated channels units count on in whole chunks
-      const int at = r.interleaved || rotated ? 8 * u : 8 * u + r.pairs;
-      Raw<F32> v[TB], w[TB];
-#pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        if (!live || t >= n) continue;
-        v[t].load(x + t * a.x_stride + at);
-        if (rotated && !r.interleaved) w[t].load(x + t * a.x_stride + at + r.pairs);
-      }
-      if (!turned) {
-        angles(cs, r, a.positions + t0, n);
-        __syncthreads();
-        turned = true;
-      }
-#pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        if (!live || t >= n) continue;
-        const float2* c = cs + t * r.pairs;
-        auto* to = o + t * a.out_stride + at;
-        if (!rotated) {
-          v[t].store(to);
-        } else if (r.interleaved) {
-          float p[8], y[8];
-          v[t].values(p);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            y[2 * i] = turned_first(p[2 * i], p[2 * i + 1], c[4 * u + i]);
-            y[2 * i + 1] = turned_second(p[2 * i], p[2 * i + 1], c[4 * u + i]);
-          }
-          store_n<F32, 8>(to, y);
-        } else {
-          float p[8], q[8], y[8];
-          v[t].values(p);
-          w[t].values(q);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            y[i] = turned_first(p[i], q[i], c[8 * u + i]);
-            q[i] = turned_second(p[i], q[i], c[8 * u + i]);
-          }
-          store_n<F32, 8>(to, y);
-          store_n<F32, 8>(to + r.pairs, q);
-        }
-      }
-    } else {
-      if (!turned) {
-        angles(cs, r, a.positions + t0, n);
-        __syncthreads();
-        turned = true;
-      }
-      for (int t = 0; live && t < n; ++t) {
-        const auto* from = x + t * a.x_stride;
-        auto* to = o + t * a.out_stride;
+  const int t0 = blockIdx.x * a.each, n = min(a.each, a.tokens - t0);
+  if constexpr (!VEC) {
+    angles(cs, r, a.positions + t0, n);
+    __syncthreads();
+    for (int k = threadIdx.x; k < a.heads * a.units; k += kThreads) {
+      const int h = (int)fdiv(a.by_units, (uint32_t)k), u = k - h * a.units;
+      const T* from = (const T*)a.x + t0 * a.x_stride + (int64_t)h * a.dim;
+      T* to = (T*)a.out + t0 * a.out_stride + (int64_t)h * a.dim;
+      const int i = r.interleaved ? 2 * u : u, j = r.interleaved ? 2 * u + 1 : u + r.pairs;
+      for (int t = 0; t < n; ++t, from += a.x_stride, to += a.out_stride) {
         if (u < r.pairs) {
           const float2 c = cs[t * r.pairs + u];
-          const int i = r.interleaved ? 2 * u : u, j = r.interleaved ? 2 * u + 1 : u + r.pairs;
           const float p = E::load(from + i), q = E::load(from + j);
           E::store(to + i, turned_first(p, q, c));
           E::store(to + j, turned_second(p, q, c));
@@ -221,6 +172,61 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, const __
           to[u + r.pairs] = from[u + r.pairs];
         }
       }
+    }
+    return;
+  }
+  const int total = n * a.heads * a.units;
+  bool turned = false;
+  for (int k0 = threadIdx.x; !turned || k0 < total; k0 += kThreads * AHEAD) {
+    T* to[AHEAD];
+    const float2* c[AHEAD];
+    bool rotated[AHEAD];
+    Raw<F32> v[AHEAD], w[AHEAD];  // the unit's values and, of pairs that lie apart, the second ones
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int k = k0 + i * kThreads;
+      if (k >= total) continue;
+      const int row = (int)fdiv(a.by_units, (uint32_t)k), u = k - row * a.units;
+      const int t = (int)fdiv(a.by_heads, (uint32_t)row), h = row - t * a.heads;
+      rotated[i] = r.interleaved ? 4 * u < r.pairs : 8 * u < r.pairs;
+      // past the rotated channels units count on in whole chunks
+      const int64_t at = (int64_t)h * a.dim + (r.interleaved || rotated[i] ? 8 * u : 8 * u + r.pairs);
+      const T* from = (const T*)a.x + (t0 + t) * a.x_stride + at;
+      to[i] = (T*)a.out + (t0 + t) * a.out_stride + at;
+      c[i] = cs + t * r.pairs + (r.interleaved ? 4 * u : 8 * u);
+      v[i].load(from);
+      if (rotated[i] && !r.interleaved) w[i].load(from + r.pairs);
+    }
+    if (!turned) {
+      angles(cs, r, a.positions + t0, n);
+      __syncthreads();
+      turned = true;
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (k0 + i * kThreads >= total) continue;
+      if (!rotated[i]) {
+        v[i].store(to[i]);
+        continue;
+      }
+      float x[8], y[8], z[8];
+      v[i].values(x);
+      if (r.interleaved) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[2 * e] = turned_first(x[2 * e], x[2 * e + 1], c[i][e]);
+          y[2 * e + 1] = turned_second(x[2 * e], x[2 * e + 1], c[i][e]);
+        }
+      } else {
+        w[i].values(z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          y[e] = turned_first(x[e], z[e], c[i][e]);
+          z[e] = turned_second(x[e], z[e], c[i][e]);
+        }
+        store_n<F32, 8>(to[i] + r.pairs, z);
+      }
+      store_n<F32, 8>(to[i], y);
     }
   }
 }
@@ -450,55 +456,63 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, const __
 }
 
 // ---- read ----
-// The same words, TB slots a block: 8 neighbouring channels of a key, or 4 of each of two groups of a value.
-template <bool F32, int NG, int TB>
+// A thread per word, as they are stored: 8 neighbouring channels of a key, or 4 of each of two groups of a value;
+// AHEAD words, a block's threads apart, on their way at a time. Slots and heads are one range, so that few heads fill
+// blocks too.
+template <bool F32, int NG, int AHEAD>
 __global__ void __launch_bounds__(kThreads) read_kernel(Cache cache, void* out_k, void* out_v, const int32_t* slots,
-                                                        int n, int32_t* err) {
+                                                        int64_t rows, FastDiv by_heads, int32_t* err) {
   using E = Elem<F32>;
-  constexpr int D = NG * kGroup, W = D / 8;
-  const int capacity = cache.pages * cache.page_size, items = 2 * cache.heads * W;
-  const int t0 = blockIdx.x * TB, m = min(TB, n - t0);
-  for (int item = threadIdx.x; item < items; item += kThreads) {
-    const int w = item % W;
-    const bool value = item >= cache.heads * W;
-    const int h = item / W - (value ? cache.heads : 0);
-    uint32_t codes[TB];
-    uint2 scale[TB];
-    int slot[TB];
-    bool there[TB];
+  constexpr int D = NG * kGroup, W = D / 8, kEach = kThreads / W;  // words a row, rows that a block has at a time
+  const int w = threadIdx.x % W;
+  const bool value = blockIdx.y;
+  const uint8_t* codes = value ? cache.v : cache.k;
+  const uint32_t* scales = value ? cache.v_scale : cache.k_scale;
+  const int64_t row0 = (int64_t)blockIdx.x * (kEach * AHEAD) + threadIdx.x / W;
+  uint32_t code[AHEAD];
+  uint2 scale[AHEAD];
+  int slot[AHEAD], head[AHEAD];
 #pragma unroll
-    for (int t = 0; t < TB; ++t) slot[t] = t < m ? slots[t0 + t] : -1;
+  for (int i = 0; i < AHEAD; ++i) {
+    const int64_t row = row0 + i * kEach;
+    slot[i] = -1;
+    if (row >= rows) continue;
+    const int at = (int)fdiv(by_heads, (uint32_t)row);
+    head[i] = (int)row - at * cache.heads;
+    slot[i] = slots[at];
+  }
 #pragma unroll
-    for (int t = 0; t < TB; ++t) {
-      there[t] = slot[t] >= 0 && slot[t] < capacity;
-      if (slot[t] >= capacity) atomicExch(err, kBadSlot);
-      if (!there[t]) continue;
-      const int64_t from = row_of(cache, slot[t], h);
-      codes[t] = __ldg((const uint32_t*)((value ? cache.v : cache.k) + from * (D / 2)) + w);
-      const uint32_t* s = (value ? cache.v_scale : cache.k_scale) + from * NG;
-      if (value) scale[t] = __ldg((const uint2*)s + w % (NG / 2));
-      else scale[t].x = scale[t].y = __ldg(s + w % NG);
+  for (int i = 0; i < AHEAD; ++i) {
+    if (slot[i] >= cache.pages * cache.page_size) {
+      atomicExch(err, kBadSlot);
+      slot[i] = -1;
     }
-    const int d = value ? (w % (NG / 2)) * 2 * kGroup + (w / (NG / 2)) * 4 : (w % NG) * kGroup + (w / NG) * 8;
-    auto* o = (typename E::T*)(value ? out_v : out_k) + ((int64_t)t0 * cache.heads + h) * D + d;
+    if (slot[i] < 0) continue;
+    const int64_t from = row_of(cache, slot[i], head[i]);
+    code[i] = __ldg((const uint32_t*)(codes + from * (D / 2)) + w);
+    const uint32_t* s = scales + from * NG;
+    if (value) scale[i] = __ldg((const uint2*)s + w % (NG / 2));
+    else scale[i].x = scale[i].y = __ldg(s + w % NG);
+  }
+  const int d = value ? (w % (NG / 2)) * 2 * kGroup + (w / (NG / 2)) * 4 : (w % NG) * kGroup + (w / NG) * 8;
+  auto* out = (typename E::T*)(value ? out_v : out_k) + d;
 #pragma unroll
-    for (int t = 0; t < TB; ++t) {
-      if (!there[t]) continue;
-      float y[8];
+  for (int i = 0; i < AHEAD; ++i) {
+    if (slot[i] < 0) continue;
+    float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t q = e < 4 ? scale[t].x : scale[t].y;
-        // 2^23 + code + 8, as the four bits with their highest turned over
-        const float c = __uint_as_float((codes[t] >> (4 * e) & 15u) ^ 0x4b000008u) - (0x1p23f + 8.0f);
-        y[e] = fmaf(c, __uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u));
-      }
-      auto* to = o + (int64_t)t * cache.heads * D;
-      if (!value) {
-        store_n<F32, 8>(to, y);
-      } else {
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t q = e < 4 ? scale[i].x : scale[i].y;
+      // 2^23 + code + 8, as the four bits with their highest turned over
+      const float c = __uint_as_float((code[i] >> (4 * e) & 15u) ^ 0x4b000008u) - (0x1p23f + 8.0f);
+      y[e] = fmaf(c, __uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u));
+    }
+    auto* to = out + (row0 + i * kEach) * D;
+    if (!value) {
+      store_n<F32, 8>(to, y);
+    } else {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) store_n<F32, 4>(to + half * kGroup, y + 4 * half);
-      }
+      for (int half = 0; half < 2; ++half) store_n<F32, 4>(to + half * kGroup, y + 4 * half);
     }
   }
 }
@@ -524,13 +538,14 @@ void launch_append(fopt_ctx* ctx, AppendArgs a, const Rope& r, int dim) {
 }
 
 template <bool F32, bool VEC>
-void launch_rotary(fopt_ctx* ctx, const RotaryArgs& a, const Rope& r, bool wide) {
-  // two tokens a block once there are blocks enough for the SMs: 16.5 us for 4096 tokens of 32 heads of 128 in
-  // bf16, against 18.5 with one and 17.6 with four, whose registers leave two blocks to an SM
-  if (wide)
-    rotary_kernel<F32, VEC, 2><<<(a.tokens + 1) / 2, kThreads, 2 * r.pairs * sizeof(float2), ctx->stream>>>(a, r);
-  else
-    rotary_kernel<F32, VEC, 1><<<a.tokens, kThreads, r.pairs * sizeof(float2), ctx->stream>>>(a, r);
+void launch_rotary(fopt_ctx* ctx, RotaryArgs a, const Rope& r) {
+  constexpr int kAhead = 2;
+  // tokens enough to occupy a block's threads kAhead times over (12 us for 14598 tokens of 3 heads of 128 in bf16,
+  // against 19 with two tokens a block), but not so many that SMs go without
+  const int64_t per_token = (int64_t)a.heads * a.units, sms = sm_count(ctx);
+  const int64_t fill = VEC ? std::min<int64_t>(kThreads * kAhead / per_token, 2048 / r.pairs) : 4;
+  a.each = (int)std::max<int64_t>(1, std::min(fill, a.tokens / (2 * sms)));
+  rotary_kernel<F32, VEC, kAhead><<<(a.tokens + a.each - 1) / a.each, kThreads, a.each * r.pairs * sizeof(float2), ctx->stream>>>(a, r);
   launched(ctx, "rotary");
 }
 
@@ -589,7 +604,7 @@ fopt_status fopt_rotary(fopt_ctx* ctx, void* out, const void* x, fopt_dtype dtyp
     const kv::Rope& r = rope->r;
     require(2 * r.pairs <= head_dim, "fopt_rotary: more rotated channels than the head has");
     const int64_t row = (int64_t)heads * head_dim;
-    require(row <= INT32_MAX, "fopt_rotary: a token's heads past 2^31 elements");
+    require(row <= 1 << 30, "fopt_rotary: a token's heads past 2^30 elements");
     require(x_stride >= row && out_stride >= row, "fopt_rotary: a token stride below heads * head_dim");
     require(out != x || x_stride == out_stride, "fopt_rotary: in place needs equal strides");
     if (ctx && tokens == 0) return;
@@ -602,10 +617,10 @@ fopt_status fopt_rotary(fopt_ctx* ctx, void* out, const void* x, fopt_dtype dtyp
     const bool vec = head_dim % 8 == 0 && (2 * r.pairs) % 8 == 0 && (r.interleaved || r.pairs % 8 == 0) &&
                      kv::aligned16(x, x_stride, sz) && kv::aligned16(out, out_stride, sz);
     const int units = vec ? (r.interleaved ? 2 * r.pairs : r.pairs) / 8 + tail / 8 : r.pairs + tail;
-    kv::RotaryArgs a{out, x, positions, x_stride, out_stride, tokens, heads, head_dim, units, make_fastdiv((uint32_t)units)};
-    const bool wide = tokens >= 4 * sm_count(ctx);
-    if (f32) vec ? kv::launch_rotary<true, true>(ctx, a, r, wide) : kv::launch_rotary<true, false>(ctx, a, r, wide);
-    else vec ? kv::launch_rotary<false, true>(ctx, a, r, wide) : kv::launch_rotary<false, false>(ctx, a, r, wide);
+    kv::RotaryArgs a{out, x, positions, x_stride, out_stride, tokens, heads, head_dim, 1, units, make_fastdiv((uint32_t)units),
+                     make_fastdiv((uint32_t)heads)};
+    if (f32) vec ? kv::launch_rotary<true, true>(ctx, a, r) : kv::launch_rotary<true, false>(ctx, a, r);
+    else vec ? kv::launch_rotary<false, true>(ctx, a, r) : kv::launch_rotary<false, false>(ctx, a, r);
   });
 }
 
@@ -649,20 +664,23 @@ fopt_status fopt_cache_read(fopt_ctx* ctx, void* out_k, void* out_v, fopt_dtype 
   return kv::checked_call(ctx, [&] {
     const kv::Cache c = kv::checked(cache, "fopt_cache_read");
     require(dtype == FOPT_BF16 || dtype == FOPT_F32, "fopt_cache_read: bf16 or f32 values");
-    require(n >= 0, "fopt_cache_read: a negative slot count");
+    require(n >= 0 && (int64_t)n * c.heads <= INT32_MAX, "fopt_cache_read: slots times heads below 0 or past 2^31");
     if (ctx && n == 0) return;
     require(out_k && out_v && slots, "fopt_cache_read: null argument");
     require(((uintptr_t)out_k | (uintptr_t)out_v) % 16 == 0, "fopt_cache_read: outputs must be 16-byte aligned");
     require(ctx != nullptr, "null context");
     DeviceGuard guard(ctx);
     const int dim = cache->head_dim;
-    auto go = [&](auto kernel, int slots_each) {
-      kernel<<<(n + slots_each - 1) / slots_each, kv::kThreads, 0, ctx->stream>>>(c, out_k, out_v, slots, n, ctx->dev_err);
+    const int64_t rows = (int64_t)n * c.heads;
+    auto go = [&](auto kernel, int ahead) {
+      const int64_t each = kv::kThreads / (dim / 8) * ahead;
+      kernel<<<dim3((unsigned)((rows + each - 1) / each), 2), kv::kThreads, 0, ctx->stream>>>(
+          c, out_k, out_v, slots, rows, make_fastdiv((uint32_t)c.heads), ctx->dev_err);
       launched(ctx, "cache read");
     };
-    // loads of four slots on their way at a time, once there are blocks enough for the SMs (9.3 us for 4096 slots of
-    // 8 heads of 128 to bf16, against 10.4 with one)
-    auto sized = [&](auto one, auto four) { n >= 4 * sm_count(ctx) ? go(four, 4) : go(one, 1); };
+    // four words of a thread on their way at a time, once there are blocks enough for the SMs
+    const bool many = rows * (dim / 8) >= (int64_t)8 * kv::kThreads * sm_count(ctx);
+    auto sized = [&](auto one, auto four) { many ? go(four, 4) : go(one, 1); };
     if (dtype == FOPT_F32)
       dim == 64    ? sized(kv::read_kernel<true, 2, 1>, kv::read_kernel<true, 2, 4>)
       : dim == 128 ? sized(kv::read_kernel<true, 4, 1>, kv::read_kernel<true, 4, 4>)
