@@ -110,8 +110,10 @@ struct Raw {
   }
 };
 
-// (cos, sin) of the first `n` tokens' pairs, from their positions, into shared memory [token][pair].
-__device__ __forceinline__ void angles(float2* cs, const Rope& r, const int32_t* positions, int n) {
+// (cos, sin) of the first `n` tokens' pairs, from their positions, into shared memory: [token][pair], or, for threads
+// that take 2^shift neighbouring pairs each, [token][two of a thread's pairs][thread][pair of the two], since lanes
+// that read 64 bytes apart share banks (which made the rotation of 4096 tokens of 32 heads of 128 take TIME).
+__device__ __forceinline__ void angles(float2* cs, const Rope& r, const int32_t* positions, int n, int shift) {
   // by a plain address: lanes that differ in it take turns at the constant bank
   const unsigned long long* turn = r.turn;
   asm("" : "+l"(turn));
@@ -121,8 +123,15 @@ __device__ __forceinline__ void angles(float2* cs, const Rope& r, const int32_t*
     const double half = (double)(long long)((unsigned long long)(long long)positions[t] * turn[p]) * 0x1p-63;
     double s, c;
     sincospi(half, &s, &c);
-    cs[k] = make_float2((float)(c * r.magnitude), (float)(s * r.magnitude));
+    const int to = shift ? t * r.pairs + ((((p & ((1 << shift) - 1)) >> 1) * (r.pairs >> shift) + (p >> shift)) << 1 | (p & 1)) : k;
+    cs[to] = make_float2((float)(c * r.magnitude), (float)(s * r.magnitude));
   }
+}
+// N of them from the place of the first two, with `units` threads' pairs between.
+template <int N>
+__device__ __forceinline__ void load_angles(float2* c, const float2* at, int units) {
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) *(float4*)(c + 2 * i) = *(const float4*)(at + 2 * i * units);
 }
 
 __device__ __forceinline__ float turned_first(float a, float b, float2 cs) {
@@ -152,10 +161,10 @@ template <bool F32, bool VEC, int AHEAD>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, const __grid_constant__ Rope r) {
   using E = Elem<F32>;
   using T = typename E::T;
-  extern __shared__ float2 cs[];
+  extern __shared__ __align__(16) float2 cs[];
   const int t0 = blockIdx.x * a.each, n = min(a.each, a.tokens - t0);
   if constexpr (!VEC) {
-    angles(cs, r, a.positions + t0, n);
+    angles(cs, r, a.positions + t0, n, 0);
     __syncthreads();
     for (int k = threadIdx.x; k < a.heads * a.units; k += kThreads) {
       const int h = (int)fdiv(a.by_units, (uint32_t)k), u = k - h * a.units;
@@ -175,7 +184,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, const __
     }
     return;
   }
-  const int total = n * a.heads * a.units;
+  const int total = n * a.heads * a.units, shift = r.interleaved ? 2 : 3;
   bool turned = false;
   for (int k0 = threadIdx.x; !turned || k0 < total; k0 += kThreads * AHEAD) {
     T* to[AHEAD];
@@ -193,12 +202,12 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, const __
       const int64_t at = (int64_t)h * a.dim + (r.interleaved || rotated[i] ? 8 * u : 8 * u + r.pairs);
       const T* from = (const T*)a.x + (t0 + t) * a.x_stride + at;
       to[i] = (T*)a.out + (t0 + t) * a.out_stride + at;
-      c[i] = cs + t * r.pairs + (r.interleaved ? 4 * u : 8 * u);
+      c[i] = cs + t * r.pairs + 2 * u;
       v[i].load(from);
       if (rotated[i] && !r.interleaved) w[i].load(from + r.pairs);
     }
     if (!turned) {
-      angles(cs, r, a.positions + t0, n);
+      angles(cs, r, a.positions + t0, n, shift);
       __syncthreads();
       turned = true;
     }
@@ -210,19 +219,22 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, const __
         continue;
       }
       float x[8], y[8], z[8];
+      float2 k[8];
       v[i].values(x);
       if (r.interleaved) {
+        load_angles<4>(k, c[i], r.pairs >> 2);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          y[2 * e] = turned_first(x[2 * e], x[2 * e + 1], c[i][e]);
-          y[2 * e + 1] = turned_second(x[2 * e], x[2 * e + 1], c[i][e]);
+          y[2 * e] = turned_first(x[2 * e], x[2 * e + 1], k[e]);
+          y[2 * e + 1] = turned_second(x[2 * e], x[2 * e + 1], k[e]);
         }
       } else {
+        load_angles<8>(k, c[i], r.pairs >> 3);
         w[i].values(z);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          y[e] = turned_first(x[e], z[e], c[i][e]);
-          z[e] = turned_second(x[e], z[e], c[i][e]);
+          y[e] = turned_first(x[e], z[e], k[e]);
+          z[e] = turned_second(x[e], z[e], k[e]);
         }
         store_n<F32, 8>(to[i] + r.pairs, z);
       }
@@ -243,7 +255,8 @@ struct AppendArgs {
   int tokens;
   int each;          // tokens a block
   FastDiv by_heads;
-  int k_vec, v_vec, pair_vec;  // whole-vector loads of k, of v, and of the other half of k's pairs
+  int k_vec, v_vec;  // whole-vector loads of k and of v
+  int pair_vec;      // a thread's eight channels are of whole pairs or of none, the other halves' too and read as vectors
 };
 
 constexpr float kLargest = 0x1p100f;
@@ -301,7 +314,7 @@ template <bool F32, int NG>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, const __grid_constant__ Rope r) {
   constexpr int D = NG * kGroup, W = D / 16;
   constexpr uint32_t kAll = 0xffffffffu;
-  extern __shared__ float2 cs[];
+  extern __shared__ __align__(16) float2 cs[];
   const int t0 = blockIdx.x * a.each, n = min(a.each, a.tokens - t0), heads = a.cache.heads;
   const int keys = n * heads * W, items = 2 * keys;
   const int lane = threadIdx.x & 31;
@@ -352,7 +365,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, const __
     if (!turned) {
       // values do not wait for the angles: items go from keys to values, so a warp without keys now has none later
       if (r.pairs) {
-        angles(cs, r, a.positions + t0, n);
+        angles(cs, r, a.positions + t0, n, !a.pair_vec ? 0 : r.interleaved ? 2 : 3);
         if (base < keys) asm volatile("barrier.cta.sync 1, %0;" ::"n"(kThreads) : "memory");
         else asm volatile("barrier.cta.arrive 1, %0;" ::"n"(kThreads) : "memory");
       }
@@ -365,23 +378,29 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, const __
       const int c = d + 8 * i;
       if (value || c >= 2 * r.pairs) continue;
       const float2* k = cs + t * r.pairs;
+      float2 turn[8];
       if (r.interleaved) {
+        if (a.pair_vec) {
+          load_angles<4>(turn, k + (c >> 3) * 2, r.pairs >> 2);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          if (c + e < 2 * r.pairs) {
-            const float2 turn = k[(c + e) >> 1];
-            const float p = f[i][e], q = f[i][e + 1];
-            f[i][e] = turned_first(p, q, turn);
-            f[i][e + 1] = turned_second(p, q, turn);
+          for (int e = 0; e < 4; ++e) turn[e] = k[min((c >> 1) + e, r.pairs - 1)];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((c >> 1) + e < r.pairs) {
+            const float p = f[i][2 * e], q = f[i][2 * e + 1];
+            f[i][2 * e] = turned_first(p, q, turn[e]);
+            f[i][2 * e + 1] = turned_second(p, q, turn[e]);
           }
         }
       } else {
         float other[8];
         y[i].values(other);
         if (a.pair_vec) {
-          k += c < r.pairs ? c : c - r.pairs;
+          load_angles<8>(turn, k + ((c < r.pairs ? c : c - r.pairs) >> 3) * 2, r.pairs >> 3);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[i][e] = __fadd_rn(__fmul_rn(f[i][e], k[e].x), __fmul_rn(other[e], k[e].y));
+          for (int e = 0; e < 8; ++e) f[i][e] = __fadd_rn(__fmul_rn(f[i][e], turn[e].x), __fmul_rn(other[e], turn[e].y));
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -654,7 +673,7 @@ fopt_status fopt_cache_append(fopt_ctx* ctx, const fopt_paged_cache* cache, cons
     a.tokens = tokens;
     a.k_vec = kv::aligned16(k, k_stride, f32 ? 4 : 2);
     a.v_vec = kv::aligned16(v, v_stride, f32 ? 4 : 2);
-    a.pair_vec = a.k_vec && r.pairs % 8 == 0;
+    a.pair_vec = r.interleaved ? r.pairs % 4 == 0 : a.k_vec && r.pairs % 8 == 0;
     f32 ? kv::launch_append<true>(ctx, a, r, dim) : kv::launch_append<false>(ctx, a, r, dim);
   });
 }
