@@ -112,7 +112,7 @@ struct Raw {
 
 // (cos, sin) of the first `n` tokens' pairs, from their positions, into shared memory: [token][pair], or, for threads
 // that take 2^shift neighbouring pairs each, [token][two of a thread's pairs][thread][pair of the two], since lanes
-// that read 64 bytes apart share banks (which made the rotation of 4096 tokens of 32 heads of 128 take TIME).
+// that read 64 bytes apart share banks (which made the rotation of 4096 tokens of 32 heads of 128 take 16.5 us, not 12.4).
 __device__ __forceinline__ void angles(float2* cs, const Rope& r, const int32_t* positions, int n, int shift) {
   // by a plain address: lanes that differ in it take turns at the constant bank
   const unsigned long long* turn = r.turn;
@@ -475,64 +475,42 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, const __
 }
 
 // ---- read ----
-// A thread per word, as they are stored: 8 neighbouring channels of a key, or 4 of each of two groups of a value;
-// AHEAD words, a block's threads apart, on their way at a time. Slots and heads are one range, so that few heads fill
-// blocks too.
-template <bool F32, int NG, int AHEAD>
+// A thread per word, as they are stored: 8 neighbouring channels of a key, or 4 of each of two groups of a value.
+// Slots and heads are one range, so that few heads fill blocks too. (10.4 us for 4608 slots of 8 heads of 128 to
+// bf16, with one, two, four or eight words of a thread on their way.)
+template <bool F32, int NG>
 __global__ void __launch_bounds__(kThreads) read_kernel(Cache cache, void* out_k, void* out_v, const int32_t* slots,
                                                         int64_t rows, FastDiv by_heads, int32_t* err) {
   using E = Elem<F32>;
-  constexpr int D = NG * kGroup, W = D / 8, kEach = kThreads / W;  // words a row, rows that a block has at a time
+  constexpr int D = NG * kGroup, W = D / 8;
   const int w = threadIdx.x % W;
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / W) + threadIdx.x / W;
+  if (row >= rows) return;
+  const int at = (int)fdiv(by_heads, (uint32_t)row), head = (int)row - at * cache.heads, slot = slots[at];
+  if (slot >= cache.pages * cache.page_size) atomicExch(err, kBadSlot);
+  if (slot < 0 || slot >= cache.pages * cache.page_size) return;
   const bool value = blockIdx.y;
-  const uint8_t* codes = value ? cache.v : cache.k;
-  const uint32_t* scales = value ? cache.v_scale : cache.k_scale;
-  const int64_t row0 = (int64_t)blockIdx.x * (kEach * AHEAD) + threadIdx.x / W;
-  uint32_t code[AHEAD];
-  uint2 scale[AHEAD];
-  int slot[AHEAD], head[AHEAD];
+  const int64_t from = row_of(cache, slot, head);
+  const uint32_t code = __ldg((const uint32_t*)((value ? cache.v : cache.k) + from * (D / 2)) + w);
+  const uint32_t* s = (value ? cache.v_scale : cache.k_scale) + from * NG;
+  uint2 scale;
+  if (value) scale = __ldg((const uint2*)s + w % (NG / 2));
+  else scale.x = scale.y = __ldg(s + w % NG);
+  float y[8];
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i) {
-    const int64_t row = row0 + i * kEach;
-    slot[i] = -1;
-    if (row >= rows) continue;
-    const int at = (int)fdiv(by_heads, (uint32_t)row);
-    head[i] = (int)row - at * cache.heads;
-    slot[i] = slots[at];
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t q = e < 4 ? scale.x : scale.y;
+    // 2^23 + code + 8, as the four bits with their highest turned over
+    const float c = __uint_as_float((code >> (4 * e) & 15u) ^ 0x4b000008u) - (0x1p23f + 8.0f);
+    y[e] = fmaf(c, __uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u));
   }
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i) {
-    if (slot[i] >= cache.pages * cache.page_size) {
-      atomicExch(err, kBadSlot);
-      slot[i] = -1;
-    }
-    if (slot[i] < 0) continue;
-    const int64_t from = row_of(cache, slot[i], head[i]);
-    code[i] = __ldg((const uint32_t*)(codes + from * (D / 2)) + w);
-    const uint32_t* s = scales + from * NG;
-    if (value) scale[i] = __ldg((const uint2*)s + w % (NG / 2));
-    else scale[i].x = scale[i].y = __ldg(s + w % NG);
-  }
-  const int d = value ? (w % (NG / 2)) * 2 * kGroup + (w / (NG / 2)) * 4 : (w % NG) * kGroup + (w / NG) * 8;
-  auto* out = (typename E::T*)(value ? out_v : out_k) + d;
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i) {
-    if (slot[i] < 0) continue;
-    float y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t q = e < 4 ? scale[i].x : scale[i].y;
-      // 2^23 + code + 8, as the four bits with their highest turned over
-      const float c = __uint_as_float((code[i] >> (4 * e) & 15u) ^ 0x4b000008u) - (0x1p23f + 8.0f);
-      y[e] = fmaf(c, __uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u));
-    }
-    auto* to = out + (row0 + i * kEach) * D;
-    if (!value) {
-      store_n<F32, 8>(to, y);
-    } else {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) store_n<F32, 4>(to + half * kGroup, y + 4 * half);
-    }
+  auto* to = (typename E::T*)(value ? out_v : out_k) + row * D;
+  if (!value) {
+    store_n<F32, 8>(to + (w % NG) * kGroup + (w / NG) * 8, y);
+  } else {
+    to += (w % (NG / 2)) * 2 * kGroup + (w / (NG / 2)) * 4;
+    store_n<F32, 4>(to, y);
+    store_n<F32, 4>(to + kGroup, y + 4);
   }
 }
 
@@ -691,23 +669,16 @@ fopt_status fopt_cache_read(fopt_ctx* ctx, void* out_k, void* out_v, fopt_dtype 
     DeviceGuard guard(ctx);
     const int dim = cache->head_dim;
     const int64_t rows = (int64_t)n * c.heads;
-    auto go = [&](auto kernel, int ahead) {
-      const int64_t each = kv::kThreads / (dim / 8) * ahead;
+    auto go = [&](auto kernel) {
+      const int64_t each = kv::kThreads / (dim / 8);
       kernel<<<dim3((unsigned)((rows + each - 1) / each), 2), kv::kThreads, 0, ctx->stream>>>(
           c, out_k, out_v, slots, rows, make_fastdiv((uint32_t)c.heads), ctx->dev_err);
       launched(ctx, "cache read");
     };
-    // four words of a thread on their way at a time, once there are blocks enough for the SMs
-    const bool many = rows * (dim / 8) >= (int64_t)8 * kv::kThreads * sm_count(ctx);
-    auto sized = [&](auto one, auto four) { many ? go(four, 4) : go(one, 1); };
     if (dtype == FOPT_F32)
-      dim == 64    ? sized(kv::read_kernel<true, 2, 1>, kv::read_kernel<true, 2, 4>)
-      : dim == 128 ? sized(kv::read_kernel<true, 4, 1>, kv::read_kernel<true, 4, 4>)
-                   : sized(kv::read_kernel<true, 8, 1>, kv::read_kernel<true, 8, 4>);
+      dim == 64 ? go(kv::read_kernel<true, 2>) : dim == 128 ? go(kv::read_kernel<true, 4>) : go(kv::read_kernel<true, 8>);
     else
-      dim == 64    ? sized(kv::read_kernel<false, 2, 1>, kv::read_kernel<false, 2, 4>)
-      : dim == 128 ? sized(kv::read_kernel<false, 4, 1>, kv::read_kernel<false, 4, 4>)
-                   : sized(kv::read_kernel<false, 8, 1>, kv::read_kernel<false, 8, 4>);
+      dim == 64 ? go(kv::read_kernel<false, 2>) : dim == 128 ? go(kv::read_kernel<false, 4>) : go(kv::read_kernel<false, 8>);
   });
 }
 
