@@ -31,6 +31,7 @@ struct AttnArgs {
   int causal;
 };
 
+constexpr int kMostKeys = INT32_MAX - 131071;  // so that tiles and pages past the last key stay within 32 bits
 constexpr float kNone = -0x1p120f;  // the maximum of a part that has no score; its sum is 0
 
 struct Seq {
@@ -46,7 +47,7 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
   const int q1 = min(max(s1, s.q0), a.tokens);
   s.queries = q1 - s.q0;
   s.rows = s.queries * a.group;
-  s.keys = (int)min((int64_t)max(n, 0), (int64_t)a.width * a.cache.page_size);
+  s.keys = (int)min((int64_t)min(max(n, 0), kMostKeys), (int64_t)a.width * a.cache.page_size);
   if (s.q0 != s0 || q1 != s1) atomicExch(a.err, kBadStart);
   if (s.keys != n) atomicExch(a.err, kBadLength);
   return s;

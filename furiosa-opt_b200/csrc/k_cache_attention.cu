@@ -787,7 +787,19 @@ extern "C" fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* 
                                   : kv::tokens_workspace<8, 1>(sms);
     // the counters first, so that no variant's partial results reach another's
     const size_t counters = 2 * kv::kCounters * sizeof(uint32_t);
-    uint8_t* ws = (uint8_t*)cache_workspace(ctx, counters + few + (rows ? kv::rows_workspace(dim, sms) : 0));
+    const size_t bytes = counters + few + (rows ? kv::rows_workspace(dim, sms) : 0);
+    // In a capture that is not the context's own the graph takes the memory for its launches from the device's pool:
+    // a workspace of the stream would be shared with all that the stream, or another graph of it, runs meanwhile.
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (!ctx->capture && ctx->stream) cuda_check(cudaStreamIsCapturing(ctx->stream, &capture), "capture status");
+    const bool borrowed = capture != cudaStreamCaptureStatusNone;
+    uint8_t* ws = nullptr;
+    if (borrowed) {
+      cuda_check(cudaMallocAsync((void**)&ws, bytes, ctx->stream), "cache workspace alloc");
+      cuda_check(cudaMemsetAsync(ws, 0, counters, ctx->stream), "cache workspace clear");
+    } else {
+      ws = (uint8_t*)cache_workspace(ctx, bytes);
+    }
     a.counter = (uint32_t*)ws;
     a.ws = (float*)(ws + counters);
     switch (dim) {
@@ -800,5 +812,6 @@ extern "C" fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* 
       a.ws = (float*)(ws + counters + few);
       kv::launch_rows(ctx, a, dim, sms);
     }
+    if (borrowed) cuda_check(cudaFreeAsync(ws, ctx->stream), "cache workspace free");
   });
 }

@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, const __
   if constexpr (!VEC) {
     angles(cs, r, a.positions + t0, n, 0);
     __syncthreads();
-    for (int k = threadIdx.x; k < a.heads * a.units; k += kThreads) {
-      const int h = (int)fdiv(a.by_units, (uint32_t)k), u = k - h * a.units;
+    for (uint32_t k = threadIdx.x; k < (uint32_t)(a.heads * a.units); k += kThreads) {
+      const int h = (int)fdiv(a.by_units, k), u = (int)k - h * a.units;
       const T* from = (const T*)a.x + t0 * a.x_stride + (int64_t)h * a.dim;
       T* to = (T*)a.out + t0 * a.out_stride + (int64_t)h * a.dim;
       const int i = r.interleaved ? 2 * u : u, j = r.interleaved ? 2 * u + 1 : u + r.pairs;
@@ -184,18 +184,19 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, const __
     }
     return;
   }
-  const int total = n * a.heads * a.units, shift = r.interleaved ? 2 : 3;
+  const uint32_t total = n * a.heads * a.units;  // a token's are below 2^31
+  const int shift = r.interleaved ? 2 : 3;
   bool turned = false;
-  for (int k0 = threadIdx.x; !turned || k0 < total; k0 += kThreads * AHEAD) {
+  for (uint32_t k0 = threadIdx.x; !turned || k0 < total; k0 += kThreads * AHEAD) {
     T* to[AHEAD];
     const float2* c[AHEAD];
     bool rotated[AHEAD];
     Raw<F32> v[AHEAD], w[AHEAD];  // the unit's values and, of pairs that lie apart, the second ones
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
-      const int k = k0 + i * kThreads;
+      const uint32_t k = k0 + i * kThreads;
       if (k >= total) continue;
-      const int row = (int)fdiv(a.by_units, (uint32_t)k), u = k - row * a.units;
+      const int row = (int)fdiv(a.by_units, k), u = (int)k - row * a.units;
       const int t = (int)fdiv(a.by_heads, (uint32_t)row), h = row - t * a.heads;
       rotated[i] = r.interleaved ? 4 * u < r.pairs : 8 * u < r.pairs;
       // past the rotated channels units count on in whole chunks
@@ -601,7 +602,7 @@ fopt_status fopt_rotary(fopt_ctx* ctx, void* out, const void* x, fopt_dtype dtyp
     const kv::Rope& r = rope->r;
     require(2 * r.pairs <= head_dim, "fopt_rotary: more rotated channels than the head has");
     const int64_t row = (int64_t)heads * head_dim;
-    require(row <= 1 << 30, "fopt_rotary: a token's heads past 2^30 elements");
+    require(row <= INT32_MAX, "fopt_rotary: a token's heads past 2^31 elements");
     require(x_stride >= row && out_stride >= row, "fopt_rotary: a token stride below heads * head_dim");
     require(out != x || x_stride == out_stride, "fopt_rotary: in place needs equal strides");
     if (ctx && tokens == 0) return;
@@ -661,7 +662,8 @@ fopt_status fopt_cache_read(fopt_ctx* ctx, void* out_k, void* out_v, fopt_dtype 
   return kv::checked_call(ctx, [&] {
     const kv::Cache c = kv::checked(cache, "fopt_cache_read");
     require(dtype == FOPT_BF16 || dtype == FOPT_F32, "fopt_cache_read: bf16 or f32 values");
-    require(n >= 0 && (int64_t)n * c.heads <= INT32_MAX, "fopt_cache_read: slots times heads below 0 or past 2^31");
+    require(n >= 0, "fopt_cache_read: a negative slot count");
+    require((int64_t)n * c.heads <= INT32_MAX, "fopt_cache_read: slots times heads past 2^31");
     if (ctx && n == 0) return;
     require(out_k && out_v && slots, "fopt_cache_read: null argument");
     require(((uintptr_t)out_k | (uintptr_t)out_v) % 16 == 0, "fopt_cache_read: outputs must be 16-byte aligned");

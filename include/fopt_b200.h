@@ -423,9 +423,11 @@ fopt_status fopt_cache_read(fopt_ctx* ctx, void* out_k, void* out_v, fopt_dtype 
  * o [tokens, hq, D] bf16 (32-byte aligned, q 16): a row that sees no key is 0; rows of tokens past q_start[batch] are left
  * as they were. Scores, maxima, sums and the output accumulate in f32. Reads nothing but the keys in
  * range: table entries and cache slots past kv_len may hold anything. A page number outside the cache
- * (its keys count as zeros), a length past table_width pages (cut) or a q_start that is not ascending
- * within 0 .. tokens (clamped) is reported as FOPT_ERR_INVALID by the next fopt_sync / fopt_d2h. All
- * lengths are device data, so a captured call replays over growing sequences. */
+ * (its keys count as zeros), a length past table_width pages or past 2^31 - 131072 (cut) or a q_start that
+ * is not ascending within 0 .. tokens (clamped) is reported as FOPT_ERR_INVALID by the next fopt_sync /
+ * fopt_d2h. All lengths are device data, so a captured call replays over growing sequences. Calls on one
+ * stream take turns with a workspace that the context keeps for the stream (drain a stream of your own
+ * before you destroy it); a captured graph has one of its own. Results do not depend on timing. */
 fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* q, const fopt_paged_cache* cache,
                                  const int32_t* table, const int32_t* q_start, const int32_t* kv_len, int32_t batch,
                                  int32_t tokens, int32_t table_width, int32_t hq, float scale, int32_t causal);

@@ -394,6 +394,17 @@ def test_attention_long_contexts(b200):
         assert np.array_equal(_down(c.run(), c.q.shape), first.astype(F))
 
 
+@pytest.mark.parametrize("D,H,group,q,n", [(64, 1, 1, 1, 30011), (128, 1, 3, 1, 20021), (256, 1, 2, 1, 9001),
+                                           (128, 1, 8, 1, 30000), (128, 1, 8, 2, 12345),   # parts of single tokens
+                                           (128, 1, 8, 16, 20000), (64, 1, 40, 5, 16385)])  # of prompts, one tile empty
+def test_attention_of_few_heads_over_many_blocks(b200, D, H, group, q, n):
+    """Segments that a hundred blocks share, of fewer rows than a block has, beside a short sequence."""
+    c = Case(b200, [q, 1], [n, 40], H, group, D, 64, seed=n)
+    first = c.check()
+    for _ in range(3):
+        assert np.array_equal(_down(c.run(), c.q.shape), first.astype(F))
+
+
 def test_attention_many_sequences(b200):
     """More sequences than a block has threads."""
     n = 700
@@ -535,6 +546,52 @@ def test_attention_on_two_streams(b200):
     finally:
         b200.set_stream(None)
     assert np.array_equal(_down(oa, a.q.shape), wa) and np.array_equal(_down(ob, b.q.shape), wb)
+
+
+def test_attention_of_prompts_and_tokens_in_graphs(b200):
+    """Both kernels' work in two captured graphs, replayed in turn and each followed by a copy of its output."""
+    cases = [Case(b200, [1, 130, 1, 40], [700, 900, 5, 40], 2, 7, 64, 16, seed=35),
+             Case(b200, [60, 1, 1], [2000, 3000, 1], 1, 8, 128, 64, seed=36)]
+    want = [c.check().astype(F) for c in cases]
+    outs = [fb.Storage(b200, "bf16", c.q.size) for c in cases]
+    b200.sync()
+    graphs = [b200.capture(lambda c=c, o=o: c.run(out=o)) for c, o in zip(cases, outs)]
+    for _ in range(10):
+        for g in graphs:
+            g.launch()
+    b200.sync()
+    for o, w in zip(outs, want):
+        assert np.array_equal(_down(o, w.shape), w)
+    for g in graphs:
+        g._h and _lib.lib().fopt_graph_destroy(b200.ctx, g._h)
+        g._h = C.c_void_p()
+
+
+def test_attention_in_a_capture_of_another_library(b200):
+    """Two graphs that torch captures on one stream and replays on two at once: neither shares a workspace."""
+    import torch
+    cases = [Case(b200, [1, 1], [4000, 900], 2, 4, 128, 64, seed=37), Case(b200, [70, 1], [800, 7000], 2, 4, 128, 64, seed=38)]
+    want = [c.check().astype(F) for c in cases]
+    outs = [fb.Storage(b200, "bf16", c.q.size) for c in cases]
+    b200.sync()
+    graphs, streams, side = [], [torch.cuda.Stream() for _ in cases], torch.cuda.Stream()
+    try:
+        for c, o in zip(cases, outs):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                b200.set_stream(torch.cuda.current_stream().cuda_stream)
+                c.run(out=o)
+            graphs.append(g)
+    finally:
+        b200.set_stream(None)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert np.array_equal(_down(o, w.shape), w)
 
 
 def test_attention_past_32_bit_offsets(b200):

@@ -152,7 +152,7 @@ def test_append_refuses_a_rotation_it_cannot_do():
 
 
 @pytest.mark.parametrize("kw,text", [(dict(dtype=2), "bf16 or f32"), (dict(n=-1), "negative"), (dict(k=None), "null"),
-                                     (dict(slots=None), "null"), (dict(v=A + 4), "aligned")])
+                                     (dict(slots=None), "null"), (dict(v=A + 4), "aligned"), (dict(n=2 ** 31 - 1), "past 2\\^31")])
 def test_read_refusals(kw, text):
     _says(_read(**kw), text)
 
@@ -161,7 +161,7 @@ def test_read_refusals(kw, text):
     (dict(batch=-1), "negative"), (dict(tokens=-1), "negative"), (dict(width=0), "empty page table"),
     (dict(hq=7), "multiple"), (dict(hq=0), "multiple"), (dict(scale=math.inf), "finite"), (dict(scale=math.nan), "finite"),
     (dict(o=None), "null"), (dict(q=None), "null"), (dict(table=None), "null"), (dict(q_start=None), "null"),
-    (dict(kv_len=None), "null"), (dict(q=A + 2), "aligned"), (dict(tokens=2 ** 30, hq=8), "too many")])
+    (dict(kv_len=None), "null"), (dict(q=A + 2), "aligned"), (dict(o=A + 16), "aligned"), (dict(tokens=2 ** 30, hq=8), "too many")])
 def test_attention_refusals(kw, text):
     _says(_attend(**kw), text)
 
