@@ -10,8 +10,9 @@
 // code = rint((x - z) / s) in [-8, 7]. The division is the IEEE one: bf16 inputs make exact halves
 // common, and those must go to even rather than to where a reciprocal's error sends them.
 //
-// All three kernels move every byte once and compute little; they are bound by memory on prompts and by
-// latency on single tokens.
+// What bounds them: the rotation memory (12.4 us for 4096 tokens of 32 heads of 128 in bf16, 67 MB: 5.4 TB/s), the
+// append instructions (15.4 us for 4096 tokens of 8 heads of 128, 21 MB, where memory would take 3.3), the read the
+// stores of its half-filled lines (10.4 us for 4608 such slots), single tokens the launch (4.3 us each).
 #include "kvcache.cuh"
 
 namespace fopt {
@@ -21,23 +22,6 @@ namespace {
 constexpr int kThreads = 256;
 
 __device__ __forceinline__ float bf(uint32_t low16) { return __uint_as_float(low16 << 16); }
-
-template <bool F32>
-struct Elem;
-template <>
-struct Elem<true> {
-  using T = float;
-  static __device__ __forceinline__ float load(const T* p) { return *p; }
-  static __device__ __forceinline__ void store(T* p, float v) { *p = v; }
-};
-template <>
-struct Elem<false> {
-  using T = uint16_t;
-  static __device__ __forceinline__ float load(const T* p) { return bf(*p); }
-  static __device__ __forceinline__ void store(T* p, float v) {
-    *p = (uint16_t)(f32_to_bf16w(__float_as_uint(v)) >> 16);
-  }
-};
 
 // x, a subnormal as a zero of its sign.
 __device__ __forceinline__ float flushed(float x) {
@@ -51,6 +35,21 @@ __device__ __forceinline__ uint32_t bf16x2_of(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(flushed(hi)), "f"(flushed(lo)));
   return w;
 }
+
+template <bool F32>
+struct Elem;
+template <>
+struct Elem<true> {
+  using T = float;
+  static __device__ __forceinline__ float value(T v) { return v; }
+  static __device__ __forceinline__ void store(T* p, float v) { *p = v; }
+};
+template <>
+struct Elem<false> {
+  using T = uint16_t;
+  static __device__ __forceinline__ float value(T v) { return bf(v); }
+  static __device__ __forceinline__ void store(T* p, float v) { *p = v == v ? (uint16_t)bf16x2_of(v, 0.0f) : 0x7fc0; }
+};
 
 // Stores N values (4 or 8). The selects of bf16x2_rule cost more than all else in these kernels, so they are left
 // to the words that need them: 0 x + sum is NaN if any x is NaN (or infinite, which the rule rounds alike).
@@ -155,8 +154,9 @@ struct RotaryArgs {
 
 // A block has `each` tokens. With vectors their units are one range, of which a thread has AHEAD at a time, a block's
 // threads apart, on their way while the angles are computed (the sines take about as long as the loads). Without,
-// most time goes into addresses, so a thread takes the same unit of each token (as one range, 45 us where this
-// takes 35: 5878 tokens of 21 heads of 97 in bf16).
+// most time goes into addresses, so a thread takes the same unit of kOnes tokens: 5878 tokens of 21 heads of 96 with
+// 35 pairs in bf16 take 22.7 us, bound by instructions (45 as one range, 35 token after token).
+constexpr int kOnes = 4;
 template <bool F32, bool VEC, int AHEAD>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, const __grid_constant__ Rope r) {
   using E = Elem<F32>;
@@ -168,17 +168,27 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, const __
     __syncthreads();
     for (uint32_t k = threadIdx.x; k < (uint32_t)(a.heads * a.units); k += kThreads) {
       const int h = (int)fdiv(a.by_units, k), u = (int)k - h * a.units;
+      const bool pair = u < r.pairs;
+      const int i = !pair ? u + r.pairs : r.interleaved ? 2 * u : u, j = !pair ? i : r.interleaved ? i + 1 : u + r.pairs;
       const T* from = (const T*)a.x + t0 * a.x_stride + (int64_t)h * a.dim;
       T* to = (T*)a.out + t0 * a.out_stride + (int64_t)h * a.dim;
-      const int i = r.interleaved ? 2 * u : u, j = r.interleaved ? 2 * u + 1 : u + r.pairs;
-      for (int t = 0; t < n; ++t, from += a.x_stride, to += a.out_stride) {
-        if (u < r.pairs) {
+      T p[kOnes], q[kOnes];
+#pragma unroll
+      for (int t = 0; t < kOnes; ++t) {
+        if (t >= n) continue;
+        p[t] = from[t * a.x_stride + i];
+        q[t] = from[t * a.x_stride + j];
+      }
+#pragma unroll
+      for (int t = 0; t < kOnes; ++t) {
+        if (t >= n) continue;
+        if (pair) {
           const float2 c = cs[t * r.pairs + u];
-          const float p = E::load(from + i), q = E::load(from + j);
-          E::store(to + i, turned_first(p, q, c));
-          E::store(to + j, turned_second(p, q, c));
+          const float x = E::value(p[t]), y = E::value(q[t]);
+          E::store(to + t * a.out_stride + i, turned_first(x, y, c));
+          E::store(to + t * a.out_stride + j, turned_second(x, y, c));
         } else {
-          to[u + r.pairs] = from[u + r.pairs];
+          to[t * a.out_stride + i] = p[t];
         }
       }
     }
@@ -309,7 +319,7 @@ struct Steps {
 // g * (NG / 2) + j of a value is channels 4 g .. + 3 of groups 2 j and 2 j + 1; a thread has 8 neighbouring channels
 // of both, and their four threads lie NG / 2 apart. Extremes cross by shuffles. Instructions bound this kernel on
 // prompts; shuffles, scales and addresses are a large part of them, so a thread has as many values as that allows:
-// 14.8 us for 4096 tokens of 8 heads of 128 in bf16, where a thread per word with the tokens of its block one after
+// 15.4 us for 4096 tokens of 8 heads of 128 in bf16, where a thread per word with the tokens of its block one after
 // the other took 18 us, and all groups' channels to four and eight threads a row, with a division a value, 27 us.
 template <bool F32, int NG>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, const __grid_constant__ Rope r) {
@@ -541,7 +551,7 @@ void launch_rotary(fopt_ctx* ctx, RotaryArgs a, const Rope& r) {
   // tokens enough to occupy a block's threads kAhead times over (12 us for 14598 tokens of 3 heads of 128 in bf16,
   // against 19 with two tokens a block), but not so many that SMs go without
   const int64_t per_token = (int64_t)a.heads * a.units, sms = sm_count(ctx);
-  const int64_t fill = VEC ? std::min<int64_t>(kThreads * kAhead / per_token, 2048 / r.pairs) : 4;
+  const int64_t fill = VEC ? std::min<int64_t>(kThreads * kAhead / per_token, 2048 / r.pairs) : kOnes;
   a.each = (int)std::max<int64_t>(1, std::min(fill, a.tokens / (2 * sms)));
   rotary_kernel<F32, VEC, kAhead><<<(a.tokens + a.each - 1) / a.each, kThreads, a.each * r.pairs * sizeof(float2), ctx->stream>>>(a, r);
   launched(ctx, "rotary");
