@@ -27,8 +27,11 @@
 // A 16-byte chunk holds 8 codes in the order that pairs come out of a word (0, 4, 1, 5, 2, 6, 3, 7): for K the
 // queries are stored in the same order, for V the output's columns are put right when they leave.
 //
-// What bounds it: the tensor cores take 32 steps of M 128, N 128, K 16 per key tile (about 3300 cycles); the
-// exponentials take 2048, the expansion about 450 issue slots of each scheduler.
+// What bounds it: the tensor cores take 34 steps of M 128, N 128, K 16 per key tile (about 3300 cycles, 1.75 us); the
+// exponentials take 2048, the expansion about 450 issue slots of each scheduler. A period is 3.0 us, since each of the
+// two tiles takes 1.9 us of softmax and then waits for 0.9 us of products: 138 us for 4 pieces of 512 tokens at 512 to
+// 4096 keys, 8 key heads of 128 and 4 query heads to each (0.56 PFLOP/s), 73 us for 8 prompts of 512, where 5.5 us
+// around the 1 to 4 periods of a segment go into its queries, first scores and output.
 #include "cache_attention.cuh"
 #include "tcgen05.cuh"
 
