@@ -57,6 +57,12 @@ __device__ __forceinline__ long long units(const AttnArgs& a, const Seq& s) {
 }
 
 // ---- small pieces ----
+// Counts an arrival: what came before it is seen by whom counts a later one.
+__device__ __forceinline__ uint32_t arrive(uint32_t* counter) {
+  uint32_t before;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before;
+}
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -166,21 +172,35 @@ struct Query {
   int limit[NB][2];           // keys that the row sees
 };
 
+// The lane's part of the rows as it is in memory: 8 channels of each group of row g (of each eight rows).
 template <int NG, int NB>
-__device__ __forceinline__ void load_query(const AttnArgs& a, const Seq& s, int head, int row0, Query<NG, NB>& q) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
-  constexpr int D = NG * kGroup;
+struct RawQuery {
+  uint4 w[NB][NG];
+  __device__ __forceinline__ void load(const AttnArgs& a, const Seq& s, int head, int row0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int r = row0 + nb * 8 + g;
+      const bool live = r < s.rows;
+      const int token = live ? token_of(a, r) : 0;
+      const uint16_t* p =
+          a.q + ((int64_t)(s.q0 + token) * a.hq + head * a.group + (live ? r - token * a.group : 0)) * (NG * kGroup);
+#pragma unroll
+      for (int j = 0; j < NG; ++j) w[nb][j] = live ? *(const uint4*)(p + j * kGroup + i * 8) : make_uint4(0, 0, 0, 0);
+    }
+  }
+};
+
+template <int NG, int NB>
+__device__ __forceinline__ void load_query(const AttnArgs& a, const Seq& s, int row0, const RawQuery<NG, NB>& raw,
+                                           Query<NG, NB>& q) {
+  const int lane = threadIdx.x & 31, i = lane & 3;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const int r = row0 + nb * 8 + g;
-    const bool live = r < s.rows;
-    const int token = live ? token_of(a, r) : 0;
-    const uint16_t* p = a.q + ((int64_t)(s.q0 + token) * a.hq + head * a.group + (live ? r - token * a.group : 0)) * D;
-    uint4 w[NG];
+    const uint4* w = raw.w[nb];
     uint32_t top = 0;  // of the magnitudes, as bf16 bits
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      w[j] = live ? *(const uint4*)(p + j * kGroup + i * 8) : make_uint4(0, 0, 0, 0);
       const uint32_t* x = (const uint32_t*)&w[j];
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = __vmaxu2(top, x[e] & 0x7fff7fffu);
@@ -517,6 +537,8 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
       sc = sc_head + (uint64_t)(uint32_t)page * page_scales;
       page = ++page_at < page_end ? table[page_at] : 0;  // for the next time
     };
+    RawQuery<NG, NB> raw;  // on its way with the page number
+    raw.load(a, s, head, row0);
     if (n < n1) {
       enter();
       k += begin * (D / 2);
@@ -552,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
 #pragma unroll 1
     for (int c = 0; c < kStages - 1; ++c) fetch();
     Query<NG, NB> q;
-    load_query<NG, NB>(a, s, head, row0, q);  // while the first keys are on their way
+    load_query<NG, NB>(a, s, row0, raw, q);  // while the first keys are on their way
     // A tile's scores are computed while the tile before is finished: two independent chains of instructions.
     auto next_stage = [](uint32_t at) { return at + S::kStage == S::kRing ? 0 : at + S::kStage; };
     float x[NB][4];
@@ -637,12 +659,10 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
     }
     if (!whole) {
       const int c0 = shares.owner(seg_at + kSegmentCost), c1 = shares.owner(seg_at + length - 1);
-      __syncthreads();  // one thread's fence below covers what the barrier has ordered before it
+      __syncthreads();  // what the barrier has ordered before it, one thread's release below covers
       if (tid == 0) {
-        __threadfence();
-        last = atomicAdd(a.counter + c0, 1u) == (uint32_t)(c1 - c0);
+        last = arrive(a.counter + c0) == (uint32_t)(c1 - c0);
         if (last) a.counter[c0] = 0;
-        __threadfence();
       }
       __syncthreads();
       if (last) {
