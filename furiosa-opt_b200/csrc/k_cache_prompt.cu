@@ -310,12 +310,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  Walk walk(a, start, shares);
+  Item it;
+  bool more = walk.next(it);  // the first segment, while tensor memory is allocated
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;  // S0, S1 (128 columns each), O0, O1 (at 256 and 384)
-  Walk walk(a, start, shares);
-  Item it;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -335,7 +336,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       };
       int n = 0, seg = 0;  // key tiles and segments so far
       bool ok = true;
-      bool more = walk.next(it);
       for (; ok && more; ++seg) {
         const int n1 = n + it.t1 - it.t0;
         ok = mbar_wait(smem_u32(&k_full[n & 1]), (n >> 1) & 1, abort_flag, a.err, 401);
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
     uint32_t scales[NG];
     int low_v = 0;
     bool fresh = true;  // the segment's first V of this warp
-    bool more = walk.next(it), ok = true;
+    bool ok = true;
     int t = more ? it.t0 : 0;
     int u = warp - 1, n = 0;  // which of a tile's eight turns (K of its quarters, then V), and the tile's number
     auto load = [&](const Spot& at) {
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       const bool here = mbar_wait(smem_u32(&met[t]), meetings++ & 1, abort_flag, a.err, 424);
       return __all_sync(0xffffffffu, here);
     };
-    bool more = walk.next(it), ok = true;
+    bool ok = true;
     Item done;  // the segment whose output is still in O_t
     float qs = 0.0f, m = 0.0f, l = 0.0f;
     int n = 0;
