@@ -306,13 +306,13 @@ GARBAGE = 2 ** 30  # a page number that must not be read
 class Case:
     """A filled cache, its sequences and their queries; spare slots and pages hold NaN."""
 
-    def __init__(self, be, q_lens, kv_lens, H, group, D, page, seed=0, pad=0, spare=2, bias=1.0, size=1.0):
+    def __init__(self, be, q_lens, kv_lens, H, group, D, page, seed=0, pad=0, spare=2, bias=1.0, size=1.0, wide=0):
         rng = np.random.default_rng(seed)
         self.be, self.H, self.group, self.D = be, H, group, D
         need = [-(-n // page) for n in kv_lens]
         pages = sum(need) + spare
         order = rng.permutation(pages)
-        self.width = max(1, max(need)) + 1
+        self.width = max(max(1, max(need)) + 1, -(-wide // page))  # a table wide enough for `wide` keys
         self.table = np.full((len(q_lens), self.width), GARBAGE, np.int64)
         self.ref, self.cache = R.Cache(pages, page, H, D), fb.PagedCache(be, pages, page, H, D)
         slots, at = [], 0
@@ -392,6 +392,65 @@ def test_attention_long_contexts(b200):
     first = c.check()
     for _ in range(3):
         assert np.array_equal(_down(c.run(), c.q.shape), first.astype(F))
+
+
+# Tables for contexts of this many keys: calls of more than 32 query rows to a key head then are the prompt kernel's
+# whatever their size (narrow tables leave small ones to the kernel for single tokens).
+WIDE = 400000
+
+
+@pytest.mark.parametrize("page", [16, 48, 64, 1024])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_pieces_and_single_tokens_in_wide_tables(b200, page, causal):
+    Case(b200, [1, 37, 0, 5, 3, 1, 64, 2], [260, 37, 99, 3, 0, 0, 129, 2], 2, 4, 128, page, pad=3, wide=WIDE).check(causal)
+
+
+@pytest.mark.parametrize("D,H,group,q,n", [(128, 2, 4, 130, 300), (64, 1, 7, 200, 200), (128, 1, 1, 257, 513),
+                                           (64, 2, 16, 40, 41), (128, 1, 32, 33, 100), (128, 1, 128, 2, 70),
+                                           (128, 1, 40, 16, 20000), (64, 1, 40, 5, 16385)])
+def test_attention_prompts_in_wide_tables(b200, D, H, group, q, n):
+    for causal in (True, False):
+        c = Case(b200, [q], [n], H, group, D, 32, seed=q, wide=WIDE)
+        first = c.check(causal)
+        assert np.array_equal(_down(c.run(causal), c.q.shape), first.astype(F))
+
+
+@pytest.mark.parametrize("size,bias", [(30.0, 1.0), (1e-4, 0.0), (0.0, 1.0), (1.0, 300.0)])
+def test_attention_of_sharp_and_flat_scores_in_wide_tables(b200, size, bias):
+    c = Case(b200, [1, 40], [500, 150], 1, 4, 128, 16, seed=11, size=size, bias=bias, wide=WIDE)
+    c.check()
+    c.check(scale=0.0)
+    c.check(scale=-0.05)
+
+
+def test_attention_in_a_wide_table_reads_no_further_than_the_lengths(b200):
+    c = Case(b200, [1, 20, 1], [33, 40, 16], 2, 4, 128, 16, seed=14, wide=WIDE)
+    want = c.check()
+    q = c.q.copy()
+    q[2, 3, 5], q[0, 1, 0] = np.nan, np.inf  # one row each
+    c.dev["q"] = _up(b200, q, "bf16")
+    got = _down(c.run(), q.shape)
+    clean = np.ones(q.shape[:2], bool)
+    clean[2, 3] = clean[0, 1] = False
+    assert np.array_equal(got[clean], want.astype(F)[clean])
+    assert np.isnan(got[2, 3]).all()
+
+
+@pytest.mark.parametrize("power", [-100, -30, 30, 90])
+def test_attention_of_values_of_any_size_in_wide_tables(b200, power):
+    c = Case(b200, [1, 33], [200, 50], 1, 4, 128, 16, seed=12, wide=WIDE)
+    s = F(2.0) ** F(power)
+    for n in ("k", "v"):
+        st = c.ref
+        st.step[n] = st.step[n] * s
+        st.offset[n] = st.offset[n] * s
+        img = dtypes.f32_to_bf16_bits(st.scale_image(n))
+        dev = getattr(c.cache, n + "_scale")
+        _lib.check(_lib.lib().fopt_h2d(b200.ctx, dev.ptr, img.ctypes.data, img.nbytes), b200.ctx)
+        b200.sync()
+    c.q = (c.q / s).astype(F)
+    c.dev["q"] = _up(b200, c.q, "bf16")
+    c.check()
 
 
 @pytest.mark.parametrize("D,H,group,q,n", [(64, 1, 1, 1, 30011), (128, 1, 3, 1, 20021), (256, 1, 2, 1, 9001),
@@ -550,8 +609,8 @@ def test_attention_on_two_streams(b200):
 
 def test_attention_of_prompts_and_tokens_in_graphs(b200):
     """Both kernels' work in two captured graphs, replayed in turn and each followed by a copy of its output."""
-    cases = [Case(b200, [1, 130, 1, 40], [700, 900, 5, 40], 2, 7, 64, 16, seed=35),
-             Case(b200, [60, 1, 1], [2000, 3000, 1], 1, 8, 128, 64, seed=36)]
+    cases = [Case(b200, [1, 130, 1, 40], [700, 900, 5, 40], 2, 7, 64, 16, seed=35, wide=WIDE),
+             Case(b200, [60, 1, 1], [2000, 3000, 1], 1, 8, 128, 64, seed=36, wide=WIDE)]
     want = [c.check().astype(F) for c in cases]
     outs = [fb.Storage(b200, "bf16", c.q.size) for c in cases]
     b200.sync()
@@ -570,7 +629,7 @@ def test_attention_of_prompts_and_tokens_in_graphs(b200):
 def test_attention_in_a_capture_of_another_library(b200):
     """Two graphs that torch captures on one stream and replays on two at once: neither shares a workspace."""
     import torch
-    cases = [Case(b200, [1, 1], [4000, 900], 2, 4, 128, 64, seed=37), Case(b200, [70, 1], [800, 7000], 2, 4, 128, 64, seed=38)]
+    cases = [Case(b200, [1, 1], [4000, 900], 2, 4, 128, 64, seed=37), Case(b200, [70, 1], [800, 7000], 2, 4, 128, 64, seed=38, wide=WIDE)]
     want = [c.check().astype(F) for c in cases]
     outs = [fb.Storage(b200, "bf16", c.q.size) for c in cases]
     b200.sync()
