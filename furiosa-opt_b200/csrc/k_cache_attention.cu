@@ -40,6 +40,8 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTileTokens = 16 * kWarps;
 constexpr int kBlocks = 3;       // resident blocks an SM, where the registers allow (168 a thread)
+template <int NG, int NB>
+constexpr int tokens_blocks() { return NG <= 4 && NB == 1 ? kBlocks : 2; }
 constexpr int kSegmentCost = 4;  // beginning and ending a segment takes about as long as this many tiles
 constexpr int kLeast = 2;        // tiles of a share
 // A part more to add up takes about a sixth of a tile. Shares of 2 tiles were best at 777 tokens of 8 heads
@@ -437,7 +439,7 @@ struct Partial {
 };
 
 template <int NG, int NB>
-__global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <= 4 ? 2 : 1) tokens_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, tokens_blocks<NG, NB>()) tokens_kernel(AttnArgs a) {
   using S = Shared<NG, NB>;
   using P = Partial<NG, NB>;
   constexpr int D = S::D, R = S::R;
@@ -740,8 +742,6 @@ __global__ void __launch_bounds__(kThreads, NG <= 4 && NB == 1 ? kBlocks : NG <=
 
 constexpr int kCounters = 1024;  // of each kernel, one for each block
 
-template <int NG, int NB>
-constexpr int tokens_blocks() { return NG <= 4 && NB == 1 ? kBlocks : NG <= 4 ? 2 : 1; }
 template <int NG, int NB>
 size_t tokens_workspace(int sms) { return (size_t)sms * tokens_blocks<NG, NB>() * 2 * Partial<NG, NB>::kFloats * sizeof(float); }
 
