@@ -799,8 +799,7 @@ extern "C" fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* 
     // 16 rows a block where a sequence has that many on average: the codes are expanded once for both halves
     const bool two = dim != 256 && (int64_t)tokens * a.group > 8 * (int64_t)batch;
     // Sequences of more than kv::kFewRows query rows go to rows_kernel, whose tiles of 256 rows take about as long
-    // as that many rows of tokens_kernel (head_dim 256 exceeds its tensor memory). The lengths are the device's,
-    // so both are launched, unless no sequence can be that long or the call has no more tokens than sequences:
+    // as that many rows of tokens_kernel. The lengths are the device's, so both are launched, unless no sequence can be that long or the call has no more tokens than sequences:
     // then it is single tokens, for which rows_kernel would only begin and end (4 us).
     // A call that leaves most of the device to tokens_kernel's blocks is its own as well, for rows_kernel's few blocks
     // take longer to begin, to end and over each segment. What each block would have at most, in tiles of 64 keys, decides,
@@ -812,7 +811,7 @@ extern "C" fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* 
     const int64_t segments = ((int64_t)tokens * a.group / (two ? 16 : 8) + batch) * cache->heads;
     const double tiles = (double)segments * (double)(width / kv::kTileTokens + 1 + kv::kSegmentCost) / (sms * (two ? 2 : kv::kBlocks));
     const bool light = tiles <= (double)(16 + std::min<int64_t>(width / 256, 64));
-    const bool rows = dim != 256 && tokens > batch && (int64_t)tokens * a.group > kv::kFewRows && !light;
+    const bool rows = tokens > batch && (int64_t)tokens * a.group > kv::kFewRows && !light;
     a.long_rows = rows ? kv::kFewRows + 1 : INT32_MAX;
     const size_t few = dim == 64 ? (two ? kv::tokens_workspace<2, 2>(sms) : kv::tokens_workspace<2, 1>(sms))
                      : dim == 128 ? (two ? kv::tokens_workspace<4, 2>(sms) : kv::tokens_workspace<4, 1>(sms))

@@ -41,10 +41,9 @@ namespace {
 
 using namespace attn;
 
-constexpr int kRows = 256, kKeys = 128;  // of a segment and of a tile
-constexpr int kExpand = 7, kRowThreads = 32 * (1 + kExpand + 8);  // warps that expand codes; 128 registers a thread
+constexpr int kRowThreads = 512;         // 128 registers each
 constexpr int kHalf = 16384;             // 128 rows of 64 f16 (128 bytes), the unit of the swizzled tiles
-constexpr int kOffsets = 128 * 32;        // 128 rows of 16 f16: the sums of a tile's q, or the offsets of a key tile
+constexpr int kOffsets = 128 * 32;        // 128 rows of 16 f16: the sums of a tile's q (or the offsets of 128 keys)
 constexpr int kCost = 2;                 // key tiles that beginning and ending a segment takes as long as
 constexpr int kLeast = 4;                // units of a share
 // A part more to add up (66 KB for each of two tiles, by one SM) takes about as long as a unit. Of 16 tokens at 131072
@@ -54,29 +53,37 @@ constexpr int kUncut = 8;                // segments of fewer tiles are not shar
 constexpr float kLazyRows = 14.0f;        // log2 by which x may exceed its base: P stays within f16, the base moves rarely
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// At D = 256 one 128-row tile of queries and 64 keys at a time are what tensor memory (64 columns of scores, 256 of
+// outputs) and shared memory hold; products and softmax take turns. 512 queries at 2382 keys and 370 at 370, 3 key
+// heads and 5 query heads to each: 79 us (203 by tokens_kernel).
 template <int NG>
 struct Tiles {
   static constexpr int D = NG * kGroup, kHalves = D / 64;
-  static constexpr int kTile = kHalves * kHalf;      // Q_t, K or V
-  // 2 Q, 2 stages of K and of V, the offset steps of Q and K, alignment, barriers and scales; more than half an
+  static constexpr int kQueries = NG == 8 ? 1 : 2, kRows = 128 * kQueries;  // row tiles and rows of a segment
+  static constexpr int kKeys = NG == 8 ? 64 : 128, kQuarters = kKeys / 32;  // of a key tile, and a warp's turns with its K
+  static constexpr int kExpand = NG == 8 ? 6 : 7;    // warps that expand codes
+  static constexpr int kQ = kHalves * kHalf;         // bytes of Q_t
+  static constexpr int kKeyHalf = kKeys * 128, kTile = kHalves * kKeyHalf;  // of 64 channels of a key tile, of K or V
+  static constexpr int kKeyOffsets = kKeys * 32;     // of its offset step
+  // Q, 2 stages of K and of V, the offset steps of Q and K, alignment, barriers and scales; more than half an
   // SM's, since a second block would only wait for tensor memory
   static constexpr int kRaw = 32 * NG * 16;  // what a warp holds of 32 tokens' K or V
-  static constexpr int kAll = 6 * kTile + 4 * kOffsets + kExpand * kRaw + 1024 + 512;
+  static constexpr int kAll = kQueries * (kQ + kOffsets) + 4 * kTile + 2 * kKeyOffsets + kExpand * kRaw + 1024 + 512;
   static constexpr int kBytes = kAll > 120000 ? kAll : 120000;
   static constexpr int kSlot = kRows * (D + 2);      // floats of a partial result
-};
 
-__device__ __forceinline__ int blocks_of(const Seq& s) { return (s.rows + kRows - 1) / kRows; }
-// Key tiles of a row block: up to the last key that its last row sees, one at least.
-__device__ __forceinline__ int tiles_of(const AttnArgs& a, const Seq& s, int rb) {
-  return max(1, (max(0, seen(a, s, min(s.rows, (rb + 1) * kRows) - 1)) + kKeys - 1) / kKeys);
-}
-__device__ __forceinline__ long long units(const AttnArgs& a, const Seq& s) {
-  if (s.rows < a.long_rows) return 0;
-  long long n = 0;
-  for (int rb = 0; rb < blocks_of(s); ++rb) n += tiles_of(a, s, rb) + kCost;
-  return n * a.cache.heads;
-}
+  static __device__ __forceinline__ int blocks_of(const Seq& s) { return (s.rows + kRows - 1) / kRows; }
+  // Key tiles of a row block: up to the last key that its last row sees, one at least.
+  static __device__ __forceinline__ int tiles_of(const AttnArgs& a, const Seq& s, int rb) {
+    return max(1, (max(0, seen(a, s, min(s.rows, (rb + 1) * kRows) - 1)) + kKeys - 1) / kKeys);
+  }
+  static __device__ __forceinline__ long long units(const AttnArgs& a, const Seq& s) {
+    if (s.rows < a.long_rows) return 0;
+    long long n = 0;
+    for (int rb = 0; rb < blocks_of(s); ++rb) n += tiles_of(a, s, rb) + kCost;
+    return n * a.cache.heads;
+  }
+};
 
 struct Item {
   Seq s;
@@ -86,6 +93,7 @@ struct Item {
 };
 
 // A block's segments in order. Every role of the block walks them by itself.
+template <typename T>
 struct Walk {
   const AttnArgs& a;
   long long pos, end, rb_at;
@@ -100,12 +108,12 @@ struct Walk {
     while (pos < end) {
       int length;
       for (;;) {  // the row block that holds pos
-        if (s.rows < a.long_rows || rb == blocks_of(s)) {
+        if (s.rows < a.long_rows || rb == T::blocks_of(s)) {
           s = sequence(a, ++b);
           rb = 0;
           continue;
         }
-        length = tiles_of(a, s, rb) + kCost;
+        length = T::tiles_of(a, s, rb) + kCost;
         if (pos < rb_at + (long long)length * a.cache.heads) break;
         rb_at += (long long)length * a.cache.heads;
         ++rb;
@@ -136,7 +144,7 @@ struct Walk {
       it.s = s;
       it.b = b;
       it.head = head;
-      it.row0 = rb * kRows;
+      it.row0 = rb * T::kRows;
       it.tiles = length - kCost;
       it.at = at;
       return true;
@@ -253,13 +261,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
   constexpr int D = T::D;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t* sQ = smem;                  // tile t at sQ + t * kTile
-  uint8_t* sK = smem + 2 * T::kTile;   // stage n at sK + n * kTile
-  uint8_t* sV = smem + 4 * T::kTile;
-  uint8_t* sQz = smem + 6 * T::kTile;  // the offset steps: of tile t at sQz + t * kOffsets, of stage n at sKz + ...
-  uint8_t* sKz = sQz + 2 * kOffsets;
-  uint8_t* raw = sKz + 2 * kOffsets;   // rows as they are in the cache, of warps 1-7
-  uint64_t* bars = (uint64_t*)(raw + kExpand * T::kRaw);
+  uint8_t* sQ = smem;  // tile t at sQ + t * kQ
+  uint8_t* sK = smem + T::kQueries * T::kQ;  // stage n at sK + n * kTile
+  uint8_t* sV = sK + 2 * T::kTile;
+  uint8_t* sQz = sV + 2 * T::kTile;  // the offset steps: of tile t at sQz + t * kOffsets, of stage n at sKz + n * kKeyOffsets
+  uint8_t* sKz = sQz + T::kQueries * kOffsets;
+  uint8_t* raw = sKz + 2 * T::kKeyOffsets;  // rows as they are in the cache, of the expanding warps
+  uint64_t* bars = (uint64_t*)(raw + T::kExpand * T::kRaw);
   uint64_t* k_full = bars;         // [2]
   uint64_t* k_empty = bars + 2;    // [2]
   uint64_t* v_full = bars + 4;     // [2]
@@ -278,10 +286,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Start start = share_start<kRowThreads>(
-      a.batch, kLeast, kByRoot, [&](int b) { return units(a, sequence(a, b)); },
+      a.batch, kLeast, kByRoot, [&](int b) { return T::units(a, sequence(a, b)); },
       [&](int b) {
         const Seq s = sequence(a, b);
-        return s.rows < a.long_rows ? 0 : tiles_of(a, s, blocks_of(s) - 1);
+        return s.rows < a.long_rows ? 0 : T::tiles_of(a, s, T::blocks_of(s) - 1);
       });
   // The launch does not wait for tokens_kernel's end (they share nothing); this kernel's end does, for what follows.
   if ((int)blockIdx.x >= start.blocks) {
@@ -292,9 +300,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&k_full[i]), 4);
+      mbar_init(smem_u32(&k_full[i]), T::kQuarters);
       mbar_init(smem_u32(&k_empty[i]), 1);
-      mbar_init(smem_u32(&v_full[i]), 4);
+      mbar_init(smem_u32(&v_full[i]), T::kQuarters);
       mbar_init(smem_u32(&v_empty[i]), 1);
       mbar_init(smem_u32(&q_full[i]), 128);
       mbar_init(smem_u32(&s_full[i]), 1);
@@ -302,7 +310,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       mbar_init(smem_u32(&o_done[i]), 1);
       mbar_init(smem_u32(&met[i]), 128);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&x_full[i]), 8);
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&x_full[i]), 2 * T::kQuarters);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -310,28 +318,28 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  Walk walk(a, start, shares);
+  Walk<T> walk(a, start, shares);
   Item it;
   bool more = walk.next(it);  // the first segment, while tensor memory is allocated
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = *tmem_slot;  // S0, S1 (128 columns each), O0, O1 (at 256 and 384)
+  const uint32_t tmem = *tmem_slot;  // S0, S1 (128 columns each), O0, O1 (at 256 and 384); or S0 and O0 of 256 columns
 
   if (warp == 0) {
     if (lane == 0) {
       // f16 x f16 -> f32, M = 128
       const uint32_t base = (1u << 4) | ((uint32_t)(128 >> 4) << 24);
-      const uint32_t qk = base | ((uint32_t)(kKeys >> 3) << 17), pv = base | ((uint32_t)(D >> 3) << 17) | kIdescBMajorMN;
+      const uint32_t qk = base | ((uint32_t)(T::kKeys >> 3) << 17), pv = base | ((uint32_t)(D >> 3) << 17) | kIdescBMajorMN;
       auto scores = [&](int t, int n) {  // S_t of key tile n
-        const uint64_t qd = sdesc(smem_u32(sQ + t * T::kTile)), kd = sdesc(smem_u32(sK + (n & 1) * T::kTile));
+        const uint64_t qd = sdesc(smem_u32(sQ + t * T::kQ)), kd = sdesc(smem_u32(sK + (n & 1) * T::kTile));
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (uint32_t)((k >> 2) * kHalf + (k & 3) * 32) >> 4;
-          mma_bf16(tmem + t * 128, qd + off, kd + off, qk, k != 0);
+          mma_bf16(tmem + t * 128, qd + ((uint32_t)((k >> 2) * kHalf + (k & 3) * 32) >> 4),
+                   kd + ((uint32_t)((k >> 2) * T::kKeyHalf + (k & 3) * 32) >> 4), qk, k != 0);
         }
         mma_bf16(tmem + t * 128, offsets_desc(smem_u32(sQz + t * kOffsets)),
-                 offsets_desc(smem_u32(sKz + (n & 1) * kOffsets)), qk, 1);
+                 offsets_desc(smem_u32(sKz + (n & 1) * T::kKeyOffsets)), qk, 1);
         commit(smem_u32(&s_full[t]));
       };
       int n = 0, seg = 0;  // key tiles and segments so far
@@ -339,7 +347,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       for (; ok && more; ++seg) {
         const int n1 = n + it.t1 - it.t0;
         ok = mbar_wait(smem_u32(&k_full[n & 1]), (n >> 1) & 1, abort_flag, a.err, 401);
-        for (int t = 0; ok && t < 2; ++t) {
+        for (int t = 0; ok && t < T::kQueries; ++t) {
           ok = mbar_wait(smem_u32(&q_full[t]), seg & 1, abort_flag, a.err, 402);
           if (!ok) break;
           fence_after();
@@ -348,16 +356,17 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         if (ok) commit(smem_u32(&k_empty[n & 1]));
         more = walk.next(it);  // the next segment, while this one's scores are on their way
         for (int first = n; ok && n < n1; ++n) {
-          for (int t = 0; ok && t < 2; ++t) {
+          for (int t = 0; ok && t < T::kQueries; ++t) {
             ok = (t || mbar_wait(smem_u32(&v_full[n & 1]), (n >> 1) & 1, abort_flag, a.err, 403)) &&
                  mbar_wait(smem_u32(&p_ready[t]), n & 1, abort_flag, a.err, 404);
             if (!ok) break;
             fence_after();
-            const uint64_t vd = vdesc(smem_u32(sV + (n & 1) * T::kTile));
+            const uint64_t vd = vdesc(smem_u32(sV + (n & 1) * T::kTile), T::kKeyHalf);
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
+            for (int k = 0; k < T::kKeys / 16; ++k)
               mma_bf16_ta(tmem + 256 + t * 128, tmem + t * 128 + 8 * k, vd + (uint64_t)(128 * k), pv, (n - first) | k);
-            if (t) commit(smem_u32(&v_empty[n & 1]));
+            const bool last_tile = t == T::kQueries - 1;
+            if (last_tile) commit(smem_u32(&v_empty[n & 1]));
             if (n + 1 == n1) {
               commit(smem_u32(&o_done[t]));
             } else {
@@ -366,14 +375,14 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
               if (!ok) break;
               fence_after();
               scores(t, n + 1);
-              if (t) commit(smem_u32(&k_empty[(n + 1) & 1]));
+              if (last_tile) commit(smem_u32(&k_empty[(n + 1) & 1]));
             }
           }
         }
       }
     }
     __syncwarp();
-  } else if (warp <= kExpand) {
+  } else if (warp <= T::kExpand) {
     const Masks m = masks();
     // The next row is on its way in registers while the current one is expanded from shared memory, where a loop can
     // index it: [piece of 16 bytes][lane]. A lane reads back what it wrote itself.
@@ -384,17 +393,30 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
     bool fresh = true;  // the segment's first V of this warp
     bool ok = true;
     int t = more ? it.t0 : 0;
-    int u = warp - 1, n = 0;  // which of a tile's eight turns (K of its quarters, then V), and the tile's number
+    constexpr int kQuarters = T::kQuarters;
+    int u = warp - 1, n = 0;  // which of a tile's turns (K of its quarters, then V), and the tile's number
+    auto in_tile = [&] {  // ... when u has been counted on
+      while (more && u >= 2 * kQuarters) {
+        u -= 2 * kQuarters;
+        ++n;
+        if (++t == it.t1) {
+          fresh = true;
+          more = walk.next(it);
+          t = it.t0;
+        }
+      }
+    };
+    in_tile();
     auto load = [&](const Spot& at) {
       int64_t row;
       const bool there = row_at(a, it, at, row);
-      load_row<4 * NG>((uint32_t*)codes, (u < 4 ? a.cache.k : a.cache.v) + row * (NG * 16), there);
-      load_row<NG>(scales, (u < 4 ? a.cache.k_scale : a.cache.v_scale) + row * NG, there);
+      load_row<4 * NG>((uint32_t*)codes, (u < kQuarters ? a.cache.k : a.cache.v) + row * (NG * 16), there);
+      load_row<NG>(scales, (u < kQuarters ? a.cache.k_scale : a.cache.v_scale) + row * NG, there);
     };
-    if (more) load(spot_of(a, it, t * kKeys + (u & 3) * 32 + lane));
+    if (more) load(spot_of(a, it, t * T::kKeys + u % kQuarters * 32 + lane));
     while (more) {
-      const bool is_v = u >= 4;
-      const int quarter = u & 3, row = quarter * 32 + lane, stage = n & 1, at4 = (n & 3) * 4 + quarter;
+      const bool is_v = u >= kQuarters;
+      const int quarter = u % kQuarters, row = quarter * 32 + lane, stage = n & 1, at4 = (n & 3) * 4 + quarter;
       const uint32_t full = smem_u32(is_v ? &v_full[stage] : &k_full[stage]);
       const uint32_t empty = smem_u32(is_v ? &v_empty[stage] : &k_empty[stage]), parity = ((n >> 1) & 1) ^ 1;
       const uint32_t known = smem_u32(&x_full[n & 3]);
@@ -405,11 +427,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         e = max(e, low_v);
       }
       const float f = power(-e);
-      // by code word of a piece: steps and offsets of what its pairs of codes are (see the loop)
-      uint32_t step[4], offset[4], z[8] = {};
+      // by code word of a piece (of two, where K's group of words is two pieces): steps and offsets of what its pairs of
+      // codes are (see the loop)
+      constexpr int kWords = NG == 8 ? 8 : 4;
+      uint32_t step[kWords], offset[kWords], z[8] = {};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int g = NG == 4 ? w : w & 1, h = NG == 4 ? w & 1 : 0;
+      for (int w = 0; w < kWords; ++w) {
+        const int g = NG == 2 ? w & 1 : w, h = NG == 2 ? 0 : NG == 4 ? w & 1 : w & 3;
         const float s = step_of(scales[g]) * f;
         step[w] = is_v ? f16x2(step_of(scales[2 * h]) * f, step_of(scales[2 * h + 1]) * f) : f16x2(s, s);
         offset[w] = is_v ? f16x2(offset_of(scales[2 * h]) * f, offset_of(scales[2 * h + 1]) * f) : 0;
@@ -421,18 +445,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < NG; ++i) mine[i * 32] = codes[i];
       // the next turn: its page is looked up while this one's row is expanded
-      u += kExpand;
-      if (u >= 8) {
-        u -= 8;
-        ++n;
-        if (++t == it.t1) {
-          fresh = true;
-          more = walk.next(it);
-          t = it.t0;
-        }
-      }
+      u += T::kExpand;
+      in_tile();
       Spot next{-1, 0, false};
-      if (more) next = spot_of(a, it, t * kKeys + (u & 3) * 32 + lane);
+      if (more) next = spot_of(a, it, t * T::kKeys + u % kQuarters * 32 + lane);
 
       ok = mbar_wait(empty, parity, abort_flag, a.err, 411);
       ok = __all_sync(0xffffffffu, ok);
@@ -443,35 +459,43 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         mbar_arrive(known);
       }
       if (!is_v) {
-        uint8_t* tz = sKz + stage * kOffsets;
+        uint8_t* tz = sKz + stage * T::kKeyOffsets;
         *(uint4*)(tz + offsets_place(row, 0)) = make_uint4(z[0], z[1], z[2], z[3]);
         *(uint4*)(tz + offsets_place(row, 1)) = make_uint4(z[4], z[5], z[6], z[7]);
       }
       uint8_t* to = (is_v ? sV : sK) + stage * T::kTile + row * 128;
       // Word w of piece i is chunk: of K (words in the order of [D % 32 / 8, D / 32]) 4 group + run, of V its number.
-      const int by_piece = is_v ? 4 : NG == 4 ? 1 : 2;
-      const int c1 = is_v ? 1 : 4, c2 = is_v ? 2 : NG == 4 ? 8 : 1, c3 = is_v ? 3 : NG == 4 ? 12 : 5;
-      auto chunk_at = [&](int c) { return (uint4*)(to + (c >> 3) * kHalf + (((c & 7) ^ (row & 7)) << 4)); };
-#pragma unroll 1
-      for (int i = 0; i < NG; ++i) {
+      auto chunk_at = [&](int c) { return (uint4*)(to + (c >> 3) * T::kKeyHalf + (((c & 7) ^ (row & 7)) << 4)); };
+      const int c1 = is_v ? 1 : 4, c2 = is_v ? 2 : NG == 2 ? 1 : 8, c3 = is_v ? 3 : NG == 2 ? 5 : 12;
+      auto piece = [&](int i, int c, int from) {
         const uint4 w = mine[i * 32];
-        const int c = i * by_piece;
-        *chunk_at(c) = expand(m, w.x, step[0], offset[0]);
-        *chunk_at(c + c1) = expand(m, w.y, step[1], offset[1]);
-        *chunk_at(c + c2) = expand(m, w.z, step[2], offset[2]);
-        *chunk_at(c + c3) = expand(m, w.w, step[3], offset[3]);
+        *chunk_at(c) = expand(m, w.x, step[from], offset[from]);
+        *chunk_at(c + c1) = expand(m, w.y, step[from + 1], offset[from + 1]);
+        *chunk_at(c + c2) = expand(m, w.z, step[from + 2], offset[from + 2]);
+        *chunk_at(c + c3) = expand(m, w.w, step[from + 3], offset[from + 3]);
+      };
+      if constexpr (NG == 8) {
+#pragma unroll 1
+        for (int i = 0; i < NG; i += 2) {
+          piece(i, is_v ? 4 * i : i >> 1, 0);
+          piece(i + 1, is_v ? 4 * i + 4 : 16 + (i >> 1), 4);
+        }
+      } else {
+        const int by_piece = is_v ? 4 : NG == 4 ? 1 : 2;
+#pragma unroll 1
+        for (int i = 0; i < NG; ++i) piece(i, i * by_piece, 0);
       }
       load(next);
       async_fence();
       __syncwarp();
       if (lane == 0) mbar_arrive(full);
     }
-  } else {
+  } else if (warp >= 8 && warp < 8 + 4 * T::kQueries) {
     const int t = (warp - 8) >> 2, quarter = warp & 3;  // tile, and the tensor-memory lanes that the warp may read
     const int r = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem + t * 128 + lanes, tO = tmem + 256 + t * 128 + lanes;
-    uint8_t* tq = sQ + t * T::kTile;
+    uint8_t* tq = sQ + t * T::kQ;
 
     // Rows of q and o (16 bytes a lane) start at their number * D.
     auto number = [&](const Item& x, int row) -> int {
@@ -649,6 +673,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
 #pragma unroll
               for (int i = 0; i < 32 / NG / 8; ++i)
                 store32(out + j * kGroup + c * (64 / NG) + 16 * i, y + 8 * i);
+              if constexpr (NG == 8) *(uint4*)(out + j * kGroup + c * 8) = *(const uint4*)y;
             }
           }
         }
@@ -667,14 +692,14 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_after();
-        const int left = limit - kt * kKeys;  // keys of the tile that the row sees
-        const bool cut = __any_sync(0xffffffffu, left < kKeys), first = kt == done.t0;
+        const int left = limit - kt * T::kKeys;  // keys of the tile that the row sees
+        const bool cut = __any_sync(0xffffffffu, left < T::kKeys), first = kt == done.t0;
         const float* kb = k_back + (n & 3) * 4;
         const float* vu = v_up + (n & 3) * 4;
         // the largest x, then the base
         float top = -INFINITY;
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {  // two loads at a time on their way
+        for (int h = 0; h < T::kKeys / 64; ++h) {  // two loads at a time on their way
           uint32_t s[64];
           tld32(tS + 64 * h, s);
           tld32(tS + 64 * h + 32, s + 32);
@@ -714,7 +739,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         }
         m = base;
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {  // P goes over columns whose scores have been read: 16 c .. 16 c + 15
+        for (int h = 0; h < T::kKeys / 64; ++h) {  // P goes over columns whose scores have been read: 16 c .. 16 c + 15
           uint32_t s[64];
           tld32(tS + 64 * h, s);
           tld32(tS + 64 * h + 32, s + 32);
@@ -762,13 +787,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
 }  // namespace
 
 size_t rows_workspace(int head_dim, int sms) {
-  return (size_t)sms * 2 * (head_dim == 64 ? Tiles<2>::kSlot : Tiles<4>::kSlot) * sizeof(float);
+  return (size_t)sms * 2 * (head_dim == 64 ? Tiles<2>::kSlot : head_dim == 128 ? Tiles<4>::kSlot : Tiles<8>::kSlot) * sizeof(float);
 }
 
 void launch_rows(fopt_ctx* ctx, const AttnArgs& a, int head_dim, int sms) {
-  static std::atomic<uint64_t> done[2];
+  static std::atomic<uint64_t> done[3];
   auto go = [&](auto kernel, int smem) {
-    allow_shared(ctx, done[head_dim == 64], (const void*)kernel, smem);
+    allow_shared(ctx, done[head_dim / 128], (const void*)kernel, smem);
     // Beside tokens_kernel and not behind it: a batch of both kinds (6 sequences, 1999 keys the longest, 7 query heads
     // to a key head of 64) takes 32 us instead of 43, and where there are prompts alone tokens_kernel's empty launch
     // is hidden.
@@ -786,7 +811,8 @@ void launch_rows(fopt_ctx* ctx, const AttnArgs& a, int head_dim, int sms) {
     launched(ctx, "cache attention");
   };
   if (head_dim == 64) go(rows_kernel<2>, Tiles<2>::kBytes);
-  else go(rows_kernel<4>, Tiles<4>::kBytes);
+  else if (head_dim == 128) go(rows_kernel<4>, Tiles<4>::kBytes);
+  else go(rows_kernel<8>, Tiles<8>::kBytes);
 }
 
 }  // namespace kv

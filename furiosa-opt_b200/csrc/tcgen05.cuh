@@ -91,9 +91,9 @@ __device__ __forceinline__ uint64_t sdesc(uint32_t addr) {
 // layout: each 64-wide half of D is one TMA box of 128 keys x 128 bytes, 128-byte swizzled in 8-key
 // atoms. Leading byte offset = the distance between the two D halves (one box), stride byte offset =
 // the distance between 8-key atoms (1024 bytes); a 16-key MMA step starts 16 x 128 bytes further on.
-__device__ __forceinline__ uint64_t vdesc(uint32_t addr) {
+__device__ __forceinline__ uint64_t vdesc(uint32_t addr, uint32_t half = 16384) {  // bytes between two D halves
   uint64_t d = (uint64_t)((addr & 0x3FFFF) >> 4);
-  d |= (uint64_t)(16384 >> 4) << 16;
+  d |= (uint64_t)(half >> 4) << 16;
   d |= (uint64_t)(1024 >> 4) << 32;
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;

@@ -399,15 +399,16 @@ def test_attention_long_contexts(b200):
 WIDE = 400000
 
 
-@pytest.mark.parametrize("page", [16, 48, 64, 1024])
+@pytest.mark.parametrize("page,D", [(16, 128), (48, 128), (64, 128), (1024, 128), (16, 64), (48, 256), (1024, 256)])
 @pytest.mark.parametrize("causal", [True, False])
-def test_attention_pieces_and_single_tokens_in_wide_tables(b200, page, causal):
-    Case(b200, [1, 37, 0, 5, 3, 1, 64, 2], [260, 37, 99, 3, 0, 0, 129, 2], 2, 4, 128, page, pad=3, wide=WIDE).check(causal)
+def test_attention_pieces_and_single_tokens_in_wide_tables(b200, page, D, causal):
+    Case(b200, [1, 37, 0, 5, 3, 1, 64, 2], [260, 37, 99, 3, 0, 0, 129, 2], 2, 4, D, page, pad=3, wide=WIDE).check(causal)
 
 
 @pytest.mark.parametrize("D,H,group,q,n", [(128, 2, 4, 130, 300), (64, 1, 7, 200, 200), (128, 1, 1, 257, 513),
                                            (64, 2, 16, 40, 41), (128, 1, 32, 33, 100), (128, 1, 128, 2, 70),
-                                           (128, 1, 40, 16, 20000), (64, 1, 40, 5, 16385)])
+                                           (128, 1, 40, 16, 20000), (64, 1, 40, 5, 16385), (256, 1, 2, 70, 257),
+                                           (256, 2, 5, 130, 700), (256, 1, 40, 1, 64), (256, 1, 8, 16, 9000)])
 def test_attention_prompts_in_wide_tables(b200, D, H, group, q, n):
     for causal in (True, False):
         c = Case(b200, [q], [n], H, group, D, 32, seed=q, wide=WIDE)
@@ -417,14 +418,16 @@ def test_attention_prompts_in_wide_tables(b200, D, H, group, q, n):
 
 @pytest.mark.parametrize("size,bias", [(30.0, 1.0), (1e-4, 0.0), (0.0, 1.0), (1.0, 300.0)])
 def test_attention_of_sharp_and_flat_scores_in_wide_tables(b200, size, bias):
-    c = Case(b200, [1, 40], [500, 150], 1, 4, 128, 16, seed=11, size=size, bias=bias, wide=WIDE)
-    c.check()
-    c.check(scale=0.0)
-    c.check(scale=-0.05)
+    for D in (128, 256):
+        c = Case(b200, [1, 40], [500, 150], 1, 4, D, 16, seed=11, size=size, bias=bias, wide=WIDE)
+        c.check()
+        c.check(scale=0.0)
+        c.check(scale=-0.05)
 
 
-def test_attention_in_a_wide_table_reads_no_further_than_the_lengths(b200):
-    c = Case(b200, [1, 20, 1], [33, 40, 16], 2, 4, 128, 16, seed=14, wide=WIDE)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attention_in_a_wide_table_reads_no_further_than_the_lengths(b200, D):
+    c = Case(b200, [1, 20, 1], [33, 40, 16], 2, 4, D, 16, seed=14, wide=WIDE)
     want = c.check()
     q = c.q.copy()
     q[2, 3, 5], q[0, 1, 0] = np.nan, np.inf  # one row each
@@ -436,9 +439,10 @@ def test_attention_in_a_wide_table_reads_no_further_than_the_lengths(b200):
     assert np.isnan(got[2, 3]).all()
 
 
+@pytest.mark.parametrize("D", [128, 256])
 @pytest.mark.parametrize("power", [-100, -30, 30, 90])
-def test_attention_of_values_of_any_size_in_wide_tables(b200, power):
-    c = Case(b200, [1, 33], [200, 50], 1, 4, 128, 16, seed=12, wide=WIDE)
+def test_attention_of_values_of_any_size_in_wide_tables(b200, power, D):
+    c = Case(b200, [1, 33], [200, 50], 1, 4, D, 16, seed=12, wide=WIDE)
     s = F(2.0) ** F(power)
     for n in ("k", "v"):
         st = c.ref
