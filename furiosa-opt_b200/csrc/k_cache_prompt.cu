@@ -61,7 +61,10 @@ struct Tiles {
   static constexpr int D = NG * kGroup, kHalves = D / 64;
   static constexpr int kQueries = NG == 8 ? 1 : 2, kRows = 128 * kQueries;  // row tiles and rows of a segment
   static constexpr int kKeys = NG == 8 ? 64 : 128, kQuarters = kKeys / 32;  // of a key tile, and a warp's turns with its K
-  static constexpr int kExpand = NG == 8 ? 6 : 7;    // warps that expand codes
+  // Warps that expand codes. More than a tile and a half of turns would let a warp come to a stage two uses ahead, which
+  // the parity that it waits for could not tell: as it is, its turn before has waited for a product that comes, in the
+  // order of issue, behind the stage's last use but one.
+  static constexpr int kExpand = NG == 8 ? 6 : 7;
   static constexpr int kQ = kHalves * kHalf;         // bytes of Q_t
   static constexpr int kKeyHalf = kKeys * 128, kTile = kHalves * kKeyHalf;  // of 64 channels of a key tile, of K or V
   static constexpr int kKeyOffsets = kKeys * 32;     // of its offset step
