@@ -10,9 +10,9 @@
 // query rows (the query heads of one key head, of one or more tokens) as the 8 columns. A single token's
 // queries fill 4 to 8 of 128 rows of a tcgen05 tile and would need the codes expanded through shared memory;
 // here a lane turns the words that it loaded into fragments in registers. What bounds it is the issue slots of 12
-// warps an SM (168 registers a thread), then the cache's bytes: 87 us for one token of each of 64 sequences of 64
-// to 8192 keys, 8 key heads of 128 and 4 query heads to each, which is 3.6 TB/s of codes and scales, 0.55 of a copy's
-// rate; 76 us for two tokens at 131072 and 100003 keys. 16 warps at 128 registers spill (95 us for the first).
+// warps an SM (168 registers a thread), then the cache's bytes: 86 us for one token of each of 64 sequences of 64
+// to 8192 keys, 8 key heads of 128 and 4 query heads to each, which is 3.6 TB/s of codes and scales, 0.56 of a copy's
+// rate; 75 us for two tokens at 131072 and 100003 keys. 16 warps at 128 registers spill (95 us for the first).
 //   * K operand: lane (g, i) = (lane / 4, lane % 4) takes the 16-byte (D = 128) run of token g that the
 //     layout [D % 32 / 8, D / 32, D % 8] puts at i: word j is 8 channels of group j, which make its operand
 //     registers of two k16 steps; q's fragments are permuted to match. (x & 0x000f000f) ^ 0x00080008 is a
