@@ -657,6 +657,22 @@ def test_attention_in_a_capture_of_another_library(b200):
         assert np.array_equal(_down(o, w.shape), w)
 
 
+def test_attention_on_the_legacy_stream(b200):
+    """Both kernels on the stream that others wait for."""
+    c = Case(b200, [1, 130, 1], [700, 900, 5], 2, 4, 128, 16, seed=39, wide=WIDE)
+    want = c.check().astype(F)
+    o = fb.Storage(b200, "bf16", c.q.size)
+    b200.sync()
+    try:
+        b200.set_stream(0)
+        for _ in range(10):
+            c.run(out=o)
+        got = _down(o, want.shape)
+    finally:
+        b200.set_stream(None)
+    assert np.array_equal(got, want)
+
+
 def test_attention_past_32_bit_offsets(b200):
     """A cache whose images pass 2^32 bytes: pages at its far end are read and written where they are."""
     H, D, page, pages = 8, 256, 1024, 4200
