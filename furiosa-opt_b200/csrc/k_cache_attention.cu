@@ -799,8 +799,9 @@ extern "C" fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* 
     // 16 rows a block where a sequence has that many on average: the codes are expanded once for both halves
     const bool two = dim != 256 && (int64_t)tokens * a.group > 8 * (int64_t)batch;
     // Sequences of more than kv::kFewRows query rows go to rows_kernel, whose tiles of 256 rows take about as long
-    // as that many rows of tokens_kernel. The lengths are the device's, so both are launched, unless no sequence can be that long or the call has no more tokens than sequences:
-    // then it is single tokens, for which rows_kernel would only begin and end (4 us).
+    // as that many rows of tokens_kernel. The lengths are the device's, so both are launched, unless no sequence can
+    // be that long or the call has no more tokens than sequences: then it is single tokens, for which rows_kernel
+    // would only begin and end (4 us).
     // A call that leaves most of the device to tokens_kernel's blocks is its own as well, for rows_kernel's few blocks
     // take longer to begin, to end and over each segment. What each block would have at most, in tiles of 64 keys, decides,
     // from the table's width; the more keys, the more rows_kernel's parts cost. At 8 key heads of 128 and 4 query heads

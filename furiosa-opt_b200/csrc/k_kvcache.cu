@@ -292,12 +292,13 @@ __device__ __forceinline__ uint32_t code_of(float x, uint32_t scale) {
   return (uint32_t)(int)fminf(fmaxf(c, -8.0f), 7.0f) & 15u;
 }
 
-// The codes without a division for each: with t = x - z and r = 1 / s to an ulp, q = t r is off by less than 2^-22 of
-// itself; the remainder t - q s is exact (s has 8 bits, so it is a multiple of 2^-30 of the binade of t and below
-// 2^-20 of it), and q + (t - q s) r is t / s to 2^-46 before its rounding. Where t / s is a half, that rounds to
-// it; where it is not, t differs from that multiple of half a step by its own last place at least, which is more than
-// half a last place of the half (again as s has 8 bits): so the sum lies on the right side, as the division's
-// rounded quotient does. A step below 2^-100, whose remainders could underflow, takes the division.
+// The codes without a division for each, by the correction step of Markstein's division (IBM J. Res. Dev. 34, 1990):
+// with t = x - z and r = 1 / s to an ulp, q = t r is off by less than 2^-22 of itself; the remainder t - q s is exact
+// (s has 8 bits, so it is a multiple of 2^-30 of the binade of t and below 2^-20 of it), and q + (t - q s) r is t / s to
+// 2^-45 before its rounding. Where t / s is a half, that rounds to it; where it is not, t differs from that multiple of
+// half a step by its own last place at least, which is more than half a last place of the half (again as s has 8 bits):
+// so the sum lies on the right side, as the division's rounded quotient does. No quotient passes 2^20: a range that is
+// not zero is at least 2^-23 of the values. A step below 2^-100, whose remainders could underflow, takes the division.
 struct Steps {
   float s, z, r;
   __device__ __forceinline__ explicit Steps(uint32_t scale) {
