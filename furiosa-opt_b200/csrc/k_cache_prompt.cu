@@ -564,10 +564,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       *(uint4*)(tz + offsets_place(r, 1)) = make_uint4(z[4], z[5], z[6], z[7]);
       async_fence();
       mbar_arrive(smem_u32(&q_full[t]));
-      // not 0, so that a hidden key stays at -inf
-      return fmaxf(scalbnf(fabsf(a.scale) * kLog2e, e - 8), 0x1p-126f);
+      return scalbnf(fabsf(a.scale) * kLog2e, e - 8);
     };
 
+    // A tile's scores are the products times the row's factor and the keys' power of two: together not 0, for a hidden
+    // key's -inf is multiplied as well.
+    auto score_factor = [](float row, float keys) { return fmaxf(row * keys, 0x1p-126f); };
     uint32_t meetings = 0;
     auto meet = [&]() -> bool {  // a barrier of the tile's softmax threads whose wait is bounded
       mbar_arrive(smem_u32(&met[t]));
@@ -722,7 +724,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
               high[1] = max3(high[1], __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
             }
             high[0] = max3(high[0], __uint_as_float(y[30]), __uint_as_float(y[31]));
-            top = fmaxf(top, fmaf(fmaxf(high[0], high[1]), qs * kb[2 * h + c], vu[2 * h + c]));
+            top = fmaxf(top, fmaf(fmaxf(high[0], high[1]), score_factor(qs, kb[2 * h + c]), vu[2 * h + c]));
           }
         }
         const float base = first ? (top == -INFINITY ? 0.0f : top) : top > m + kLazyRows ? top : m;
@@ -754,7 +756,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
           }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float v_e = vu[2 * h + c], f = qs * kb[2 * h + c], up = v_e - m;
+            const float v_e = vu[2 * h + c], f = score_factor(qs, kb[2 * h + c]), up = v_e - m;
             const uint64_t f2 = pack_f32x2(f, f), up2 = pack_f32x2(up, up);
             uint64_t part[2] = {0, 0};
             uint32_t p[16];

@@ -1,0 +1,100 @@
+"""Attention over the 4-bit cache where its numbers are far apart: keys and values of very different sizes next to
+each other, seen, hidden and of no weight; against 64 bits.
+
+The bound is per key, so that a key of no weight allows no error. With p the probabilities and a stored number's parts
+(code + 8) step + |offset - 8 step|, an output is off by at most
+    sum p (2^-9 + 2 e + 2 sum p e) parts(v) + 2^-8 |o|,    e = 2^-19 |scale| sum |q| parts(k) + 2^-18:
+2^-9 for four roundings of 2^-11 (of a probability, of a value, and of both where they are small beside the largest),
+e for a score's f32 sums and its exponential, 2^-8 for the output's own rounding to bf16."""
+import numpy as np
+import pytest
+
+import furiosa_opt_b200 as fb
+from oracle import cache_ref as R
+from test_gpu_kvcache import WIDE, _bf, _down, _m, _up
+
+pytestmark = pytest.mark.gpu
+
+F = np.float32
+
+
+def _bound(q, ref, pages, q_len, n, scale, causal):
+    """(o, bound) [T, Hq, D] of one sequence's queries."""
+    T, Hq, D = q.shape
+    group = Hq // ref.heads
+    o, tol = np.zeros((T, Hq, D)), np.zeros((T, Hq, D))
+    K, V, KA, VA = ref.values("k"), ref.values("v"), ref.parts("k"), ref.parts("v")
+    for h in range(ref.heads):
+        k, v, ka, va = (x[pages, h].reshape(-1, D)[:n] for x in (K, V, KA, VA))
+        rows = slice(h * group, (h + 1) * group)
+        for t in range(T):
+            seen = max(0, n - q_len + t + 1) if causal else n
+            if not seen:
+                continue
+            qd = q[t, rows].astype(np.float64)
+            x = qd @ k[:seen].T * scale
+            p = np.exp(x - x.max(-1, keepdims=True))
+            p /= p.sum(-1, keepdims=True)
+            e = 2.0 ** -19 * abs(scale) * (np.abs(qd) @ ka[:seen].T) + 2.0 ** -18
+            with np.errstate(over="ignore", invalid="ignore"):
+                pe = np.where(p > 0, p * e, 0.0)
+            o[t, rows] = p @ v[:seen]
+            tol[t, rows] = (2.0 ** -9 * p + 2 * pe + 2 * p * pe.sum(-1, keepdims=True)) @ va[:seen] \
+                + 2.0 ** -8 * np.abs(o[t, rows])
+    return o, tol
+
+
+def _check(be, q, k, v, D, group, scale=None, causal=True, wide=False, page=16, slack=0.0):
+    """q [T, H group, D] over k, v [n, H, D] (f32), the last T tokens; beside it a sequence of one ordinary token, which
+    has nothing to do with it. Two runs give the same bits. `slack`: an error that is allowed besides."""
+    n, H, _ = k.shape
+    T = q.shape[0]
+    need = -(-n // page)
+    rng = np.random.default_rng(n)
+    order = rng.permutation(need + 2)
+    mine = order[:need]
+    ref, cache = R.Cache(need + 2, page, H, D), fb.PagedCache(be, need + 2, page, H, D)
+    slots = mine[np.arange(n) // page] * page + np.arange(n) % page
+    other = _bf(rng.standard_normal((1, H, D)))
+    for a, b, s in ((k, v, slots), (other, other, [order[need] * page])):
+        be.cache_append(cache, _up(be, a, "f32"), _up(be, b, "f32"), _up(be, s, "i32"))
+        ref.append(a, b, s)
+    width = max(need, -(-WIDE // page)) if wide else need
+    table = np.full((2, width), -1, np.int64)
+    table[0, :need], table[1, 0] = mine, order[need]
+    scale = D ** -0.5 if scale is None else scale
+    both = np.concatenate([q, _bf(rng.standard_normal((1, H * group, D)))])
+    args = (_up(be, both, "bf16"), cache, _up(be, table, "i32"), _up(be, [0, T, T + 1], "i32"), _up(be, [n, 1], "i32"), H * group)
+    got = _down(be.cache_attention(*args, scale=scale, causal=causal), both.shape).astype(np.float64)
+    again = _down(be.cache_attention(*args, scale=scale, causal=causal), both.shape)
+    be.sync()
+    assert np.array_equal(got, again.astype(np.float64), equal_nan=True)
+    want, tol = _bound(both[:T], ref, mine, T, n, scale, causal)
+    alone, tol1 = _bound(both[T:], ref, order[need:need + 1], 1, 1, scale, causal)
+    want, tol = np.concatenate([want, alone]), np.concatenate([tol, tol1])
+    assert np.isfinite(got).all(), np.argwhere(~np.isfinite(got))[:4]
+    err = np.abs(got - want) - tol - slack
+    assert np.all(err <= 0), (err.max(), np.unravel_index(err.argmax(), err.shape), np.count_nonzero(err > 0))
+
+
+def _plain(rng, n, H, D):
+    """Ordinary keys and values: channels of different sizes and means."""
+    k = rng.standard_normal((n, H, D)) * (0.5 + np.abs(rng.standard_normal((1, H, D)))) + rng.standard_normal((1, H, D))
+    v = rng.standard_normal((n, H, D)) + 0.2 * rng.standard_normal((1, H, D))
+    return k.astype(F), v.astype(F)
+
+
+KINDS = [(1, False), (20, False), (40, True)]  # new tokens, and whether the prompts' kernel takes them
+
+
+# ---- hidden keys beside scores that are zero ----
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("power", [-30, -100])
+@pytest.mark.parametrize("size,scale", [(0.0, None), (1.0, 0.0), (2.0 ** -20, None)])
+@pytest.mark.parametrize("T,wide", KINDS)
+def test_zero_scores_of_small_keys(b200, D, power, size, scale, T, wide):
+    """Queries, the scale or both so small that every score is zero, over small keys: the mean of what a row sees."""
+    rng = np.random.default_rng(1)
+    k, v = _plain(rng, 150, 1, D)
+    q = _bf(rng.standard_normal((T, 4, D)) * size)
+    _check(b200, q, np.ldexp(k, power), v, D, 4, scale=scale, wide=wide)
