@@ -113,61 +113,60 @@ struct fopt_graph {
   cudaGraphExec_t exec = nullptr;
   std::unordered_set<void*> owned;  // allocations of the capture that it did not free
   bool launched = false;
-  void* cache_ws = nullptr;         // this graph's own cache-attention workspace
-  size_t cache_ws_bytes = 0;
-  std::vector<void*> outgrown;      // smaller workspaces that earlier calls of the capture recorded
+  // This graph's own cache-attention workspaces: the one that calls of the capture take, and before it those that
+  // earlier calls recorded and later ones outgrew.
+  std::vector<fopt::Workspace> cache_ws;
   int64_t kernels = 0;              // kernels the captured step launches (counted per replay)
   int64_t launches_before = 0;
 };
 
 namespace fopt {
 
+static void clear_if_stale(fopt_ctx* ctx, Workspace& ws) {
+  if (ws.clear_at == ctx->expiries) return;
+  cuda_check(cudaMemsetAsync(ws.p, 0, ws.bytes, ctx->stream), "cache workspace clear");
+  ws.clear_at = ctx->expiries;
+}
+
 // Zeroed device memory that calls on one stream, or the calls of one captured graph, take turns with.
 // Eager calls share a buffer per stream and each graph has its own, so that launches which may overlap
-// (two streams, two graphs, a graph beside eager calls) never share one. Callers leave its counters zero.
+// (two streams, two graphs, a graph beside eager calls) never share one. Callers leave its counters zero; after an
+// expired wait, which may have left arrivals behind, it is cleared before its next use, on the stream of that use.
 void* cache_workspace(fopt_ctx* ctx, size_t bytes) {
-  auto zeroed = [&](size_t n) {
+  auto zeroed = [&](Workspace& ws) {
     void* p = nullptr;
-    cuda_check(cudaMalloc(&p, n), "cache workspace alloc");
+    cuda_check(cudaMalloc(&p, bytes), "cache workspace alloc");
     // on a stream of its own: the context's may be capturing
     cudaStream_t s;
     cuda_check(cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking), "cache workspace stream");
-    cudaError_t e = cudaMemsetAsync(p, 0, n, s);
+    cudaError_t e = cudaMemsetAsync(p, 0, bytes, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     cudaStreamDestroy(s);
     if (e != cudaSuccess) cudaFree(p);
     cuda_check(e, "cache workspace clear");
-    ctx->cache_ws_live[p] = n;
-    return p;
+    ws = {p, bytes, ctx->expiries};
   };
-  if (fopt_graph* g = ctx->capture) {
-    if (bytes > g->cache_ws_bytes) {
-      if (g->cache_ws) g->outgrown.push_back(g->cache_ws);
-      g->cache_ws = nullptr;
-      g->cache_ws_bytes = 0;
-      g->cache_ws = zeroed(bytes);
-      g->cache_ws_bytes = bytes;
+  if (fopt_graph* g = ctx->capture) {  // cleared before a launch, if it has to be
+    if (g->cache_ws.empty() || bytes > g->cache_ws.back().bytes) {
+      Workspace ws;
+      zeroed(ws);
+      g->cache_ws.push_back(ws);
     }
-    return g->cache_ws;
+    return g->cache_ws.back().p;
   }
-  auto& ws = ctx->cache_ws[ctx->stream];
-  if (bytes > ws.second) {
-    void* old = ws.first;
-    ws = {nullptr, 0};
-    ctx->cache_ws_live.erase(old);
+  Workspace& ws = ctx->cache_ws[ctx->stream];
+  if (bytes > ws.bytes) {
+    void* old = ws.p;
+    ws = {};
     if (old) cuda_check(cudaFree(old), "cache workspace free");  // waits for its last reader
-    ws.first = zeroed(bytes);
-    ws.second = bytes;
+    zeroed(ws);
   }
-  return ws.first;
+  clear_if_stale(ctx, ws);
+  return ws.p;
 }
 
-static void release_graph_ws(fopt_ctx* ctx, fopt_graph* g) {
-  if (g->cache_ws) g->outgrown.push_back(g->cache_ws);
-  for (void* p : g->outgrown) {
-    ctx->cache_ws_live.erase(p);
-    cudaFree(p);
-  }
+static void release_graph_ws(fopt_graph* g) {
+  for (Workspace& ws : g->cache_ws) cudaFree(ws.p);
 }
 
 }  // namespace fopt
@@ -182,12 +181,12 @@ fopt_status fopt_init(int device, fopt_ctx** out) {
     ctx->device = device;
     cuda_check(cudaStreamCreateWithFlags(&ctx->own_stream, cudaStreamNonBlocking), "stream create");
     ctx->stream = ctx->own_stream;
-    cuda_check(cudaMalloc(&ctx->dev_err, sizeof(int32_t)), "error word");
+    cuda_check(cudaMalloc(&ctx->dev_err, 2 * sizeof(int32_t)), "error words");
     cudaMemPool_t pool;
     cuda_check(cudaDeviceGetDefaultMemPool(&pool, device), "default mem pool");
     uint64_t keep = UINT64_MAX;
     cuda_check(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep), "mem pool threshold");
-    cuda_check(cudaMemset(ctx->dev_err, 0, sizeof(int32_t)), "error word");
+    cuda_check(cudaMemset(ctx->dev_err, 0, 2 * sizeof(int32_t)), "error words");
   });
   if (st != FOPT_OK) {
     g_noctx_err = ctx->err;
@@ -209,7 +208,7 @@ fopt_status fopt_destroy(fopt_ctx* ctx) {
   if (ctx->gemm_ws) cudaFree(ctx->gemm_ws);
   if (ctx->gemm_cnt) cudaFree(ctx->gemm_cnt);
   for (auto& kv : ctx->cache_ws)
-    if (kv.second.first) cudaFree(kv.second.first);
+    if (kv.second.p) cudaFree(kv.second.p);
   for (void* p : ctx->retired) cudaFree(p);
   if (ctx->copy_in) cudaStreamDestroy(ctx->copy_in);
   if (ctx->copy_out) cudaStreamDestroy(ctx->copy_out);
@@ -227,18 +226,19 @@ fopt_status fopt_destroy(fopt_ctx* ctx) {
 
 const char* fopt_last_error(const fopt_ctx* ctx) { return ctx ? ctx->err.c_str() : g_noctx_err.c_str(); }
 
-// After a stream sync: surface (and clear) a device-side bounded-wait expiry.
+// After a stream sync: surface (and clear) a device-side bounded-wait expiry, or an index that a kernel skipped.
 static void check_device_error(fopt_ctx* ctx) {
-  int32_t code = 0;
-  cuda_check(cudaMemcpy(&code, ctx->dev_err, sizeof(code), cudaMemcpyDeviceToHost), "error word read");
-  if (code) {
-    cuda_check(cudaMemset(ctx->dev_err, 0, sizeof(code)), "error word clear");
-    if (code >= kBadIndex) throw Fail{FOPT_ERR_INVALID, bad_index_message(code)};
-    ctx->gemm_cnt_dirty = true;
-    // a kernel that gave up may have left arrivals behind
-    for (auto& ws : ctx->cache_ws_live) cuda_check(cudaMemset(ws.first, 0, ws.second), "cache workspace clear");
-    throw Fail{FOPT_ERR_TIMEOUT, "a kernel's bounded wait expired (code " + std::to_string(code) + ")"};
-  }
+  int32_t code[2] = {0, 0};  // an expired wait, a bad index
+  cuda_check(cudaMemcpy(code, ctx->dev_err, sizeof(code), cudaMemcpyDeviceToHost), "error words read");
+  if (!code[0] && !code[1]) return;
+  cuda_check(cudaMemset(ctx->dev_err, 0, sizeof(code)), "error words clear");
+  const std::string index = code[1] ? bad_index_message(code[1]) : "";
+  if (!code[0]) throw Fail{FOPT_ERR_INVALID, index};
+  // a kernel that gave up may have left arrivals behind
+  ctx->gemm_cnt_dirty = true;
+  ctx->expiries++;
+  throw Fail{FOPT_ERR_TIMEOUT, "a kernel's bounded wait expired (code " + std::to_string(code[0]) + ")" +
+                                   (code[1] ? "; also, " + index : "")};
 }
 
 fopt_status fopt_sync(fopt_ctx* ctx) {
@@ -355,7 +355,7 @@ fopt_status fopt_capture_end(fopt_ctx* ctx, fopt_graph** out) {
     ctx->deferred_free.clear();
     if (e != cudaSuccess) {
       if (g->graph) cudaGraphDestroy(g->graph);
-      release_graph_ws(ctx, g);
+      release_graph_ws(g);
       delete g;
       cuda_check(e, "graph capture");
     }
@@ -369,6 +369,11 @@ fopt_status fopt_graph_launch(fopt_ctx* ctx, fopt_graph* g) {
   return guarded(ctx, [&] {
     require(g && g->exec, "fopt_graph_launch: no graph");
     require(!ctx->capture, "fopt_graph_launch: a capture is open");
+    for (Workspace& ws : g->cache_ws) clear_if_stale(ctx, ws);
+    if (ctx->gemm_cnt_dirty && ctx->gemm_cnt) {  // the graph may hold split GEMMs
+      cuda_check(cudaMemsetAsync(ctx->gemm_cnt, 0, ctx->gemm_cnt_n * 4, ctx->stream), "gemm counters clear");
+      ctx->gemm_cnt_dirty = false;
+    }
     cuda_check(cudaGraphLaunch(g->exec, ctx->stream), "cudaGraphLaunch");
     g->launched = true;
     ctx->launches += g->kernels;
@@ -387,7 +392,7 @@ fopt_status fopt_graph_destroy(fopt_ctx* ctx, fopt_graph* g) {
     cuda_check(cudaStreamSynchronize(ctx->stream), "sync");
     if (g->exec) cudaGraphExecDestroy(g->exec);
     if (g->graph) cudaGraphDestroy(g->graph);
-    release_graph_ws(ctx, g);
+    release_graph_ws(g);
     delete g;
     if (--ctx->graphs_alive == 0) {
       for (void* p : ctx->retired) cudaFree(p);

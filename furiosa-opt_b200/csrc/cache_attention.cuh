@@ -21,7 +21,8 @@ struct AttnArgs {
   const int32_t* table;
   const int32_t* q_start;
   const int32_t* kv_len;
-  int32_t* err;
+  int32_t* err;  // expired waits
+  int32_t* bad;  // indices that were skipped
   float* ws;          // partial results: two slots a block
   uint32_t* counter;  // arrivals at the segment that begins in a block; zero between launches
   int batch, tokens, width, hq, group;
@@ -48,8 +49,8 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
   s.queries = q1 - s.q0;
   s.rows = s.queries * a.group;
   s.keys = (int)min((int64_t)min(max(n, 0), kMostKeys), (int64_t)a.width * a.cache.page_size);
-  if (s.q0 != s0 || q1 != s1) atomicExch(a.err, kBadStart);
-  if (s.keys != n) atomicExch(a.err, kBadLength);
+  if (s.q0 != s0 || q1 != s1) atomicExch(a.bad, kBadStart);
+  if (s.keys != n) atomicExch(a.bad, kBadLength);
   return s;
 }
 // Keys that the sequence's query row sees (at most 0: none).

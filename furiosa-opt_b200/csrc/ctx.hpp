@@ -66,6 +66,15 @@ struct FoldKPlan {
 
 struct fopt_graph;
 
+namespace fopt {
+// Zeroed device memory whose counters kernels leave at zero, unless a wait of theirs expires.
+struct Workspace {
+  void* p = nullptr;
+  size_t bytes = 0;
+  uint64_t clear_at = 0;  // the context's expiries when it was last cleared
+};
+}  // namespace fopt
+
 struct fopt_ctx {
   int device = 0;
   fopt_graph* capture = nullptr;        // the step being captured into a CUDA graph, if any
@@ -83,7 +92,10 @@ struct fopt_ctx {
   std::map<std::string, std::shared_ptr<fopt::FoldKPlan>> folds;
   void* nccl_comm = nullptr;
   int nranks = 1, rank = 0;
-  int32_t* dev_err = nullptr;  // device error word: bounded waits that expire write a code here
+  // Two device error words, so that neither kind hides the other: bounded waits that expire write a code into the
+  // first, kernels that skip an index in device data into the second.
+  int32_t* dev_err = nullptr;
+  int32_t* bad_index() const { return dev_err + 1; }
   void* scratch = nullptr;  // grow-only device scratch for kernels that need it
   size_t scratch_bytes = 0;
   void* gemm_ws = nullptr;  // split-K partial accumulators of the paired GEMM's last wave
@@ -91,8 +103,8 @@ struct fopt_ctx {
   uint32_t* gemm_cnt = nullptr;  // arrival counters of the split tiles (zero between launches)
   size_t gemm_cnt_n = 0;
   bool gemm_cnt_dirty = false;
-  std::map<cudaStream_t, std::pair<void*, size_t>> cache_ws;  // cache-attention workspace of each stream
-  std::map<void*, size_t> cache_ws_live;  // these and the captured graphs' own, with their sizes
+  uint64_t expiries = 0;  // expired waits so far: a workspace that was last clear before one is cleared before its next use
+  std::map<cudaStream_t, fopt::Workspace> cache_ws;  // cache-attention workspace of each stream
   cudaStream_t copy_in = nullptr, copy_out = nullptr;  // host <-> device pipelines of the host-buffer calls
   void* pinned[2] = {nullptr, nullptr};  // host staging for file -> device streaming
   cudaEvent_t pinned_ev[2] = {nullptr, nullptr};
@@ -144,10 +156,8 @@ inline void launched(fopt_ctx* ctx, const char* what) {
 void* scratch(fopt_ctx* ctx, size_t bytes);
 void* cache_workspace(fopt_ctx* ctx, size_t bytes);
 
-// Codes of the device error word from kBadIndex on report an index in device data that a kernel skipped
-// (FOPT_ERR_INVALID); smaller ones are expired waits.
-constexpr int kBadIndex = 0x1000;
-constexpr int kBadSlot = kBadIndex, kBadPage = kBadIndex + 1, kBadLength = kBadIndex + 2, kBadStart = kBadIndex + 3;
+// Codes of the second error word: an index in device data that a kernel skipped (FOPT_ERR_INVALID).
+constexpr int kBadSlot = 1, kBadPage = 2, kBadLength = 3, kBadStart = 4;
 inline const char* bad_index_message(int code) {
   switch (code) {
     case kBadSlot: return "a cache slot past the cache's pages";

@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, tokens_blocks<NG, NB>()) tokens_kern
     bool there;
     auto enter = [&] {  // the page's first rows
       there = (uint32_t)page < (uint32_t)a.cache.pages;
-      if (!there && lane == 0) atomicExch(a.err, kBadPage);
+      if (!there && lane == 0) atomicExch(a.bad, kBadPage);
       k = k_head + (uint64_t)(uint32_t)page * page_codes;
       sc = sc_head + (uint64_t)(uint32_t)page * page_scales;
       page = ++page_at < page_end ? table[page_at] : 0;  // for the next time
@@ -785,6 +785,7 @@ extern "C" fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* 
     a.q_start = q_start;
     a.kv_len = kv_len;
     a.err = ctx->dev_err;
+    a.bad = ctx->bad_index();
     a.batch = batch;
     a.tokens = tokens;
     a.width = table_width;

@@ -243,7 +243,7 @@ __device__ __forceinline__ Spot spot_of(const AttnArgs& a, const Item& it, int t
 }
 __device__ __forceinline__ bool row_at(const AttnArgs& a, const Item& it, const Spot& p, int64_t& row) {
   const bool there = p.page >= 0 && p.page < a.cache.pages;
-  if (p.inside && !there) atomicExch(a.err, kBadPage);
+  if (p.inside && !there) atomicExch(a.bad, kBadPage);
   row = there ? ((int64_t)p.page * a.cache.heads + it.head) * a.cache.page_size + p.in_page : 0;
   return there;
 }

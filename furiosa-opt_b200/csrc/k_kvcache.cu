@@ -262,7 +262,7 @@ struct AppendArgs {
   const int32_t* slots;
   const int32_t* positions;
   int64_t k_stride, v_stride;
-  int32_t* err;
+  int32_t* bad;
   int tokens;
   int each;          // tokens a block
   FastDiv by_heads;
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, const __
     }
     if (!live || slot < 0) continue;
     if (slot >= a.cache.pages * a.cache.page_size) {
-      atomicExch(a.err, kBadSlot);
+      atomicExch(a.bad, kBadSlot);
       continue;
     }
     const int64_t to = row_of(a.cache, slot, h);
@@ -492,14 +492,14 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, const __
 // bf16, with one, two, four or eight words of a thread on their way.)
 template <bool F32, int NG>
 __global__ void __launch_bounds__(kThreads) read_kernel(Cache cache, void* out_k, void* out_v, const int32_t* slots,
-                                                        int64_t rows, FastDiv by_heads, int32_t* err) {
+                                                        int64_t rows, FastDiv by_heads, int32_t* bad) {
   using E = Elem<F32>;
   constexpr int D = NG * kGroup, W = D / 8;
   const int w = threadIdx.x % W;
   const int64_t row = (int64_t)blockIdx.x * (kThreads / W) + threadIdx.x / W;
   if (row >= rows) return;
   const int at = (int)fdiv(by_heads, (uint32_t)row), head = (int)row - at * cache.heads, slot = slots[at];
-  if (slot >= cache.pages * cache.page_size) atomicExch(err, kBadSlot);
+  if (slot >= cache.pages * cache.page_size) atomicExch(bad, kBadSlot);
   if (slot < 0 || slot >= cache.pages * cache.page_size) return;
   const bool value = blockIdx.y;
   const int64_t from = row_of(cache, slot, head);
@@ -659,7 +659,7 @@ fopt_status fopt_cache_append(fopt_ctx* ctx, const fopt_paged_cache* cache, cons
     a.positions = positions;
     a.k_stride = k_stride;
     a.v_stride = v_stride;
-    a.err = ctx->dev_err;
+    a.bad = ctx->bad_index();
     a.tokens = tokens;
     a.k_vec = kv::aligned16(k, k_stride, f32 ? 4 : 2);
     a.v_vec = kv::aligned16(v, v_stride, f32 ? 4 : 2);
@@ -685,7 +685,7 @@ fopt_status fopt_cache_read(fopt_ctx* ctx, void* out_k, void* out_v, fopt_dtype 
     auto go = [&](auto kernel) {
       const int64_t each = kv::kThreads / (dim / 8);
       kernel<<<dim3((unsigned)((rows + each - 1) / each), 2), kv::kThreads, 0, ctx->stream>>>(
-          c, out_k, out_v, slots, rows, make_fastdiv((uint32_t)c.heads), ctx->dev_err);
+          c, out_k, out_v, slots, rows, make_fastdiv((uint32_t)c.heads), ctx->bad_index());
       launched(ctx, "cache read");
     };
     if (dtype == FOPT_F32)

@@ -1,0 +1,85 @@
+"""What a device-side error leaves behind. The expired wait is made on the host: its code is written where a kernel would
+write it, and arrivals are left in a workspace as a kernel that gave up would leave them; no wait runs out."""
+import ctypes as C
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+import furiosa_opt_b200 as fb
+from furiosa_opt_b200 import _lib
+from test_gpu_kvcache import Case, _down, _up
+
+pytestmark = pytest.mark.gpu
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+SOURCE = """
+#include "ctx.hpp"
+extern "C" void* expired(fopt_ctx* c) { return c->dev_err; }
+extern "C" void* workspace(fopt_ctx* c) { return c->cache_ws.begin()->second.p; }
+"""
+
+
+@pytest.fixture(scope="module")
+def inside(tmp_path_factory):
+    """The addresses of a context's word for expired waits and of its only workspace."""
+    d = tmp_path_factory.mktemp("inside")
+    (d / "inside.cu").write_text(SOURCE)
+    csrc = os.path.join(os.path.dirname(HERE), "furiosa-opt_b200", "csrc")
+    subprocess.run(["nvcc", "-std=c++17", "-arch=sm_100a", "-shared", "-Xcompiler", "-fPIC", "-I", csrc, "-o", str(d / "inside.so"),
+                    str(d / "inside.cu")], check=True)
+    lib = C.CDLL(str(d / "inside.so"))
+    for f in (lib.expired, lib.workspace):
+        f.restype, f.argtypes = C.c_void_p, [C.c_void_p]
+    return lib
+
+
+def _write(be, address, words):
+    a = np.asarray(words, np.int32)
+    _lib.check(_lib.lib().fopt_h2d(be.ctx, address, a.ctypes.data, a.nbytes), be.ctx)
+
+
+def test_a_bad_index_does_not_hide_an_expired_wait(inside):
+    """Both are reported, once, and the arrivals that the wait left behind are gone for the next call."""
+    be = fb.B200(0)
+    c = Case(be, [1, 1], [9001, 40], 2, 4, 128, 64, seed=51)
+    good = c.check()
+    past = _up(be, [c.cache.slots], "i32")  # a slot past the cache
+    out = fb.Storage(be, "bf16", 256), fb.Storage(be, "bf16", 256)
+    _write(be, inside.expired(be.ctx), [401])
+    be.cache_read(c.cache, past, out=out)
+    with pytest.raises(fb._lib.FoptError, match="wait expired.*slot past") as e:
+        be.sync()
+    assert e.value.status == 5
+    be.sync()
+    be.cache_read(c.cache, past, out=out)
+    with pytest.raises(fb._lib.FoptError, match="slot past") as e:
+        be.sync()
+    assert e.value.status == 1
+    assert np.array_equal(_down(c.run(), c.q.shape), good)
+
+
+def test_an_expired_wait_leaves_no_arrivals(inside):
+    """Arrivals in the workspace of one stream, the wait reported on another."""
+    import torch
+    be = fb.B200(0)
+    c = Case(be, [1, 1], [9001, 40], 2, 4, 128, 64, seed=52)
+    side = torch.cuda.Stream()
+    be.sync()
+    be.set_stream(side.cuda_stream)  # the only stream that attention runs on, so that its workspace is the only one
+    want = _down(c.run(), c.q.shape)
+    graph = be.capture(lambda: c.run())
+    ws = inside.workspace(be.ctx)
+    be.set_stream(None)
+    for _ in range(2):
+        _write(be, ws, [1] * 1024)
+        _write(be, inside.expired(be.ctx), [401])
+        with pytest.raises(fb._lib.FoptError, match="wait expired"):
+            be.sync()
+        be.set_stream(side.cuda_stream)
+        for _ in range(2):
+            assert np.array_equal(_down(c.run(), c.q.shape), want)
+        assert np.array_equal(_down(graph.launch(), c.q.shape), want)
+        be.set_stream(None)
+    graph.close()
