@@ -23,9 +23,12 @@
 //     group for four tokens; byte permutes pair two tokens' channels.
 //   * probabilities go from the scores' fragment to the V product's by movmatrix, as p step in f16: half a
 //     step of it is 2^-11, an eighth of the output's own rounding. p offset is summed in f32.
-//   * the maximum moves only when a score exceeds it by 2^8 (a warp vote), so the rescaling is rare. Steps of V
-//     are scaled by a power of two that follows them the same way, which keeps p step within f16 at any
-//     magnitude of V.
+//   * the maximum moves only when a score exceeds it by 2^6 (a warp vote), so the rescaling is rare. Steps of V
+//     are scaled by a power of two that follows the largest the same way, which keeps p step within f16's upper end.
+//     Its lower end is looked at behind the last key: a product p step is off by 2^-11 of itself or by 2^-25 at most,
+//     so a run of n keys is right to 2^-10 of the sum of its products if that sum is 2^-14 n at least. Where one is
+//     not (a group whose steps are far below another's, or whose tokens of weight have steps far below those of
+//     tokens without), the warp takes its run once more, with products in f32.
 // Four warps take a run of 16-token tiles each, with their own rings of cp.async stages (no block barrier
 // while keys stream), and merge their (maximum, sum, output) at the end of a segment.
 //
@@ -48,7 +51,9 @@ constexpr int kLeast = 2;        // tiles of a share
 // (12.4 us; 14.0 with 4), of 8 at 15179 of two heads (20.6; 29.3 with 2), of 8 to 16 at 131072 of one (24.8; 26.8 with 5).
 constexpr float kByRoot = 0.4f;
 constexpr int kStages = 4;
-constexpr float kLazy = 8.0f;    // log2 by which a score may exceed the running maximum before it moves
+constexpr float kLazy = 6.0f;    // log2 by which a score may exceed the running maximum before it moves
+constexpr int kStepTop = 6;      // the largest step is brought to [2^6, 2^7) ...
+constexpr float kStepRoom = 512.0f;  // ... and may grow to 2^9: p step <= 2^15
 constexpr int kFewRows = 32;     // query rows per key head up to which a sequence is tokens_kernel's
 // The sequence's tiles (one at least: a sequence without keys still writes its rows), and how long its segments
 // and all of them together are in the division of work.
@@ -127,7 +132,7 @@ __device__ __forceinline__ float sum_over_g(float x) {
   return x;
 }
 
-// Shared memory of a block: the warps' rings, then (the rings drained) their partial outputs.
+// Shared memory of a block: the warps' rings, each then (drained) its warp's partial output.
 template <int NG, int NB>
 struct Shared {
   static constexpr int D = NG * kGroup, R = 8 * NB;
@@ -136,7 +141,8 @@ struct Shared {
   static constexpr int kStage = 2 * (kCodes + kScales);
   static constexpr int kRing = kStages * kStage;
   static constexpr int kRow = D + 4;                                    // floats; the pad spreads rows over banks
-  static constexpr int kBytes = kWarps * (kRing > R * kRow * 4 ? kRing : R * kRow * 4);
+  static_assert(R * kRow * 4 <= kRing);
+  static constexpr int kBytes = kWarps * kRing;
 };
 
 // Where a 16-byte chunk of a token's V codes sits in its row: rows two apart, which one load reads
@@ -151,15 +157,32 @@ __device__ __forceinline__ int v_chunk(int token, int chunk) {
 // A warp's state over a segment's keys.
 template <int NG, int NB>
 struct State {
-  // [channel 32 j + 4 g + 2 mm (+ 1 for c2, c3)] x [row 2 i, 2 i + 1]: sum of p step (code + 8), in 2^24 for the
-  // even channels (c0, c1) and 2^20 for the odd ones
+  // [channel 32 j + 4 g + 2 mm (+ 1 for c2, c3)] x [row 2 i, 2 i + 1]: sum of p step (code + 8). From the MMAs, in
+  // 2^24 for the even channels (c0, c1) and 2^20 for the odd ones
   float o[NB][NG][2][4];
   float e[NB][NG][2];      // sum of p (offset - 8 step), this lane's tokens
-  // p = 2^(score - m). The base m is that of p 2^-ev, so that p step fits f16 at any magnitude of V: it is the score's
-  // maximum (lagging by up to 2^kLazy) plus ev
+  // p = 2^(score - m). The base m is that of p 2^-ev, so that p step fits f16's upper end at any magnitude of V: it is
+  // the score's maximum (lagging by up to kLazy) plus ev
   float m[NB][2], l[NB][2];
   float ev;
-  float vlimit;            // the largest step that p step still holds
+  float vlimit;            // the largest step that p step still holds; infinite: products in f32, or to be done so
+  uint32_t stepped;        // groups of which a token of the lane's had a step, a bit each
+  __device__ __forceinline__ void clear(bool wide) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      m[nb][0] = m[nb][1] = 0.0f;
+      l[nb][0] = l[nb][1] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        e[nb][j][0] = e[nb][j][1] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[nb][j][0][c] = o[nb][j][1][c] = 0.0f;
+      }
+    }
+    stepped = 0;
+    ev = 0.0f;
+    vlimit = wide ? INFINITY : 0.0f;
+  }
 };
 
 template <int NG, int NB>
@@ -323,12 +346,12 @@ __device__ __forceinline__ void scores(const uint8_t* stage, const Places& at, c
   }
 }
 
-// The tile's softmax and its share of the output; token0 is its first.
+// The tile's softmax and its share of the output; token0 is its first. wide: the products in f32.
 template <int NG, int NB>
-__device__ __forceinline__ void values(const uint8_t* stage, const Places& at, int token0, int keys, int sure, bool first,
+__device__ __forceinline__ void values(const uint8_t* stage, const Places& at, int token0, int keys, int sure, bool first, bool wide,
                                        const Query<NG, NB>& q, State<NG, NB>& s, float (*x)[4]) {
   using S = Shared<NG, NB>;
-  const int lane = threadIdx.x & 31, g = lane >> 2;
+  const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
   uint32_t vm[2][NG];
 #pragma unroll
   for (int h = 0; h < 2; ++h) load_words<NG>(vm[h], stage + 2 * S::kCodes + S::kScales + at.scale + 8 * h * NG * 4);
@@ -359,17 +382,22 @@ __device__ __forceinline__ void values(const uint8_t* stage, const Places& at, i
     step[1][j] = step_of(vm[1][j]);
     steps = max3(steps, step[0][j], step[1][j]);
   }
+  if (s.stepped + 1 != 1u << NG) {  // seldom after the first tile
+#pragma unroll
+    for (int j = 0; j < NG; ++j) s.stepped |= (step[0][j] + step[1][j] > 0.0f) << j;
+  }
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) tops = max3(max3(tops, x[nb][0], x[nb][1]), x[nb][2], x[nb][3]);
   if (__any_sync(0xffffffffu, first || tops > kLazy - s.ev || steps > s.vlimit)) {
+    float lift = 0.0f;  // of ev, for p <= 2^kLazy
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) steps = fmaxf(steps, __shfl_xor_sync(0xffffffffu, steps, o));
-    float lift = 0.0f;  // of ev: the largest step to 2^ev [2^4, 2^5), and room up to 2^7: p <= 2^8 keeps 2^15
     if (steps > s.vlimit) {
-      const float ev = (float)max(ilogbf(steps) - 4, -100);  // further down p 2^-ev would pass the f32 range
+      const float ev = (float)max(ilogbf(steps) - kStepTop, -100);  // further down p 2^-ev would pass the f32 range
       lift = first ? 0.0f : ev - s.ev;
       s.ev = ev;
-      s.vlimit = fminf(exp2f(ev) * 0x1p7f, 0x1.fep127f);
+      s.vlimit = fminf(exp2f(ev) * kStepRoom, 0x1.fep127f);
+      if (lift > 100.0f) s.vlimit = INFINITY;  // what is scaled down past f32's range may have had weight
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -403,28 +431,130 @@ __device__ __forceinline__ void values(const uint8_t* stage, const Places& at, i
       x[nb][c] = exp2_(x[nb][c]);
       s.l[nb][c & 1] += x[nb][c];
     }
-  // V: words of tokens 2 i, 2 i + 1, 2 i + 8, 2 i + 9
-  uint32_t vw[4][NG / 2];
+  if (wide) {
 #pragma unroll
-  for (int t = 0; t < 4; ++t)  // (2 i + 1) / 2 and (2 i + 8) / 2 mod 4 are i: the chunk is the same
-    load_words<NG / 2>(vw[t], stage + S::kCodes + at.v + ((t & 1) + 8 * (t >> 1)) * (S::D / 2));
+    for (int j = 0; j < NG; ++j) {
+      const float z0 = fmaf(-8.0f, step[0][j], offset_of(vm[0][j])), z1 = fmaf(-8.0f, step[1][j], offset_of(vm[1][j]));
 #pragma unroll
-  for (int j = 0; j < NG; ++j) {
-    const uint32_t sel = j & 1 ? 0x7632u : 0x5410u;
-    const uint32_t x01 = __byte_perm(vw[0][j >> 1], vw[1][j >> 1], sel), x23 = __byte_perm(vw[2][j >> 1], vw[3][j >> 1], sel);
-    const uint32_t y01 = x01 >> 8, y23 = x23 >> 8;
-    const float s0 = step[0][j], s1 = step[1][j];
-    const float z0 = fmaf(-8.0f, s0, offset_of(vm[0][j])), z1 = fmaf(-8.0f, s1, offset_of(vm[1][j]));
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const uint32_t b0 = transposed(f16x2(x[nb][0] * s0, x[nb][1] * s0));
-      const uint32_t b1 = transposed(f16x2(x[nb][2] * s1, x[nb][3] * s1));
-      mma(s.o[nb][j][0], codes_low(at.masks, x01), codes_high(at.masks, x01), codes_low(at.masks, x23), codes_high(at.masks, x23), b0, b1);
-      mma(s.o[nb][j][1], codes_low(at.masks, y01), codes_high(at.masks, y01), codes_low(at.masks, y23), codes_high(at.masks, y23), b0, b1);
+        for (int c = 0; c < 2; ++c) s.e[nb][j][c] = fmaf(x[nb][c], z0, fmaf(x[nb][c + 2], z1, s.e[nb][j][c]));
+    }
+    // token by token: its probabilities from the lane that has them, its codes of this lane's channels
 #pragma unroll
-      for (int c = 0; c < 2; ++c) s.e[nb][j][c] = fmaf(x[nb][c], z0, fmaf(x[nb][c + 2], z1, s.e[nb][j][c]));
+    for (int h = 0; h < 2; ++h) {
+      const int left = min(8, keys - token0 - 8 * h);
+#pragma unroll 1
+      for (int tg = 0; tg < left; ++tg) {
+        const int t = 8 * h + tg, chunk = g * NG * 2;
+        uint32_t w[NG / 2];
+        load_words<NG / 2>(w, stage + S::kCodes + t * (S::D / 2) + v_chunk<NG>(t, chunk >> 4) * 16 + (chunk & 15));
+        const uint32_t* scale = (const uint32_t*)(stage + 2 * S::kCodes + S::kScales) + t * NG;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const float p0 = __shfl_sync(0xffffffffu, x[nb][2 * h], 4 * tg + i), p1 = __shfl_sync(0xffffffffu, x[nb][2 * h + 1], 4 * tg + i);
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            const float v = step_of(scale[j]);
+            const float v0 = p0 * v, v1 = p1 * v;
+            const uint32_t codes = (w[j >> 1] >> (16 * (j & 1))) ^ 0x8888u;  // code + 8 of the four channels
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float c = (float)(codes >> (4 * e) & 15u);
+              float* o = &s.o[nb][j][e >> 1][2 * (e & 1)];
+              o[0] = fmaf(v0, c, o[0]);
+              o[1] = fmaf(v1, c, o[1]);
+            }
+          }
+        }
+      }
+    }
+  } else {
+    // V: words of tokens 2 i, 2 i + 1, 2 i + 8, 2 i + 9
+    uint32_t vw[4][NG / 2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)  // (2 i + 1) / 2 and (2 i + 8) / 2 mod 4 are i: the chunk is the same
+      load_words<NG / 2>(vw[t], stage + S::kCodes + at.v + ((t & 1) + 8 * (t >> 1)) * (S::D / 2));
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const uint32_t sel = j & 1 ? 0x7632u : 0x5410u;
+      const uint32_t x01 = __byte_perm(vw[0][j >> 1], vw[1][j >> 1], sel), x23 = __byte_perm(vw[2][j >> 1], vw[3][j >> 1], sel);
+      const uint32_t y01 = x01 >> 8, y23 = x23 >> 8;
+      const float s0 = step[0][j], s1 = step[1][j];
+      const float z0 = fmaf(-8.0f, s0, offset_of(vm[0][j])), z1 = fmaf(-8.0f, s1, offset_of(vm[1][j]));
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const uint32_t b0 = transposed(f16x2(x[nb][0] * s0, x[nb][1] * s0));
+        const uint32_t b1 = transposed(f16x2(x[nb][2] * s1, x[nb][3] * s1));
+        mma(s.o[nb][j][0], codes_low(at.masks, x01), codes_high(at.masks, x01), codes_low(at.masks, x23), codes_high(at.masks, x23), b0, b1);
+        mma(s.o[nb][j][1], codes_low(at.masks, y01), codes_high(at.masks, y01), codes_low(at.masks, y23), codes_high(at.masks, y23), b0, b1);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) s.e[nb][j][c] = fmaf(x[nb][c], z0, fmaf(x[nb][c + 2], z1, s.e[nb][j][c]));
+      }
     }
   }
+}
+
+// Whether the products of a run of n keys may have lost too much to f16's lower end, for the whole warp: some row's
+// sum over some group is below 2^-14 n a channel, of codes + 8 that are 8 on average (the sum over its 32 channels is
+// compared, first a lane's four by themselves: where each of them suffices nothing is exchanged).
+template <int NG, int NB>
+__device__ __forceinline__ bool too_small(const State<NG, NB>& s, int n) {
+  auto lane_sum = [&](int nb, int j, int c) {
+    return fmaf(s.o[nb][j][0][c] + s.o[nb][j][1][c], 0x1p24f, (s.o[nb][j][0][c + 2] + s.o[nb][j][1][c + 2]) * 0x1p20f);
+  };
+  const float least = (float)n * (0x1p-14f * 8.0f * 32.0f);
+  bool low = false, lost = s.vlimit == INFINITY;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        low |= lane_sum(nb, j, c) < least * 0.125f;
+        lost |= fabsf(s.e[nb][j][c]) == INFINITY;  // offsets of another size than any step
+      }
+  if (!__any_sync(0xffffffffu, low || lost)) return false;
+  low = lost;
+  const uint32_t stepped = __reduce_or_sync(0xffffffffu, s.stepped);
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    if (!(stepped >> j & 1)) continue;  // no step: products of zeros
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float sum = sum_over_g(lane_sum(nb, j, c)), l = sum_over_g(s.l[nb][c]);  // by all lanes
+        low |= sum < least && l > 0.0f;
+      }
+  }
+  return __any_sync(0xffffffffu, low);
+}
+
+// The warp's part of the output, its rows' maxima and sums. What leaves has the score's base, which is comparable with
+// other warps'.
+template <int NG, int NB, typename Rows>
+__device__ __forceinline__ void leave(const State<NG, NB>& st, float even, float odd, float* out, Rows& ml) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
+  const float back = power((int)st.ev);
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int r = nb * 8 + 2 * i + c;
+      const float l = sum_over_g(st.l[nb][c]) * back;
+      if (g == 0) {
+        ml[0][warp][r] = l > 0.0f ? st.m[nb][c] - st.ev : kNone;
+        ml[1][warp][r] = l;
+      }
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        const float e = sum_over_g(st.e[nb][j][c]);
+        *(float4*)(out + r * Shared<NG, NB>::kRow + j * kGroup + 4 * g) =
+            make_float4(fmaf(st.o[nb][j][0][c], even, e) * back, fmaf(st.o[nb][j][0][c + 2], odd, e) * back,
+                        fmaf(st.o[nb][j][1][c], even, e) * back, fmaf(st.o[nb][j][1][c + 2], odd, e) * back);
+      }
+    }
 }
 
 // A block's partial results of the segment that it shares: [slot][row][D] outputs, then maxima and sums.
@@ -439,7 +569,7 @@ struct Partial {
 };
 
 template <int NG, int NB>
-__global__ void __launch_bounds__(kThreads, tokens_blocks<NG, NB>()) tokens_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, tokens_blocks<NG, NB>()) tokens_kernel(const __grid_constant__ AttnArgs a) {
   using S = Shared<NG, NB>;
   using P = Partial<NG, NB>;
   constexpr int D = S::D, R = S::R;
@@ -447,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, tokens_blocks<NG, NB>()) tokens_kern
   __shared__ float ml[2][kWarps][R];
   __shared__ float4 shares_of[kThreads];
   __shared__ int last;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i = lane & 3;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // rows_kernel, if it is launched behind, may begin: it works on other sequences, in memory of its own
   asm volatile("griddepcontrol.launch_dependents;");
@@ -500,131 +630,105 @@ __global__ void __launch_bounds__(kThreads, tokens_blocks<NG, NB>()) tokens_kern
     const int most = seen(a, s, row0 + rows - 1);
     const int sure = seen(a, s, row0);
     State<NG, NB> st;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      st.m[nb][0] = st.m[nb][1] = 0.0f;
-      st.l[nb][0] = st.l[nb][1] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        st.e[nb][j][0] = st.e[nb][j][1] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) st.o[nb][j][0][c] = st.o[nb][j][1][c] = 0.0f;
+    bool first;
+    // This warp's run of the segment's tiles, with products in f16 and, if they lost too much, once more in f32.
+    for (bool wide = false;; wide = true) {
+      st.clear(wide);
+      // the run's 16-token tiles, and where in which page it begins
+      const int tiles16 = max(0, (min(t1 * kTileTokens, most) - t0 * kTileTokens + 15) / 16);
+      int n = t0 * kWarps + tiles16 * warp / kWarps;
+      const int n1 = t0 * kWarps + tiles16 * (warp + 1) / kWarps;
+      const int32_t* table = a.table + (int64_t)b * a.width;
+      int page_at = (int)fdiv(a.cache.by_page, (uint32_t)n * 16);  // entry of the table that `page` is
+      const int page_end = (n1 * 16 + a.cache.page_size - 1) / a.cache.page_size;
+      const int begin = n * 16 - page_at * a.cache.page_size;  // within the first page
+      int left = (a.cache.page_size - begin) / 16;             // tiles of the page not yet fetched
+      int page = n < n1 ? table[page_at] : 0;
+      int fetched = n;
+      // a page of all heads is less than 2^32 bytes: its number times that is one instruction
+      const uint32_t page_codes = (uint32_t)a.cache.heads * a.cache.page_size * (D / 2);
+      const uint32_t page_scales = (uint32_t)a.cache.heads * a.cache.page_size * (NG * 4);
+      const uint8_t* k_head = k_lane + (int64_t)head * a.cache.page_size * (D / 2);
+      const uint8_t* sc_head = scale_lane + (int64_t)head * a.cache.page_size * (NG * 4);
+      const uint8_t *k, *sc;
+      bool there;
+      auto enter = [&] {  // the page's first rows
+        there = (uint32_t)page < (uint32_t)a.cache.pages;
+        if (!there && lane == 0) atomicExch(a.bad, kBadPage);
+        k = k_head + (uint64_t)(uint32_t)page * page_codes;
+        sc = sc_head + (uint64_t)(uint32_t)page * page_scales;
+        page = ++page_at < page_end ? table[page_at] : 0;  // for the next time
+      };
+      RawQuery<NG, NB> raw;  // on its way with the page number
+      raw.load(a, s, head, row0);
+      if (n < n1) {
+        enter();
+        k += begin * (D / 2);
+        sc += begin * (NG * 4);
       }
-    }
-    st.ev = 0.0f;
-    st.vlimit = 0.0f;
-
-    // this warp's run of the segment's 16-token tiles, and where in which page it begins
-    const int tiles16 = max(0, (min(t1 * kTileTokens, most) - t0 * kTileTokens + 15) / 16);
-    int n = t0 * kWarps + tiles16 * warp / kWarps;
-    const int n1 = t0 * kWarps + tiles16 * (warp + 1) / kWarps;
-    const int32_t* table = a.table + (int64_t)b * a.width;
-    int page_at = (int)fdiv(a.cache.by_page, (uint32_t)n * 16);  // entry of the table that `page` is
-    const int page_end = (n1 * 16 + a.cache.page_size - 1) / a.cache.page_size;
-    const int begin = n * 16 - page_at * a.cache.page_size;  // within the first page
-    int left = (a.cache.page_size - begin) / 16;             // tiles of the page not yet fetched
-    int page = n < n1 ? table[page_at] : 0;
-    int fetched = n;
-    // a page of all heads is less than 2^32 bytes: its number times that is one instruction
-    const uint32_t page_codes = (uint32_t)a.cache.heads * a.cache.page_size * (D / 2);
-    const uint32_t page_scales = (uint32_t)a.cache.heads * a.cache.page_size * (NG * 4);
-    const uint8_t* k_head = k_lane + (int64_t)head * a.cache.page_size * (D / 2);
-    const uint8_t* sc_head = scale_lane + (int64_t)head * a.cache.page_size * (NG * 4);
-    const uint8_t *k, *sc;
-    bool there;
-    auto enter = [&] {  // the page's first rows
-      there = (uint32_t)page < (uint32_t)a.cache.pages;
-      if (!there && lane == 0) atomicExch(a.bad, kBadPage);
-      k = k_head + (uint64_t)(uint32_t)page * page_codes;
-      sc = sc_head + (uint64_t)(uint32_t)page * page_scales;
-      page = ++page_at < page_end ? table[page_at] : 0;  // for the next time
-    };
-    RawQuery<NG, NB> raw;  // on its way with the page number
-    raw.load(a, s, head, row0);
-    if (n < n1) {
-      enter();
-      k += begin * (D / 2);
-      sc += begin * (NG * 4);
-    }
-    uint32_t into = 0, from = 0;  // stages, in bytes
-    auto fetch = [&] {
-      if (fetched < n1) {
-        if (left == 0) {
-          left = a.cache.page_size / 16;
-          enter();
+      uint32_t into = 0, from = 0;  // stages, in bytes
+      auto fetch = [&] {
+        if (fetched < n1) {
+          if (left == 0) {
+            left = a.cache.page_size / 16;
+            enter();
+          }
+          const uint32_t to = ring_u32 + into;
+          if (there) {
+#pragma unroll
+            for (int c = 0; c * 32 < S::kCodes / 16; ++c) copy16(to + c * 512, k + c * 512);
+#pragma unroll
+            for (int c = 0; c * 32 < S::kCodes / 16; ++c) copy16(to + (c & 1 ? v_to1 : v_to0) + c * 512, k + v_from_k + c * 512);
+#pragma unroll
+            for (int c = 0; c * 32 < S::kScaleLanes; ++c)
+              if (lane < S::kScaleLanes) copy16(to + scale_to + c * 256, sc + c * 256);
+          } else {
+            for (int c = lane; c < S::kStage / 16; c += 32) *(uint4*)(ring + into + c * 16) = make_uint4(0, 0, 0, 0);
+          }
+          k += S::kCodes;
+          sc += S::kScales;
+          --left;
+          ++fetched;
         }
-        const uint32_t to = ring_u32 + into;
-        if (there) {
-#pragma unroll
-          for (int c = 0; c * 32 < S::kCodes / 16; ++c) copy16(to + c * 512, k + c * 512);
-#pragma unroll
-          for (int c = 0; c * 32 < S::kCodes / 16; ++c) copy16(to + (c & 1 ? v_to1 : v_to0) + c * 512, k + v_from_k + c * 512);
-#pragma unroll
-          for (int c = 0; c * 32 < S::kScaleLanes; ++c)
-            if (lane < S::kScaleLanes) copy16(to + scale_to + c * 256, sc + c * 256);
-        } else {
-          for (int c = lane; c < S::kStage / 16; c += 32) *(uint4*)(ring + into + c * 16) = make_uint4(0, 0, 0, 0);
-        }
-        k += S::kCodes;
-        sc += S::kScales;
-        --left;
-        ++fetched;
-      }
-      copies_commit();
-      into = into + S::kStage == S::kRing ? 0 : into + S::kStage;
-    };
+        copies_commit();
+        into = into + S::kStage == S::kRing ? 0 : into + S::kStage;
+      };
 #pragma unroll 1
-    for (int c = 0; c < kStages - 1; ++c) fetch();
-    Query<NG, NB> q;
-    load_query<NG, NB>(a, s, row0, raw, q);  // while the first keys are on their way
-    // A tile's scores are computed while the tile before is finished: two independent chains of instructions.
-    auto next_stage = [](uint32_t at) { return at + S::kStage == S::kRing ? 0 : at + S::kStage; };
-    float x[NB][4];
-    if (n < n1) {
-      copies_wait<kStages - 2>();
-      __syncwarp();
-      scores<NG, NB>(ring, at, q, x);
-    }
-    bool first = true;
-#pragma unroll 1
-    for (; n < n1; ++n) {
-      fetch();
-      copies_wait<kStages - 2>();
-      __syncwarp();
-      const uint32_t then = next_stage(from);
-      float ahead[NB][4];
-      scores<NG, NB>(ring + then, at, q, ahead);  // behind the last tile: of what the stage holds, and not used
-      values<NG, NB>(ring + from, at, n * 16, s.keys, sure, first, q, st, x);
-      first = false;
-      __syncwarp();  // all lanes have read the stage before the next copies into it
-      from = then;
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) x[nb][c] = ahead[nb][c];
-    }
-    copies_wait<0>();
-    __syncthreads();  // every warp's ring is drained: the outputs go over them
-
-    float* out = (float*)smem + warp * R * S::kRow;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int r = nb * 8 + 2 * i + c;
-        const float l = sum_over_g(st.l[nb][c]);
-        if (g == 0) {
-          ml[0][warp][r] = l > 0.0f ? st.m[nb][c] : kNone;
-          ml[1][warp][r] = l;
-        }
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
-          const float e = sum_over_g(st.e[nb][j][c]);
-          *(float4*)(out + r * S::kRow + j * kGroup + 4 * g) =
-              make_float4(fmaf(st.o[nb][j][0][c], 0x1p24f, e), fmaf(st.o[nb][j][0][c + 2], 0x1p20f, e),
-                          fmaf(st.o[nb][j][1][c], 0x1p24f, e), fmaf(st.o[nb][j][1][c + 2], 0x1p20f, e));
-        }
+      for (int c = 0; c < kStages - 1; ++c) fetch();
+      Query<NG, NB> q;
+      load_query<NG, NB>(a, s, row0, raw, q);  // while the first keys are on their way
+      // A tile's scores are computed while the tile before is finished: two independent chains of instructions.
+      auto next_stage = [](uint32_t at) { return at + S::kStage == S::kRing ? 0 : at + S::kStage; };
+      float x[NB][4];
+      if (n < n1) {
+        copies_wait<kStages - 2>();
+        __syncwarp();
+        scores<NG, NB>(ring, at, q, x);
       }
+      first = true;
+#pragma unroll 1
+      for (; n < n1; ++n) {
+        fetch();
+        copies_wait<kStages - 2>();
+        __syncwarp();
+        const uint32_t then = next_stage(from);
+        float ahead[NB][4];
+        scores<NG, NB>(ring + then, at, q, ahead);  // behind the last tile: of what the stage holds, and not used
+        values<NG, NB>(ring + from, at, n * 16, s.keys, sure, first, wide, q, st, x);
+        first = false;
+        __syncwarp();  // all lanes have read the stage before the next copies into it
+        from = then;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) x[nb][c] = ahead[nb][c];
+      }
+      copies_wait<0>();
+      __syncwarp();  // the ring is drained: the warp's output goes over it
+      if (!wide && !first && too_small<NG, NB>(st, (tiles16 / kWarps + 1) * 16)) continue;
+      leave<NG, NB>(st, wide ? 1.0f : 0x1p24f, wide ? 1.0f : 0x1p20f, (float*)ring, ml);
+      break;
+    }
     __syncthreads();
 
     auto write_row = [&](int r, int d, float4 v, float l) {  // channels d .. d + 3 of row r
@@ -645,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, tokens_blocks<NG, NB>()) tokens_kern
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float f = exp2_(ml[0][w][r] - m);
-        const float4 v = *(const float4*)((const float*)smem + (w * R + r) * S::kRow + d);
+        const float4 v = *(const float4*)((const float*)(smem + w * S::kRing) + r * S::kRow + d);
         l = fmaf(f, ml[1][w][r], l);
         sum.x = fmaf(f, v.x, sum.x), sum.y = fmaf(f, v.y, sum.y), sum.z = fmaf(f, v.z, sum.z), sum.w = fmaf(f, v.w, sum.w);
       }

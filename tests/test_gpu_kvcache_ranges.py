@@ -85,6 +85,7 @@ def _plain(rng, n, H, D):
 
 
 KINDS = [(1, False), (20, False), (40, True)]  # new tokens, and whether the prompts' kernel takes them
+FEW = KINDS[:2]
 
 
 # ---- hidden keys beside scores that are zero ----
@@ -98,3 +99,119 @@ def test_zero_scores_of_small_keys(b200, D, power, size, scale, T, wide):
     k, v = _plain(rng, 150, 1, D)
     q = _bf(rng.standard_normal((T, 4, D)) * size)
     _check(b200, q, np.ldexp(k, power), v, D, 4, scale=scale, wide=wide)
+
+
+# ---- values far smaller or larger than 1, and of both kinds in one sequence ----
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("power", [-115, -100, 97])
+@pytest.mark.parametrize("T,wide", FEW)
+def test_many_equal_scores_over_values_of_any_size(b200, D, power, T, wide):
+    """The sum of the probabilities stays in range however the values are scaled."""
+    rng = np.random.default_rng(2)
+    k, v = _plain(rng, 900, 1, D)
+    q = np.zeros((T, 4, D), F)
+    v = np.ldexp(np.clip(v, -6, 6) + F(2), power)  # means that do not cancel
+    _check(b200, q, k, v, D, 4, wide=wide, slack=2.0 ** -126)  # smaller numbers are zeros
+
+
+def _aimed(rng, T, group, D):
+    """Queries near the direction of ones: keys of `a` in every channel score a sqrt(D) (1 +- 0.1) or so."""
+    return _bf(1 + 0.25 * rng.standard_normal((T, group, D)))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("low,high", [(-60, 90), (-100, 40), (-20, 20)])
+@pytest.mark.parametrize("weight", [True, False])  # whether the large values have any
+@pytest.mark.parametrize("large_first", [True, False])
+@pytest.mark.parametrize("T,wide", FEW)
+def test_small_values_beside_large_ones(b200, D, low, high, weight, large_first, T, wide):
+    """Runs of tiny values and of huge ones, which different warps and blocks meet: where the huge ones have no
+    weight, the output is of the tiny ones."""
+    rng = np.random.default_rng(3)
+    k, v = _plain(rng, 2500, 1, D)
+    large = np.arange(2500) < 1100 if large_first else np.arange(2500) >= 1400
+    large[-T:] = False  # the new tokens' own
+    v = np.ldexp(v, np.where(large, high, low)[:, None, None]).astype(F)
+    if not weight:
+        k[large] = -60
+    _check(b200, _aimed(rng, T, 4, D), k, v, D, 4, wide=wide, slack=2.0 ** -126)
+
+
+# ---- one key apart from all others ----
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("power", [10, 14, 18, 22, 40, 128])
+@pytest.mark.parametrize("at", [0, 137, 940])
+@pytest.mark.parametrize("T,wide", FEW)
+def test_a_large_value_of_no_weight(b200, D, power, at, T, wide):
+    """One key that no query wants, with a value 2^power times as large as the others (past 2^127: infinite)."""
+    rng = np.random.default_rng(4)
+    k, v = _plain(rng, 1000, 1, D)
+    k[at] = -60
+    with np.errstate(over="ignore"):
+        v[at] = v[at] * F(2) ** F(power)
+    _check(b200, _aimed(rng, T, 4, D), k, v, D, 4, wide=wide)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("power", [16, 30, 60, 128])
+@pytest.mark.parametrize("which", ["k", "v", "kv"])
+@pytest.mark.parametrize("T,wide", [(20, False)])
+def test_a_large_key_and_value_that_most_rows_do_not_see(b200, D, power, which, T, wide):
+    """A new token whose key, value or both are 2^power times the others' or infinite: the tokens before it do not
+    see it, and their answers are what they are without it."""
+    rng = np.random.default_rng(5)
+    k, v = _plain(rng, 300, 2, D)
+    q = _bf(rng.standard_normal((T, 8, D)))
+    with np.errstate(over="ignore"):
+        for n, x in (("k", k), ("v", v)):
+            if n in which:
+                x[296] = np.abs(x[296]) * F(2) ** F(power)
+    q[-4:] = -np.abs(q[-4:])  # who sees it does not want it
+    if "k" not in which:
+        k[296] = 60
+    _check(b200, q, k, v, D, 4, wide=wide)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("power", [12, 20, 60, 128])
+@pytest.mark.parametrize("at", [3, 137])
+@pytest.mark.parametrize("T,wide", FEW)
+def test_a_large_key_of_no_weight(b200, D, power, at, T, wide):
+    """A key 2^power times as long as the others that every query turns away from."""
+    rng = np.random.default_rng(6)
+    k, v = _plain(rng, 300, 1, D)
+    with np.errstate(over="ignore"):
+        k[at] = -F(8) * F(2) ** F(power)
+    _check(b200, _aimed(rng, T, 4, D), k, v, D, 4, wide=wide)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("power", [8, 16, 40, 128])
+@pytest.mark.parametrize("T,wide", FEW)
+def test_a_large_channel_leaves_other_groups_alone(b200, D, power, T, wide):
+    """A key like any other, one of whose channels has a value 2^power times the rest: what its group's other channels
+    can say goes, other groups' outputs stay. The prompts' kernel follows a token's largest group, and the others as
+    long as they are no less than 2^-18 of it."""
+    if wide and power > 16:
+        pytest.skip("past what the prompts' kernel holds")
+    rng = np.random.default_rng(7)
+    k, v = _plain(rng, 400, 1, D)
+    with np.errstate(over="ignore"):
+        v[77, 0, 5] = F(3) * F(2) ** F(power)
+    _check(b200, _bf(rng.standard_normal((T, 4, D))), k, v, D, 4, wide=wide)
+
+
+# ---- many keys of little weight each ----
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bits", [14, 18, 22, 25])
+@pytest.mark.parametrize("sink", [1.0, 2.0 ** -6])  # the size of the heavy key's own value
+@pytest.mark.parametrize("T,wide", FEW)
+def test_a_long_flat_tail_behind_one_heavy_key(b200, D, bits, sink, T, wide):
+    """The first key has 2^bits times the weight of each of 20000 equal others."""
+    rng = np.random.default_rng(8)
+    n = 20000
+    k = np.zeros((n, 1, D), F)
+    v = np.broadcast_to(rng.standard_normal((1, 1, D)).astype(F) + F(1), (n, 1, D)).copy()
+    k[0] = bits * np.log(2) / D ** 0.5  # times ones
+    v[0] = rng.standard_normal((1, D)) * sink
+    _check(b200, np.ones((T, 2, D), F), k, v, D, 2, wide=wide, page=64)
