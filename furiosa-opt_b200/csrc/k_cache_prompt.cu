@@ -21,8 +21,9 @@
 //
 // f16 holds 11 bits of a value where bf16 would hold 8, but not every size of it: every 32
 // tokens' K is scaled by a power of two and V by another, so that the largest is in [2^4, 2^9). K's comes back with the
-// scores. V's, 2^ev, goes into the exponent: with x = score + ev, P = 2^(x - m) and l = sum P 2^-ev, O = sum P V 2^-ev
-// and l share the base m, which follows the largest x as it would the largest score.
+// scores. V's, 2^ev, goes into the exponent: with x = score + ev, P = 2^(x - m) and O = sum P V 2^-ev, where the base m
+// follows the largest x. The sum of probabilities has a base of its own, a score n near the largest: l = sum P
+// 2^(m - ev - n), so that V's size takes nothing from its range; outputs are O / l 2^(m - n).
 //
 // A 16-byte chunk holds 8 codes in the order that pairs come out of a word (0, 4, 1, 5, 2, 6, 3, 7): for K the
 // queries are stored in the same order, for V the output's columns are put right when they leave.
@@ -51,6 +52,8 @@ constexpr int kLeast = 4;                // units of a share
 constexpr float kByRoot = 1.0f;
 constexpr int kUncut = 8;                // segments of fewer tiles are not shared between blocks
 constexpr float kLazyRows = 14.0f;        // log2 by which x may exceed its base: P stays within f16, the base moves rarely
+constexpr float kLazySum = 20.0f;         // ... and a score that of l, where it is looked at
+constexpr float kFarBack = 80.0f;         // log2 up to which P gives its share of l: probabilities below 2^-46 may vanish
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // At D = 256 one 128-row tile of queries and 64 keys at a time are what tensor memory (64 columns of scores, 256 of
@@ -73,7 +76,7 @@ struct Tiles {
   static constexpr int kRaw = 32 * NG * 16;  // what a warp holds of 32 tokens' K or V
   static constexpr int kAll = kQueries * (kQ + kOffsets) + 4 * kTile + 2 * kKeyOffsets + kExpand * kRaw + 1024 + 512;
   static constexpr int kBytes = kAll > 120000 ? kAll : 120000;
-  static constexpr int kSlot = kRows * (D + 2);      // floats of a partial result
+  static constexpr int kSlot = kRows * (D + 3);      // floats of a partial result
 
   static __device__ __forceinline__ int blocks_of(const Seq& s) { return (s.rows + kRows - 1) / kRows; }
   // Key tiles of a row block: up to the last key that its last row sees, one at least.
@@ -248,14 +251,16 @@ __device__ __forceinline__ bool row_at(const AttnArgs& a, const Item& it, const 
   return there;
 }
 
-// The exponent that brings the largest of a warp's values to [2^4, 2^9), from the sizes of their groups.
+constexpr int kLowest = -120;  // of the exponents
+
+// The exponent that brings the largest of a warp's values to [2^4, 2^9), from the sizes of their groups; `none` for zeros.
 template <int NG>
-__device__ __forceinline__ int warp_exponent(const uint32_t* scales) {
+__device__ __forceinline__ int warp_exponent(const uint32_t* scales, int none) {
   float top = 0.0f;
 #pragma unroll
   for (int j = 0; j < NG; ++j) top = fmaxf(top, fmaf(8.0f, step_of(scales[j]), fabsf(offset_of(scales[j]))));
   const uint32_t all = __reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu);
-  return all ? min(max((int)(all >> 23) - 127 - 4, -120), 120) : 0;
+  return all ? min(max((int)(all >> 23) - 127 - 4, kLowest), 120) : none;
 }
 
 template <int NG>
@@ -392,8 +397,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
     uint4* mine = (uint4*)(raw + (warp - 1) * T::kRaw) + lane;
     uint4 codes[NG];
     uint32_t scales[NG];
-    int low_v = 0;
-    bool fresh = true;  // the segment's first V of this warp
     bool ok = true;
     int t = more ? it.t0 : 0;
     constexpr int kQuarters = T::kQuarters;
@@ -403,7 +406,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         u -= 2 * kQuarters;
         ++n;
         if (++t == it.t1) {
-          fresh = true;
           more = walk.next(it);
           t = it.t0;
         }
@@ -423,12 +425,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       const uint32_t full = smem_u32(is_v ? &v_full[stage] : &k_full[stage]);
       const uint32_t empty = smem_u32(is_v ? &v_empty[stage] : &k_empty[stage]), parity = ((n >> 1) & 1) ^ 1;
       const uint32_t known = smem_u32(&x_full[n & 3]);
-      int e = warp_exponent<NG>(scales);
-      if (is_v) {  // V far below the segment's first is not brought up all the way: l would pass the f32 range
-        if (fresh) low_v = e - 40;
-        fresh = false;
-        e = max(e, low_v);
-      }
+      // zeros of V do not lift the base of P; what is past the keys has no part in it
+      const int e = warp_exponent<NG>(scales, is_v && t * T::kKeys + quarter * 32 < it.s.keys ? kLowest : 0);
       const float f = power(-e);
       // by code word of a piece (of two, where K's group of words is two pieces): steps and offsets of what its pairs of
       // codes are (see the loop)
@@ -576,9 +574,21 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       const bool here = mbar_wait(smem_u32(&met[t]), meetings++ & 1, abort_flag, a.err, 424);
       return __all_sync(0xffffffffu, here);
     };
+    auto scale_outputs = [&](float f) {  // the row's O_t, complete and not being added to
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tld32(tO + 32 * c, o);
+        tld_wait_regs(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+        tst32(tO + 32 * c, o);
+      }
+      tst_wait();
+    };
     bool ok = true;
     Item done;  // the segment whose output is still in O_t
-    float qs = 0.0f, m = 0.0f, l = 0.0f;
+    float qs = 0.0f, m = 0.0f, l = 0.0f, ml = 0.0f;  // ml: the base of l
     int n = 0;
     // Each part stands here once, in one place: the roles' code together has to stay in the instruction cache.
     for (int seg = 0; more || seg; ++seg) {
@@ -594,8 +604,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         if (!ok) break;
         fence_after();
         const bool whole = done.t0 == 0 && done.t1 == done.tiles, rows = done.row0 + t * 128 < done.s.rows;
-        // partial results: [D / 4][128] float4, so that a warp's rows are contiguous, then maxima and sums
-        auto slot = [&](int block, bool begins) { return a.ws + ((int64_t)block * 2 + begins) * T::kSlot + t * 128 * (D + 2); };
+        // partial results: [D / 4][128] float4, so that a warp's rows are contiguous, then the bases and sums
+        auto slot = [&](int block, bool begins) { return a.ws + ((int64_t)block * 2 + begins) * T::kSlot + t * 128 * (D + 3); };
         int c0 = 0, c1 = 0;
         bool output = rows;
         if (!whole && rows) {
@@ -608,8 +618,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) ((float4*)part)[(8 * c + i) * 128 + r] = *(float4*)(o + 4 * i);
           }
-          part[D * 128 + r] = l > 0.0f ? m : l == l ? kNone : m;  // a NaN sum stays one
-          part[D * 128 + 128 + r] = l;
+          part[D * 128 + r] = l == 0.0f ? kNone : m;  // a NaN sum stays one
+          part[D * 128 + 128 + r] = l == 0.0f ? kNone : ml;
+          part[D * 128 + 256 + r] = l;
           c0 = shares.owner(done.at + kCost);
           c1 = shares.owner(done.at + done.tiles + kCost - 1);
           if (!(ok = meet())) break;
@@ -624,14 +635,18 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
           output = last[t];
           if (!(ok = meet())) break;  // last[t] has been read
           if (output) {  // the parts' sum goes into O_t
-            float top = kNone;
+            m = ml = kNone;
             l = 0.0f;
-#pragma unroll 4
-            for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(slot(c, c == c0) + D * 128 + r));
 #pragma unroll 4
             for (int c = c0; c <= c1; ++c) {
               const float* q = slot(c, c == c0) + D * 128 + r;
-              l = fmaf(exp2_(__ldcg(q) - top), __ldcg(q + 128), l);
+              m = fmaxf(m, __ldcg(q));
+              ml = fmaxf(ml, __ldcg(q + 128));
+            }
+#pragma unroll 4
+            for (int c = c0; c <= c1; ++c) {
+              const float* q = slot(c, c == c0) + D * 128 + 128 + r;
+              l = fmaf(exp2_(__ldcg(q) - ml), __ldcg(q + 128), l);
             }
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -641,7 +656,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
 #pragma unroll 2
               for (int b = c0; b <= c1; ++b) {
                 const float* q = slot(b, b == c0);
-                const float f = exp2_(__ldcg(q + D * 128 + r) - top);
+                const float f = exp2_(__ldcg(q + D * 128 + r) - m);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                   const float4 v = __ldcg((const float4*)q + (8 * c + i) * 128 + r);
@@ -655,7 +670,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
           }
         }
         if (output) {
-          const float scale = l != 0.0f ? 1.0f / l : 0.0f;
+          // 2^(m - ml) / l, which may lie outside f32 where the outputs do not: then a part of it goes in ahead
+          float apart = m - ml;
+          if (__any_sync(0xffffffffu, apart < -90.0f)) {
+            scale_outputs(apart < -90.0f ? 0x1p-64f : 1.0f);
+            if (apart < -90.0f) apart += 64.0f;
+          }
+          const float half = exp2_(0.5f * apart), scale = l != 0.0f ? 1.0f / l * half * half : 0.0f;
           const int row = done.row0 + t * 128 + r, mine = row < done.s.rows ? number(done, row) : -1;
           uint16_t* out = a.o + (int64_t)max(mine, 0) * D;
 #pragma unroll 1
@@ -690,7 +711,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       more = walk.next(it);  // while the first scores are on their way
       const int row = done.row0 + t * 128 + r;
       const int limit = row < done.s.rows ? seen(a, done.s, row) : done.s.keys;  // rows past the last are not stored
-      m = l = 0.0f;
+      m = l = ml = 0.0f;
       for (int kt = done.t0; kt < done.t1; ++kt, ++n) {
         ok = mbar_wait(smem_u32(&x_full[n & 3]), (n >> 2) & 1, abort_flag, a.err, 421) &&
              mbar_wait(smem_u32(&s_full[t]), n & 1, abort_flag, a.err, 422);
@@ -702,7 +723,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         const float* kb = k_back + (n & 3) * 4;
         const float* vu = v_up + (n & 3) * 4;
         // the largest x, then the base
-        float top = -INFINITY;
+        float top = -INFINITY, least = INFINITY;  // least: the smallest ev
 #pragma unroll 1
         for (int h = 0; h < T::kKeys / 64; ++h) {  // two loads at a time on their way
           uint32_t s[64];
@@ -725,54 +746,83 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
             }
             high[0] = max3(high[0], __uint_as_float(y[30]), __uint_as_float(y[31]));
             top = fmaxf(top, fmaf(fmaxf(high[0], high[1]), score_factor(qs, kb[2 * h + c]), vu[2 * h + c]));
+            least = fminf(least, vu[2 * h + c]);
           }
         }
         const float base = first ? (top == -INFINITY ? 0.0f : top) : top > m + kLazyRows ? top : m;
-        if (!first && __any_sync(0xffffffffu, base != m)) {
-          // S_t was issued behind the last O_t += P_t V: it is complete
-          const float f = exp2_(m - base);
-          l *= f;
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tld32(tO + 32 * c, o);
-            tld_wait_regs(o);
+        if (first) {  // not above the largest score
+          float largest = vu[0];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tst32(tO + 32 * c, o);
-          }
+          for (int i = 1; i < T::kQuarters; ++i) largest = fmaxf(largest, vu[i]);
+          ml = base - largest;
+        }
+        // Where V is far smaller than what set the base, or scores have risen far above l's, P has lost bits that l needs
+        // (or l would pass f32's range): the two part.
+        bool far = base - least - ml > kFarBack;
+        if (__any_sync(0xffffffffu, far || (!first && base != m))) {
+          // S_t was issued behind the last O_t += P_t V: it is complete
+          if (!first) scale_outputs(exp2_(m - base));
+          far = __any_sync(0xffffffffu, far);
         }
         m = base;
+        if (far) {
 #pragma unroll 1
-        for (int h = 0; h < T::kKeys / 64; ++h) {  // P goes over columns whose scores have been read: 16 c .. 16 c + 15
-          uint32_t s[64];
-          tld32(tS + 64 * h, s);
-          tld32(tS + 64 * h + 32, s + 32);
-          tld_wait_regs(s);
-          tld_wait_regs(s + 32);
-          if (cut) {
-            hide(s, left - 64 * h);
-            hide(s + 32, left - 64 * h - 32);
-          }
+          for (int c = 0; c < T::kQuarters; ++c) {
+            uint32_t s[32], p[16];
+            tld32(tS + 32 * c, s);
+            tld_wait_regs(s);
+            if (cut) hide(s, left - 32 * c);
+            const float v_e = vu[c], f = score_factor(qs, kb[c]);
+            float most = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float v_e = vu[2 * h + c], f = score_factor(qs, kb[2 * h + c]), up = v_e - m;
-            const uint64_t f2 = pack_f32x2(f, f), up2 = pack_f32x2(up, up);
-            uint64_t part[2] = {0, 0};
-            uint32_t p[16];
+            for (int i = 0; i < 32; ++i) {
+              s[i] = __float_as_uint(__uint_as_float(s[i]) * f);
+              most = fmaxf(most, __uint_as_float(s[i]));
+            }
+            if (most > ml + kLazySum) {
+              l *= exp2_(ml - most);
+              ml = most;
+            }
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              float x0, x1;
-              unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[32 * c + i]), __uint_as_float(s[32 * c + i + 1])), f2, up2), x0, x1);
-              const float p0 = exp2_(x0), p1 = exp2_(x1);
-              part[(i >> 1) & 1] = add_f32x2(part[(i >> 1) & 1], pack_f32x2(p0, p1));
-              p[i >> 1] = f16x2(p0, p1);
+              const float x0 = __uint_as_float(s[i]), x1 = __uint_as_float(s[i + 1]);
+              l += exp2_(x0 - ml) + exp2_(x1 - ml);
+              p[i >> 1] = f16x2(exp2_(x0 + v_e - m), exp2_(x1 + v_e - m));
             }
-            tst16(tS + 32 * h + 16 * c, p);
-            float s0, s1, s2, s3;
-            unpack_f32x2(part[0], s0, s1);
-            unpack_f32x2(part[1], s2, s3);
-            l = fmaf((s0 + s1) + (s2 + s3), exp2_(-v_e), l);
+            tst16(tS + 16 * c, p);
+          }
+        } else {
+#pragma unroll 1
+          for (int h = 0; h < T::kKeys / 64; ++h) {  // P goes over columns whose scores have been read: 16 c .. 16 c + 15
+            uint32_t s[64];
+            tld32(tS + 64 * h, s);
+            tld32(tS + 64 * h + 32, s + 32);
+            tld_wait_regs(s);
+            tld_wait_regs(s + 32);
+            if (cut) {
+              hide(s, left - 64 * h);
+              hide(s + 32, left - 64 * h - 32);
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float v_e = vu[2 * h + c], f = score_factor(qs, kb[2 * h + c]), up = v_e - m;
+              const uint64_t f2 = pack_f32x2(f, f), up2 = pack_f32x2(up, up);
+              uint64_t part[2] = {0, 0};
+              uint32_t p[16];
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float x0, x1;
+                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[32 * c + i]), __uint_as_float(s[32 * c + i + 1])), f2, up2), x0, x1);
+                const float p0 = exp2_(x0), p1 = exp2_(x1);
+                part[(i >> 1) & 1] = add_f32x2(part[(i >> 1) & 1], pack_f32x2(p0, p1));
+                p[i >> 1] = f16x2(p0, p1);
+              }
+              tst16(tS + 32 * h + 16 * c, p);
+              float s0, s1, s2, s3;
+              unpack_f32x2(part[0], s0, s1);
+              unpack_f32x2(part[1], s2, s3);
+              l = fmaf((s0 + s1) + (s2 + s3), exp2_(m - v_e - ml), l);
+            }
           }
         }
         tst_wait();

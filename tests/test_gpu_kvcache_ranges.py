@@ -104,7 +104,7 @@ def test_zero_scores_of_small_keys(b200, D, power, size, scale, T, wide):
 # ---- values far smaller or larger than 1, and of both kinds in one sequence ----
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("power", [-115, -100, 97])
-@pytest.mark.parametrize("T,wide", FEW)
+@pytest.mark.parametrize("T,wide", KINDS)
 def test_many_equal_scores_over_values_of_any_size(b200, D, power, T, wide):
     """The sum of the probabilities stays in range however the values are scaled."""
     rng = np.random.default_rng(2)
