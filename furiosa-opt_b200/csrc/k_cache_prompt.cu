@@ -20,9 +20,12 @@
 // the sums of q in two f16 parts.
 //
 // f16 holds 11 bits of a value where bf16 would hold 8, but not every size of it: every 32
-// tokens' K is scaled by a power of two and V by another, so that the largest is in [2^4, 2^9). K's comes back with the
-// scores. V's, 2^ev, goes into the exponent: with x = score + ev, P = 2^(x - m) and O = sum P V 2^-ev, where the base m
-// follows the largest x. The sum of probabilities has a base of its own, a score n near the largest: l = sum P
+// tokens' K is scaled by a power of two and V by another, so that the largest is in [2^4, 2^9); where tokens are more
+// than 2^6 apart, each by its own, so that a large one, hidden or of no weight, takes nothing from its neighbours. K's
+// comes back with the scores. V's, 2^ev, goes into the exponent: with x = score + ev, P = 2^(x - m) and O = sum P V 2^-ev,
+// where the base m follows the largest x, which P brings to 2^10 at least: f16 holds 24 bits below that, so tokens of
+// little weight count, a hundred thousand of them too. What one scale has to hold are the groups of 32 channels of one
+// token: 2^-18 of the largest and less loses bits. The sum of probabilities has a base of its own, a score n near the largest: l = sum P
 // 2^(m - ev - n), so that V's size takes nothing from its range; outputs are O / l 2^(m - n).
 //
 // A 16-byte chunk holds 8 codes in the order that pairs come out of a word (0, 4, 1, 5, 2, 6, 3, 7): for K the
@@ -51,7 +54,10 @@ constexpr int kLeast = 4;                // units of a share
 // keys of one head of 8 query heads: 159 us; 347 without this rule, in shares of 7 units.
 constexpr float kByRoot = 1.0f;
 constexpr int kUncut = 8;                // segments of fewer tiles are not shared between blocks
-constexpr float kLazyRows = 14.0f;        // log2 by which x may exceed its base: P stays within f16, the base moves rarely
+// log2 of the largest P as the base is set, and up to which it may grow before the base moves. (On the cases above
+// 10 to 15 take no longer than 0 to 14.)
+constexpr float kNominal = 10.0f, kMostP = 15.0f;
+constexpr int kEven = 6;                  // log2 by which 32 tokens' sizes may differ under one scale
 constexpr float kLazySum = 20.0f;         // ... and a score that of l, where it is looked at
 constexpr float kFarBack = 80.0f;         // log2 up to which P gives its share of l: probabilities below 2^-46 may vanish
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -74,7 +80,8 @@ struct Tiles {
   // Q, 2 stages of K and of V, the offset steps of Q and K, alignment, barriers and scales; more than half an
   // SM's, since a second block would only wait for tensor memory
   static constexpr int kRaw = 32 * NG * 16;  // what a warp holds of 32 tokens' K or V
-  static constexpr int kAll = kQueries * (kQ + kOffsets) + 4 * kTile + 2 * kKeyOffsets + kExpand * kRaw + 1024 + 512;
+  static constexpr int kExponents = 4 * kKeys;  // of K, and of V: a byte for each token of four key tiles
+  static constexpr int kAll = kQueries * (kQ + kOffsets) + 4 * kTile + 2 * kKeyOffsets + kExpand * kRaw + 1024 + 512 + 2 * kExponents;
   static constexpr int kBytes = kAll > 120000 ? kAll : 120000;
   static constexpr int kSlot = kRows * (D + 3);      // floats of a partial result
 
@@ -253,14 +260,77 @@ __device__ __forceinline__ bool row_at(const AttnArgs& a, const Item& it, const 
 
 constexpr int kLowest = -120;  // of the exponents
 
-// The exponent that brings the largest of a warp's values to [2^4, 2^9), from the sizes of their groups; `none` for zeros.
+// The exponents that bring the largest values of a warp's tokens to [2^4, 2^9), from the sizes of their groups: the
+// largest of them for all, or, where they lie further apart than kEven, each its own. Zeros do not count: `none` if
+// there is nothing else.
+struct Exponents {
+  int all, own;
+  bool apart;
+};
 template <int NG>
-__device__ __forceinline__ int warp_exponent(const uint32_t* scales, int none) {
+__device__ __forceinline__ Exponents exponents(const uint32_t* scales, int none) {
   float top = 0.0f;
 #pragma unroll
   for (int j = 0; j < NG; ++j) top = fmaxf(top, fmaf(8.0f, step_of(scales[j]), fabsf(offset_of(scales[j]))));
-  const uint32_t all = __reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu);
-  return all ? min(max((int)(all >> 23) - 127 - 4, kLowest), 120) : none;
+  const int size = (int)((__float_as_uint(top) & 0x7fffffffu) >> 23);
+  const int most = __reduce_max_sync(0xffffffffu, size), least = __reduce_min_sync(0xffffffffu, size ? size : 255);
+  auto exponent = [](int bits) { return min(max(bits - 127 - 4, kLowest), 120); };
+  Exponents e{most ? exponent(most) : none, 0, most - least > kEven};
+  e.own = e.apart ? exponent(size ? size : least) : e.all;
+  return e;
+}
+
+
+// A tile's scores are the products times the row's factor and the keys' power of two: together not 0, for a hidden key's
+// -inf is multiplied as well.
+__device__ __forceinline__ float score_factor(float row, float keys) { return fmaxf(row * keys, 0x1p-126f); }
+
+// The softmax of tiles whose tokens have exponents of their own, 32 at a time: the scores in s and the ev in v. By themselves,
+// so that the roles' code beside them stays as it is (within rows_kernel they cost 15 us of 142, called for or not).
+__device__ __forceinline__ void own_scores(uint32_t columns, int left, float qs, const int8_t* k, const int8_t* v_own, float* s, float* v) {
+  tld32(columns, (uint32_t*)s);
+  tld_wait_regs((uint32_t*)s);
+  hide((uint32_t*)s, left);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    s[i] *= score_factor(qs, power(k[i]));
+    v[i] = (float)v_own[i];
+  }
+}
+// The largest x.
+__device__ __noinline__ float own_top(uint32_t columns, int left, float qs, const int8_t* k, const int8_t* v_own, int quarters) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < quarters; ++c) {
+    float s[32], v[32];
+    own_scores(columns + 32 * c, left - 32 * c, qs, k + 32 * c, v_own + 32 * c, s, v);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i] + v[i]);
+  }
+  return top;
+}
+// P in place of the scores, and (l, ml) with the tile's share: the base of l moves where scores rise far above it.
+__device__ __noinline__ float2 own_weights(uint32_t columns, int left, float qs, const int8_t* k, const int8_t* v_own, int quarters, float m, float l, float ml) {
+#pragma unroll 1
+  for (int c = 0; c < quarters; ++c) {
+    float s[32], v[32];
+    uint32_t p[16];
+    own_scores(columns + 32 * c, left - 32 * c, qs, k + 32 * c, v_own + 32 * c, s, v);
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) most = fmaxf(most, s[i]);
+    if (most > ml + kLazySum) {
+      l *= exp2_(ml - most);
+      ml = most;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      l += exp2_(s[i] - ml) + exp2_(s[i + 1] - ml);
+      p[i >> 1] = f16x2(exp2_(s[i] + v[i] - m), exp2_(s[i + 1] + v[i + 1] - m));
+    }
+    tst16(columns + 16 * c, p);
+  }
+  return make_float2(l, ml);
 }
 
 template <int NG>
@@ -291,6 +361,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
   uint32_t* tmem_slot = (uint32_t*)(v_up + 16);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   int* last = (int*)(tmem_slot + 2);    // [2]
+  uint64_t* apart = (uint64_t*)(last + 2);  // [4] a byte for K and V of each 32 tokens: do they have exponents of their own?
+  int8_t* k_own = (int8_t*)bars + 512;      // [4][kKeys] the tokens' exponents
+  int8_t* v_own = k_own + T::kExponents;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Start start = share_start<kRowThreads>(
@@ -318,7 +391,10 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       mbar_init(smem_u32(&o_done[i]), 1);
       mbar_init(smem_u32(&met[i]), 128);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&x_full[i]), 2 * T::kQuarters);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(&x_full[i]), 2 * T::kQuarters);
+      apart[i] = 0;
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -426,8 +502,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       const uint32_t empty = smem_u32(is_v ? &v_empty[stage] : &k_empty[stage]), parity = ((n >> 1) & 1) ^ 1;
       const uint32_t known = smem_u32(&x_full[n & 3]);
       // zeros of V do not lift the base of P; what is past the keys has no part in it
-      const int e = warp_exponent<NG>(scales, is_v && t * T::kKeys + quarter * 32 < it.s.keys ? kLowest : 0);
-      const float f = power(-e);
+      const Exponents e = exponents<NG>(scales, is_v && t * T::kKeys + quarter * 32 < it.s.keys ? kLowest : 0);
+      const float f = power(-e.own);
       // by code word of a piece (of two, where K's group of words is two pieces): steps and offsets of what its pairs of
       // codes are (see the loop)
       constexpr int kWords = NG == 8 ? 8 : 4;
@@ -454,9 +530,13 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       ok = mbar_wait(empty, parity, abort_flag, a.err, 411);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      if (lane == 0) {  // place n % 4: the softmax of tile n - 4 is over, or the product of n - 2 could not be
-        if (is_v) v_up[at4] = (float)e;
-        else k_back[at4] = power(e);
+      // place n % 4: the softmax of tile n - 4 is over, or the product of n - 2 could not be
+      (is_v ? v_own : k_own)[(at4 & ~3) * (T::kKeys / 4) + row] = (int8_t)e.own;
+      __syncwarp();
+      if (lane == 0) {
+        if (is_v) v_up[at4] = (float)e.all;
+        else k_back[at4] = power(e.all);
+        ((uint8_t*)(apart + (at4 >> 2)))[(is_v ? 4 : 0) + quarter] = e.apart;
         mbar_arrive(known);
       }
       if (!is_v) {
@@ -565,9 +645,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       return scalbnf(fabsf(a.scale) * kLog2e, e - 8);
     };
 
-    // A tile's scores are the products times the row's factor and the keys' power of two: together not 0, for a hidden
-    // key's -inf is multiplied as well.
-    auto score_factor = [](float row, float keys) { return fmaxf(row * keys, 0x1p-126f); };
     uint32_t meetings = 0;
     auto meet = [&]() -> bool {  // a barrier of the tile's softmax threads whose wait is bounded
       mbar_arrive(smem_u32(&met[t]));
@@ -671,12 +748,12 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         }
         if (output) {
           // 2^(m - ml) / l, which may lie outside f32 where the outputs do not: then a part of it goes in ahead
-          float apart = m - ml;
-          if (__any_sync(0xffffffffu, apart < -90.0f)) {
-            scale_outputs(apart < -90.0f ? 0x1p-64f : 1.0f);
-            if (apart < -90.0f) apart += 64.0f;
+          float lift = m - ml;
+          if (__any_sync(0xffffffffu, lift < -90.0f)) {
+            scale_outputs(lift < -90.0f ? 0x1p-64f : 1.0f);
+            if (lift < -90.0f) lift += 64.0f;
           }
-          const float half = exp2_(0.5f * apart), scale = l != 0.0f ? 1.0f / l * half * half : 0.0f;
+          const float half = exp2_(0.5f * lift), scale = l != 0.0f ? 1.0f / l * half * half : 0.0f;
           const int row = done.row0 + t * 128 + r, mine = row < done.s.rows ? number(done, row) : -1;
           uint16_t* out = a.o + (int64_t)max(mine, 0) * D;
 #pragma unroll 1
@@ -724,8 +801,11 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         const float* vu = v_up + (n & 3) * 4;
         // the largest x, then the base
         float top = -INFINITY, least = INFINITY;  // least: the smallest ev
+        const int8_t *ko = k_own + (n & 3) * T::kKeys, *vo = v_own + (n & 3) * T::kKeys;
+        const bool uneven = apart[n & 3] != 0;
+        if (uneven) top = own_top(tS, left, qs, ko, vo, T::kQuarters);
 #pragma unroll 1
-        for (int h = 0; h < T::kKeys / 64; ++h) {  // two loads at a time on their way
+        for (int h = 0; !uneven && h < T::kKeys / 64; ++h) {  // two loads at a time on their way
           uint32_t s[64];
           tld32(tS + 64 * h, s);
           tld32(tS + 64 * h + 32, s + 32);
@@ -749,7 +829,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
             least = fminf(least, vu[2 * h + c]);
           }
         }
-        const float base = first ? (top == -INFINITY ? 0.0f : top) : top > m + kLazyRows ? top : m;
+        const float base = first ? (top == -INFINITY ? 0.0f : top - kNominal) : top > m + kMostP ? top - kNominal : m;
         if (first) {  // not above the largest score
           float largest = vu[0];
 #pragma unroll
@@ -758,7 +838,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         }
         // Where V is far smaller than what set the base, or scores have risen far above l's, P has lost bits that l needs
         // (or l would pass f32's range): the two part.
-        bool far = base - least - ml > kFarBack;
+        bool far = uneven || base - least - ml > kFarBack;
         if (__any_sync(0xffffffffu, far || (!first && base != m))) {
           // S_t was issued behind the last O_t += P_t V: it is complete
           if (!first) scale_outputs(exp2_(m - base));
@@ -766,31 +846,9 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         }
         m = base;
         if (far) {
-#pragma unroll 1
-          for (int c = 0; c < T::kQuarters; ++c) {
-            uint32_t s[32], p[16];
-            tld32(tS + 32 * c, s);
-            tld_wait_regs(s);
-            if (cut) hide(s, left - 32 * c);
-            const float v_e = vu[c], f = score_factor(qs, kb[c]);
-            float most = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              s[i] = __float_as_uint(__uint_as_float(s[i]) * f);
-              most = fmaxf(most, __uint_as_float(s[i]));
-            }
-            if (most > ml + kLazySum) {
-              l *= exp2_(ml - most);
-              ml = most;
-            }
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float x0 = __uint_as_float(s[i]), x1 = __uint_as_float(s[i + 1]);
-              l += exp2_(x0 - ml) + exp2_(x1 - ml);
-              p[i >> 1] = f16x2(exp2_(x0 + v_e - m), exp2_(x1 + v_e - m));
-            }
-            tst16(tS + 16 * c, p);
-          }
+          const float2 sum = own_weights(tS, left, qs, ko, vo, T::kQuarters, m, l, ml);
+          l = sum.x;
+          ml = sum.y;
         } else {
 #pragma unroll 1
           for (int h = 0; h < T::kKeys / 64; ++h) {  // P goes over columns whose scores have been read: 16 c .. 16 c + 15

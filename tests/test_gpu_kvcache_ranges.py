@@ -85,7 +85,6 @@ def _plain(rng, n, H, D):
 
 
 KINDS = [(1, False), (20, False), (40, True)]  # new tokens, and whether the prompts' kernel takes them
-FEW = KINDS[:2]
 
 
 # ---- hidden keys beside scores that are zero ----
@@ -123,7 +122,7 @@ def _aimed(rng, T, group, D):
 @pytest.mark.parametrize("low,high", [(-60, 90), (-100, 40), (-20, 20)])
 @pytest.mark.parametrize("weight", [True, False])  # whether the large values have any
 @pytest.mark.parametrize("large_first", [True, False])
-@pytest.mark.parametrize("T,wide", FEW)
+@pytest.mark.parametrize("T,wide", KINDS)
 def test_small_values_beside_large_ones(b200, D, low, high, weight, large_first, T, wide):
     """Runs of tiny values and of huge ones, which different warps and blocks meet: where the huge ones have no
     weight, the output is of the tiny ones."""
@@ -141,7 +140,7 @@ def test_small_values_beside_large_ones(b200, D, low, high, weight, large_first,
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("power", [10, 14, 18, 22, 40, 128])
 @pytest.mark.parametrize("at", [0, 137, 940])
-@pytest.mark.parametrize("T,wide", FEW)
+@pytest.mark.parametrize("T,wide", KINDS)
 def test_a_large_value_of_no_weight(b200, D, power, at, T, wide):
     """One key that no query wants, with a value 2^power times as large as the others (past 2^127: infinite)."""
     rng = np.random.default_rng(4)
@@ -155,7 +154,7 @@ def test_a_large_value_of_no_weight(b200, D, power, at, T, wide):
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("power", [16, 30, 60, 128])
 @pytest.mark.parametrize("which", ["k", "v", "kv"])
-@pytest.mark.parametrize("T,wide", [(20, False)])
+@pytest.mark.parametrize("T,wide", [(20, False), (40, True)])
 def test_a_large_key_and_value_that_most_rows_do_not_see(b200, D, power, which, T, wide):
     """A new token whose key, value or both are 2^power times the others' or infinite: the tokens before it do not
     see it, and their answers are what they are without it."""
@@ -175,7 +174,7 @@ def test_a_large_key_and_value_that_most_rows_do_not_see(b200, D, power, which, 
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("power", [12, 20, 60, 128])
 @pytest.mark.parametrize("at", [3, 137])
-@pytest.mark.parametrize("T,wide", FEW)
+@pytest.mark.parametrize("T,wide", KINDS)
 def test_a_large_key_of_no_weight(b200, D, power, at, T, wide):
     """A key 2^power times as long as the others that every query turns away from."""
     rng = np.random.default_rng(6)
@@ -186,14 +185,11 @@ def test_a_large_key_of_no_weight(b200, D, power, at, T, wide):
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
-@pytest.mark.parametrize("power", [8, 16, 40, 128])
-@pytest.mark.parametrize("T,wide", FEW)
-def test_a_large_channel_leaves_other_groups_alone(b200, D, power, T, wide):
+@pytest.mark.parametrize("T,wide,power", [(T, False, p) for T in (1, 20) for p in (8, 16, 40, 128)] + [(40, True, 8), (40, True, 16)])
+def test_a_large_channel_leaves_other_groups_alone(b200, D, T, wide, power):
     """A key like any other, one of whose channels has a value 2^power times the rest: what its group's other channels
     can say goes, other groups' outputs stay. The prompts' kernel follows a token's largest group, and the others as
     long as they are no less than 2^-18 of it."""
-    if wide and power > 16:
-        pytest.skip("past what the prompts' kernel holds")
     rng = np.random.default_rng(7)
     k, v = _plain(rng, 400, 1, D)
     with np.errstate(over="ignore"):
@@ -205,7 +201,7 @@ def test_a_large_channel_leaves_other_groups_alone(b200, D, power, T, wide):
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("bits", [14, 18, 22, 25])
 @pytest.mark.parametrize("sink", [1.0, 2.0 ** -6])  # the size of the heavy key's own value
-@pytest.mark.parametrize("T,wide", FEW)
+@pytest.mark.parametrize("T,wide", KINDS)
 def test_a_long_flat_tail_behind_one_heavy_key(b200, D, bits, sink, T, wide):
     """The first key has 2^bits times the weight of each of 20000 equal others."""
     rng = np.random.default_rng(8)
