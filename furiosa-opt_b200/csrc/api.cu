@@ -122,6 +122,8 @@ struct fopt_graph {
 
 namespace fopt {
 
+constexpr size_t kMostWorkspaces = 16;  // of streams, kept
+
 static void clear_if_stale(fopt_ctx* ctx, Workspace& ws) {
   if (ws.clear_at == ctx->expiries) return;
   cuda_check(cudaMemsetAsync(ws.p, 0, ws.bytes, ctx->stream), "cache workspace clear");
@@ -144,7 +146,7 @@ void* cache_workspace(fopt_ctx* ctx, size_t bytes) {
     cudaStreamDestroy(s);
     if (e != cudaSuccess) cudaFree(p);
     cuda_check(e, "cache workspace clear");
-    ws = {p, bytes, ctx->expiries};
+    ws = {p, bytes, ctx->expiries, ws.used};
   };
   if (fopt_graph* g = ctx->capture) {  // cleared before a launch, if it has to be
     if (g->cache_ws.empty() || bytes > g->cache_ws.back().bytes) {
@@ -154,10 +156,19 @@ void* cache_workspace(fopt_ctx* ctx, size_t bytes) {
     }
     return g->cache_ws.back().p;
   }
+  if (ctx->cache_ws.size() >= kMostWorkspaces && !ctx->cache_ws.count(ctx->stream)) {
+    auto oldest = ctx->cache_ws.begin();
+    for (auto it = oldest; it != ctx->cache_ws.end(); ++it)
+      if (it->second.used < oldest->second.used) oldest = it;
+    void* p = oldest->second.p;
+    ctx->cache_ws.erase(oldest);
+    cuda_check(cudaFree(p), "cache workspace free");  // waits for its last reader
+  }
   Workspace& ws = ctx->cache_ws[ctx->stream];
+  ws.used = ++ctx->cache_ws_uses;
   if (bytes > ws.bytes) {
     void* old = ws.p;
-    ws = {};
+    ws = {nullptr, 0, 0, ws.used};
     if (old) cuda_check(cudaFree(old), "cache workspace free");  // waits for its last reader
     zeroed(ws);
   }

@@ -72,6 +72,7 @@ struct Workspace {
   void* p = nullptr;
   size_t bytes = 0;
   uint64_t clear_at = 0;  // the context's expiries when it was last cleared
+  uint64_t used = 0;      // the context's count of uses at the last one
 };
 }  // namespace fopt
 
@@ -104,7 +105,10 @@ struct fopt_ctx {
   size_t gemm_cnt_n = 0;
   bool gemm_cnt_dirty = false;
   uint64_t expiries = 0;  // expired waits so far: a workspace that was last clear before one is cleared before its next use
-  std::map<cudaStream_t, fopt::Workspace> cache_ws;  // cache-attention workspace of each stream
+  // Cache-attention workspaces of the streams that used one last. A stream may be destroyed without the context being
+  // told, so their number is bounded.
+  std::map<cudaStream_t, fopt::Workspace> cache_ws;
+  uint64_t cache_ws_uses = 0;
   cudaStream_t copy_in = nullptr, copy_out = nullptr;  // host <-> device pipelines of the host-buffer calls
   void* pinned[2] = {nullptr, nullptr};  // host staging for file -> device streaming
   cudaEvent_t pinned_ev[2] = {nullptr, nullptr};

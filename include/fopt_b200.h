@@ -427,7 +427,9 @@ fopt_status fopt_cache_read(fopt_ctx* ctx, void* out_k, void* out_v, fopt_dtype 
  * is not ascending within 0 .. tokens (clamped) is reported as FOPT_ERR_INVALID by the next fopt_sync /
  * fopt_d2h. All lengths are device data, so a captured call replays over growing sequences. Calls on one
  * stream take turns with a workspace that the context keeps for the stream (drain a stream of your own
- * before you destroy it); a captured graph has one of its own. Results do not depend on timing. */
+ * before you destroy it), for the 16 streams that called last; a captured graph has one of its own until it is destroyed. A
+ * workspace takes up to 45 MB on a device of 148 SMs (up to 5 MB where all calls have at most 32 query rows to a key head).
+ * Results do not depend on timing. */
 fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* q, const fopt_paged_cache* cache,
                                  const int32_t* table, const int32_t* q_start, const int32_t* kv_len, int32_t batch,
                                  int32_t tokens, int32_t table_width, int32_t hq, float scale, int32_t causal);

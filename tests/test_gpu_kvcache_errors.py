@@ -1,4 +1,4 @@
-"""What a device-side error leaves behind. The expired wait is made on the host: its code is written where a kernel would
+"""What a device-side error leaves behind, and what streams do. The expired wait is made on the host: its code is written where a kernel would
 write it, and arrivals are left in a workspace as a kernel that gave up would leave them; no wait runs out."""
 import ctypes as C
 import os
@@ -9,7 +9,7 @@ import pytest
 
 import furiosa_opt_b200 as fb
 from furiosa_opt_b200 import _lib
-from test_gpu_kvcache import Case, _down, _up
+from test_gpu_kvcache import WIDE, Case, _down, _up
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,24 @@ def test_an_expired_wait_leaves_no_arrivals(inside):
         assert np.array_equal(_down(graph.launch(), c.q.shape), want)
         be.set_stream(None)
     graph.close()
+
+
+def test_many_streams_hold_few_workspaces():
+    """A program that takes another stream for each request: what the context keeps for them is bounded."""
+    import torch
+    be = fb.B200(0)
+    c = Case(be, [70, 1], [800, 3000], 2, 4, 128, 64, seed=53, wide=WIDE)
+    want = c.check()
+    streams = [torch.cuda.Stream() for _ in range(28)]
+    assert len({s.cuda_stream for s in streams}) == 28
+    out = fb.Storage(be, "bf16", c.q.size)
+    be.sync()
+    before = torch.cuda.mem_get_info()[0]
+    for s in streams + streams[:3]:
+        be.set_stream(s.cuda_stream)
+        c.run(out=out)
+        be.sync()
+    be.set_stream(None)
+    held = before - torch.cuda.mem_get_info()[0]
+    assert np.array_equal(_down(out, want.shape), want)
+    assert held <= 16 * 48 * 2 ** 20, held
