@@ -415,21 +415,25 @@ fopt_status fopt_cache_append(fopt_ctx* ctx, const fopt_paged_cache* cache, cons
  * rows of negative slots are left as they were. */
 fopt_status fopt_cache_read(fopt_ctx* ctx, void* out_k, void* out_v, fopt_dtype dtype, const fopt_paged_cache* cache,
                             const int32_t* slots, int32_t n);
-/* softmax(scale q K^T) V over the cache for `batch` sequences of any lengths in one call. Sequence b has
- * the query tokens q_start[b] .. q_start[b + 1] - 1 of q [tokens, hq, D] (bf16; q_start has batch + 1
- * entries) and the kv_len[b] keys whose key i lies in page table[b * table_width + i / page_size], slot i %
- * page_size. Causal: the queries are the sequence's last tokens, so query j of n sees keys 0 ..
- * kv_len[b] - n + j; otherwise every query sees all kv_len[b]. Query head h reads key head h / (hq / H).
- * o [tokens, hq, D] bf16 (32-byte aligned, q 16): a row that sees no key is 0; rows of tokens past q_start[batch] are left
- * as they were. Scores, maxima, sums and the output accumulate in f32. Reads nothing but the keys in
- * range: table entries and cache slots past kv_len may hold anything. A page number outside the cache
- * (its keys count as zeros), a length past table_width pages or past 2^31 - 131072 (cut) or a q_start that
- * is not ascending within 0 .. tokens (clamped) is reported as FOPT_ERR_INVALID by the next fopt_sync /
- * fopt_d2h. All lengths are device data, so a captured call replays over growing sequences. Calls on one
- * stream take turns with a workspace that the context keeps for the stream (drain a stream of your own
- * before you destroy it), for the 16 streams that called last; a captured graph has one of its own until it is destroyed. A
- * workspace takes up to 45 MB on a device of 148 SMs (up to 5 MB where all calls have at most 32 query rows to a key head).
- * Results do not depend on timing. */
+/* softmax(scale q K^T) V over the cache for `batch` sequences of any lengths in one call. Sequence b has the
+ * query tokens q_start[b] .. q_start[b + 1] - 1 of q [tokens, hq, D] (bf16; q_start has batch + 1 entries) and
+ * the kv_len[b] keys whose key i lies in page table[b * table_width + i / page_size], slot i % page_size.
+ * Causal: the queries are the sequence's last tokens, so query j of n sees keys 0 .. kv_len[b] - n + j;
+ * otherwise every query sees all kv_len[b]. Query head h reads key head h / (hq / H). o [tokens, hq, D] bf16
+ * (32-byte aligned, q 16): a row that sees no key is 0; rows of tokens past q_start[batch] are left as they
+ * were. Scores, maxima, sums and the output accumulate in f32. Reads nothing but the keys in range: table
+ * entries and cache slots past kv_len may hold anything. A page number outside the cache (its keys count as
+ * zeros), a length past table_width pages or past 2^31 - 131072 (cut) or a q_start that is not ascending within
+ * 0 .. tokens (clamped; a row that two sequences then name may hold anything) is reported as FOPT_ERR_INVALID by
+ * the next fopt_sync / fopt_d2h. Keys and values may be of any size beside each other: one that is large,
+ * infinite (stored as 2^100) or hidden changes no answer in which it has no part. Sequences of more than 32
+ * query rows to a key head follow each token's largest group of 32 channels, in f16: where one group's values,
+ * of a token that has weight, are 2^18 or more times another group's, the other group's outputs lose bits, and
+ * vanish from 2^30 on. All lengths are device data, so a captured call replays over growing sequences. Calls on
+ * one stream take turns with a workspace that the context keeps for the stream (drain a stream of your own
+ * before you destroy it), for the 16 streams that called last; a captured graph has one of its own until it is
+ * destroyed. A workspace takes up to 45 MB on a device of 148 SMs (up to 5 MB where all calls have at most 32
+ * query rows to a key head). Results do not depend on timing. */
 fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* q, const fopt_paged_cache* cache,
                                  const int32_t* table, const int32_t* q_start, const int32_t* kv_len, int32_t batch,
                                  int32_t tokens, int32_t table_width, int32_t hq, float scale, int32_t causal);

@@ -1,4 +1,4 @@
-"""What a device-side error leaves behind, and what streams do. The expired wait is made on the host: its code is written where a kernel would
+"""What a device-side error leaves behind, what streams hold, and calls of nothing. The expired wait is made on the host: its code is written where a kernel would
 write it, and arrivals are left in a workspace as a kernel that gave up would leave them; no wait runs out."""
 import ctypes as C
 import os
@@ -104,3 +104,45 @@ def test_many_streams_hold_few_workspaces():
     held = before - torch.cuda.mem_get_info()[0]
     assert np.array_equal(_down(out, want.shape), want)
     assert held <= 16 * 48 * 2 ** 20, held
+
+
+def test_empty_calls():
+    """No tokens, no slots, no queries: nothing is read, written or reported."""
+    be = fb.B200(0)
+    c = Case(be, [1, 1], [40, 20], 2, 4, 128, 16, seed=54)
+    want = c.check()
+    images = [s.to_bytes() for s in (c.cache.k, c.cache.v, c.cache.k_scale, c.cache.v_scale)]
+    none, zero = fb.Storage(be, "bf16", 0), fb.Storage(be, "i32", 0)
+    rope = fb.Rope([1.0] * 64)
+    assert be.rotary(none, zero, rope, 2).n == 0
+    be.cache_append(c.cache, none, none, zero, positions=zero, rope=rope)
+    assert [s.n for s in be.cache_read(c.cache, zero)] == [0, 0]
+    d = c.dev
+    assert be.cache_attention(none, c.cache, d["table"], _up(be, [0, 0, 0], "i32"), d["kv_len"], 8).n == 0
+    be.sync()
+    assert images == [s.to_bytes() for s in (c.cache.k, c.cache.v, c.cache.k_scale, c.cache.v_scale)]
+    assert np.array_equal(_down(c.run(), c.q.shape), want)
+
+
+def test_a_bad_start_leaves_other_sequences_alone():
+    """A start past the tokens: the sequences before it are what they are without it."""
+    be = fb.B200(0)
+    c = Case(be, [1, 1, 1], [40, 20, 64], 1, 4, 128, 16, seed=55)
+    good = c.check()
+    c.dev["q_start"] = _up(be, [0, 1, 5, 3], "i32")
+    got = c.run()
+    with pytest.raises(fb._lib.FoptError, match="query starts"):
+        be.sync()
+    assert np.array_equal(_down(got, c.q.shape)[0], good[0])
+
+
+def test_forward_is_what_it_was_before_the_cached_step():
+    """`DecoderBlockW8A8.forward` gives the bits that it gave before `step` came beside it."""
+    import hashlib
+    be = fb.B200(0)
+    for shape, digest in (((128, 256, 2, 1, 512, 1, 128), "811494477c50f9293115cca434eb574a80e8ff96f18e7c81c6e09cd9479271c2"),
+                          ((256, 512, 4, 2, 1024, 2, 128), "85bfc8c21782b66ae849c6e88f167df57835970b4c65ba51655290a4ee749b90")):
+        blk = fb.workloads.DecoderBlockW8A8(be, *shape, seed=9)
+        x = fb.dtypes.f32_to_bf16_bits(np.random.default_rng(1).standard_normal(shape[0] * shape[1]).astype(np.float32))
+        y = blk.forward(be.from_vec(blk.m("[T, H]"), x, "bf16")).to_bytes()
+        assert hashlib.sha256(bytes(y)).hexdigest() == digest
