@@ -158,14 +158,12 @@ __device__ __forceinline__ int v_chunk(int token, int chunk) {
 template <int NG, int NB>
 struct State {
   // [channel 32 j + 4 g + 2 mm (+ 1 for c2, c3)] x [row 2 i, 2 i + 1]: sum of p step (code + 8). From the MMAs, in
-  // 2^24 for the even channels (c0, c1) and 2^20 for the odd ones
+  // 2^ev and 2^24 for the even channels (c0, c1), 2^20 for the odd ones
   float o[NB][NG][2][4];
   float e[NB][NG][2];      // sum of p (offset - 8 step), this lane's tokens
-  // p = 2^(score - m). The base m is that of p 2^-ev, so that p step fits f16's upper end at any magnitude of V: it is
-  // the score's maximum (lagging by up to kLazy) plus ev
-  float m[NB][2], l[NB][2];
-  float ev;
-  float vlimit;            // the largest step that p step still holds; infinite: products in f32, or to be done so
+  float m[NB][2], l[NB][2];  // p = 2^(score - m), m the score's maximum (lagging by up to kLazy); sum of p
+  int ev;                  // p step goes into the MMAs as 2^-ev of it, to fit f16's upper end at any magnitude of V
+  float vlimit;            // the largest step that p step still holds; infinite: products in f32
   uint32_t stepped;        // groups of which a token of the lane's had a step, a bit each
   __device__ __forceinline__ void clear(bool wide) {
 #pragma unroll
@@ -180,7 +178,7 @@ struct State {
       }
     }
     stepped = 0;
-    ev = 0.0f;
+    ev = 0;
     vlimit = wide ? INFINITY : 0.0f;
   }
 };
@@ -349,16 +347,17 @@ __device__ __forceinline__ void scores(const uint8_t* stage, const Places& at, c
 // The tile's softmax and its share of the output; token0 is its first. wide: the products in f32.
 template <int NG, int NB>
 __device__ __forceinline__ void values(const uint8_t* stage, const Places& at, int token0, int keys, int sure, bool first, bool wide,
-                                       const Query<NG, NB>& q, State<NG, NB>& s, float (*x)[4]) {
+                                       const Query<NG, NB>& q, State<NG, NB>& s, const float (*raw)[4]) {
   using S = Shared<NG, NB>;
   const int lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
   uint32_t vm[2][NG];
 #pragma unroll
   for (int h = 0; h < 2; ++h) load_words<NG>(vm[h], stage + 2 * S::kCodes + S::kScales + at.scale + 8 * h * NG * 4);
+  float x[NB][4];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) x[nb][c] = fmaf(x[nb][c], q.scale[nb][c & 1], -s.m[nb][c & 1]);
+    for (int c = 0; c < 4; ++c) x[nb][c] = fmaf(raw[nb][c], q.scale[nb][c & 1], -s.m[nb][c & 1]);
   if (token0 + 16 > sure) {  // some row does not see all of it
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -388,38 +387,38 @@ __device__ __forceinline__ void values(const uint8_t* stage, const Places& at, i
   }
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) tops = max3(max3(tops, x[nb][0], x[nb][1]), x[nb][2], x[nb][3]);
-  if (__any_sync(0xffffffffu, first || tops > kLazy - s.ev || steps > s.vlimit)) {
-    float lift = 0.0f;  // of ev, for p <= 2^kLazy
+  if (__any_sync(0xffffffffu, first || tops > kLazy || steps > s.vlimit)) {
+    float fall = 1.0f;  // of o, when the steps' power of two moves
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) steps = fmaxf(steps, __shfl_xor_sync(0xffffffffu, steps, o));
     if (steps > s.vlimit) {
-      const float ev = (float)max(ilogbf(steps) - kStepTop, -100);  // further down p 2^-ev would pass the f32 range
-      lift = first ? 0.0f : ev - s.ev;
+      const int ev = max(ilogbf(steps) - kStepTop, -120);
+      if (s.vlimit > 0.0f) fall = s.ev - ev < -126 ? 0.0f : power(s.ev - ev);  // before the first step there is no o
       s.ev = ev;
-      s.vlimit = fminf(exp2f(ev) * kStepRoom, 0x1.fep127f);
-      if (lift > 100.0f) s.vlimit = INFINITY;  // what is scaled down past f32's range may have had weight
+      s.vlimit = fminf(power(ev) * kStepRoom, 0x1.fep127f);
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        // the base moves up by the largest score over it, and with ev; the first tile's scores set it
-        const float top_score = max_over_g(fmaxf(x[nb][c], x[nb][c + 2]));
-        float up;
-        if (first) up = top_score == -INFINITY ? 0.0f : top_score + s.ev;
-        else up = (top_score > kLazy - (s.ev - lift) ? top_score + (s.ev - lift) : 0.0f) + lift;
-        const float f = first ? 0.0f : exp2_(-up);
-        s.m[nb][c] += up;
-        x[nb][c] -= up;
-        x[nb][c + 2] -= up;
+        // The base moves to the largest score, if that lies far above it; the first tile's scores set it. From the scores
+        // themselves, rounded alike: relative to a base far away they have lost bits.
+        const float scale = q.scale[nb][c];
+        const float x0 = x[nb][c] == -INFINITY ? -INFINITY : raw[nb][c] * scale, x1 = x[nb][c + 2] == -INFINITY ? -INFINITY : raw[nb][c + 2] * scale;
+        const float top = max_over_g(fmaxf(x0, x1)), was = s.m[nb][c];
+        const float m = first ? (top == -INFINITY ? 0.0f : top) : top - was > kLazy ? top : was;
+        const float f = first ? 0.0f : exp2_(was - m), fo = f * fall;
+        s.m[nb][c] = m;
+        x[nb][c] = x0 - m;
+        x[nb][c + 2] = x1 - m;
         s.l[nb][c] *= f;
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
           s.e[nb][j][c] *= f;
 #pragma unroll
           for (int mm = 0; mm < 2; ++mm) {
-            s.o[nb][j][mm][c] *= f;
-            s.o[nb][j][mm][c + 2] *= f;
+            s.o[nb][j][mm][c] *= fo;
+            s.o[nb][j][mm][c + 2] *= fo;
           }
         }
       }
@@ -431,15 +430,15 @@ __device__ __forceinline__ void values(const uint8_t* stage, const Places& at, i
       x[nb][c] = exp2_(x[nb][c]);
       s.l[nb][c & 1] += x[nb][c];
     }
+#pragma unroll
+  for (int j = 0; j < NG; ++j) {
+    const float z0 = fmaf(-8.0f, step[0][j], offset_of(vm[0][j])), z1 = fmaf(-8.0f, step[1][j], offset_of(vm[1][j]));
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) s.e[nb][j][c] = fmaf(x[nb][c], z0, fmaf(x[nb][c + 2], z1, s.e[nb][j][c]));
+  }
   if (wide) {
-#pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      const float z0 = fmaf(-8.0f, step[0][j], offset_of(vm[0][j])), z1 = fmaf(-8.0f, step[1][j], offset_of(vm[1][j]));
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) s.e[nb][j][c] = fmaf(x[nb][c], z0, fmaf(x[nb][c + 2], z1, s.e[nb][j][c]));
-    }
     // token by token: its probabilities from the lane that has them, its codes of this lane's channels
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -475,21 +474,23 @@ __device__ __forceinline__ void values(const uint8_t* stage, const Places& at, i
 #pragma unroll
     for (int t = 0; t < 4; ++t)  // (2 i + 1) / 2 and (2 i + 8) / 2 mod 4 are i: the chunk is the same
       load_words<NG / 2>(vw[t], stage + S::kCodes + at.v + ((t & 1) + 8 * (t >> 1)) * (S::D / 2));
+    const float down = power(-s.ev);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[nb][c] *= down;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       const uint32_t sel = j & 1 ? 0x7632u : 0x5410u;
       const uint32_t x01 = __byte_perm(vw[0][j >> 1], vw[1][j >> 1], sel), x23 = __byte_perm(vw[2][j >> 1], vw[3][j >> 1], sel);
       const uint32_t y01 = x01 >> 8, y23 = x23 >> 8;
       const float s0 = step[0][j], s1 = step[1][j];
-      const float z0 = fmaf(-8.0f, s0, offset_of(vm[0][j])), z1 = fmaf(-8.0f, s1, offset_of(vm[1][j]));
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const uint32_t b0 = transposed(f16x2(x[nb][0] * s0, x[nb][1] * s0));
         const uint32_t b1 = transposed(f16x2(x[nb][2] * s1, x[nb][3] * s1));
         mma(s.o[nb][j][0], codes_low(at.masks, x01), codes_high(at.masks, x01), codes_low(at.masks, x23), codes_high(at.masks, x23), b0, b1);
         mma(s.o[nb][j][1], codes_low(at.masks, y01), codes_high(at.masks, y01), codes_low(at.masks, y23), codes_high(at.masks, y23), b0, b1);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) s.e[nb][j][c] = fmaf(x[nb][c], z0, fmaf(x[nb][c + 2], z1, s.e[nb][j][c]));
       }
     }
   }
@@ -504,18 +505,15 @@ __device__ __forceinline__ bool too_small(const State<NG, NB>& s, int n) {
     return fmaf(s.o[nb][j][0][c] + s.o[nb][j][1][c], 0x1p24f, (s.o[nb][j][0][c + 2] + s.o[nb][j][1][c + 2]) * 0x1p20f);
   };
   const float least = (float)n * (0x1p-14f * 8.0f * 32.0f);
-  bool low = false, lost = s.vlimit == INFINITY;
+  bool low = false;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int j = 0; j < NG; ++j)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        low |= lane_sum(nb, j, c) < least * 0.125f;
-        lost |= fabsf(s.e[nb][j][c]) == INFINITY;  // offsets of another size than any step
-      }
-  if (!__any_sync(0xffffffffu, low || lost)) return false;
-  low = lost;
+      for (int c = 0; c < 2; ++c) low |= lane_sum(nb, j, c) < least * 0.125f;
+  if (!__any_sync(0xffffffffu, low)) return false;
+  low = false;
   const uint32_t stepped = __reduce_or_sync(0xffffffffu, s.stepped);
 #pragma unroll
   for (int j = 0; j < NG; ++j) {
@@ -531,28 +529,27 @@ __device__ __forceinline__ bool too_small(const State<NG, NB>& s, int n) {
   return __any_sync(0xffffffffu, low);
 }
 
-// The warp's part of the output, its rows' maxima and sums. What leaves has the score's base, which is comparable with
-// other warps'.
+// The warp's part of the output, its rows' maxima and sums.
 template <int NG, int NB, typename Rows>
-__device__ __forceinline__ void leave(const State<NG, NB>& st, float even, float odd, float* out, Rows& ml) {
+__device__ __forceinline__ void leave(const State<NG, NB>& st, bool wide, float* out, Rows& ml) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
-  const float back = power((int)st.ev);
+  const float even = wide ? 1.0f : 0x1p24f, odd = wide ? 1.0f : 0x1p20f, back = power(st.ev);
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int r = nb * 8 + 2 * i + c;
-      const float l = sum_over_g(st.l[nb][c]) * back;
+      const float l = sum_over_g(st.l[nb][c]);
       if (g == 0) {
-        ml[0][warp][r] = l > 0.0f ? st.m[nb][c] - st.ev : kNone;
+        ml[0][warp][r] = l > 0.0f ? st.m[nb][c] : kNone;
         ml[1][warp][r] = l;
       }
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         const float e = sum_over_g(st.e[nb][j][c]);
         *(float4*)(out + r * Shared<NG, NB>::kRow + j * kGroup + 4 * g) =
-            make_float4(fmaf(st.o[nb][j][0][c], even, e) * back, fmaf(st.o[nb][j][0][c + 2], odd, e) * back,
-                        fmaf(st.o[nb][j][1][c], even, e) * back, fmaf(st.o[nb][j][1][c + 2], odd, e) * back);
+            make_float4(fmaf(st.o[nb][j][0][c] * even, back, e), fmaf(st.o[nb][j][0][c + 2] * odd, back, e),
+                        fmaf(st.o[nb][j][1][c] * even, back, e), fmaf(st.o[nb][j][1][c + 2] * odd, back, e));
       }
     }
 }
@@ -726,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, tokens_blocks<NG, NB>()) tokens_kern
       copies_wait<0>();
       __syncwarp();  // the ring is drained: the warp's output goes over it
       if (!wide && !first && too_small<NG, NB>(st, (tiles16 / kWarps + 1) * 16)) continue;
-      leave<NG, NB>(st, wide ? 1.0f : 0x1p24f, wide ? 1.0f : 0x1p20f, (float*)ring, ml);
+      leave<NG, NB>(st, wide, (float*)ring, ml);
       break;
     }
     __syncthreads();

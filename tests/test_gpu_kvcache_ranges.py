@@ -3,9 +3,10 @@ each other, seen, hidden and of no weight; against 64 bits.
 
 The bound is per key, so that a key of no weight allows no error. With p the probabilities and a stored number's parts
 (code + 8) step + |offset - 8 step|, an output is off by at most
-    sum p (2^-9 + 2 e + 2 sum p e) parts(v) + 2^-8 |o|,    e = 2^-19 |scale| sum |q| parts(k) + 2^-18:
+    sum p 2^-9 parts(v) + sum p 2 e |v - o| + 2^-8 |o|,    e = 2^-19 |scale| sum |q| parts(k) + 2^-18:
 2^-9 for four roundings of 2^-11 (of a probability, of a value, and of both where they are small beside the largest),
-e for a score's f32 sums and its exponential, 2^-8 for the output's own rounding to bf16."""
+e for a score's f32 sums and its exponential (a score that is off by d moves p to p (1 + d), and o by p d (v - o); twice
+that, for the terms of second order), 2^-8 for the output's own rounding to bf16."""
 import numpy as np
 import pytest
 
@@ -36,11 +37,11 @@ def _bound(q, ref, pages, q_len, n, scale, causal):
             p = np.exp(x - x.max(-1, keepdims=True))
             p /= p.sum(-1, keepdims=True)
             e = 2.0 ** -19 * abs(scale) * (np.abs(qd) @ ka[:seen].T) + 2.0 ** -18
-            with np.errstate(over="ignore", invalid="ignore"):
-                pe = np.where(p > 0, p * e, 0.0)
             o[t, rows] = p @ v[:seen]
-            tol[t, rows] = (2.0 ** -9 * p + 2 * pe + 2 * p * pe.sum(-1, keepdims=True)) @ va[:seen] \
-                + 2.0 ** -8 * np.abs(o[t, rows])
+            tol[t, rows] = 2.0 ** -9 * (p @ va[:seen]) + 2.0 ** -8 * np.abs(o[t, rows])
+            for r, (pr, er) in enumerate(zip(p, e)):
+                of = pr > 1e-30
+                tol[t, h * group + r] += 2 * (pr[of] * er[of]) @ np.abs(v[:seen][of] - o[t, h * group + r])
     return o, tol
 
 
@@ -211,3 +212,43 @@ def test_a_long_flat_tail_behind_one_heavy_key(b200, D, bits, sink, T, wide):
     k[0] = bits * np.log(2) / D ** 0.5  # times ones
     v[0] = rng.standard_normal((1, D)) * sink
     _check(b200, np.ones((T, 2, D), F), k, v, D, 2, wide=wide, page=64)
+
+
+# ---- scores far from zero ----
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("power", [-100, 0, 10, 24, 40, 97])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("size", [-30, 0, 60])
+@pytest.mark.parametrize("T,wide", KINDS[:2])
+def test_equal_keys_of_any_size(b200, D, power, sign, size, T, wide):
+    """Keys that are all the same: the mean of the values that a row sees, however far the scores are from zero."""
+    rng = np.random.default_rng(9)
+    n, group = T + 30, 4
+    k = np.full((n, 1, D), np.ldexp(sign * 3.0, power), F)
+    v = np.ldexp(rng.standard_normal((n, 1, D)) + 1, size).astype(F)
+    q = _aimed(rng, T, group, D)
+    cache, ref = fb.PagedCache(b200, 8, 32, 1, D), R.Cache(8, 32, 1, D)
+    b200.cache_append(cache, _up(b200, k, "f32"), _up(b200, v, "f32"), _up(b200, np.arange(n), "i32"))
+    ref.append(k, v, np.arange(n))
+    table = np.full((1, WIDE // 32 if wide else 8), -1)
+    table[0, :8] = np.arange(8)
+    got = _down(b200.cache_attention(_up(b200, q, "bf16"), cache, _up(b200, table, "i32"), _up(b200, [0, T], "i32"),
+                                     _up(b200, [n], "i32"), group), q.shape).astype(np.float64)
+    b200.sync()
+    V, A = (x.reshape(-1, D)[:n] for x in (ref.values("v")[:, 0], ref.parts("v")[:, 0]))
+    for t in range(T):
+        seen = n - T + t + 1
+        want, tol = V[:seen].mean(0), (2.0 ** -9 + 2.0 ** -18) * A[:seen].mean(0)
+        assert np.all(np.abs(got[t] - want) <= tol + 2.0 ** -8 * np.abs(want)), (t, np.abs(got[t] - want).max())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("power", [10, 20, 24, 40, 97])
+@pytest.mark.parametrize("size", [-30, 0, 60])
+@pytest.mark.parametrize("T,wide", KINDS[:2])
+def test_ordinary_keys_behind_ones_far_below(b200, D, power, size, T, wide):
+    """Runs that begin with keys of no weight whose scores are far below all others'."""
+    rng = np.random.default_rng(10)
+    k, v = _plain(rng, 700, 1, D)
+    k[:100], k[300:400] = -np.ldexp(3.0, power), -np.ldexp(5.0, power)
+    _check(b200, _aimed(rng, T, 4, D), k, np.ldexp(v, size), D, 4, wide=wide)
