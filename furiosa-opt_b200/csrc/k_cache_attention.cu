@@ -404,7 +404,8 @@ __device__ __forceinline__ void values(const uint8_t* stage, const Places& at, i
         // The base moves to the largest score, if that lies far above it; the first tile's scores set it. From the scores
         // themselves, rounded alike: relative to a base far away they have lost bits.
         const float scale = q.scale[nb][c];
-        const float x0 = x[nb][c] == -INFINITY ? -INFINITY : raw[nb][c] * scale, x1 = x[nb][c + 2] == -INFINITY ? -INFINITY : raw[nb][c + 2] * scale;
+        const float x0 = x[nb][c] == -INFINITY ? -INFINITY : __fmul_rn(raw[nb][c], scale);
+        const float x1 = x[nb][c + 2] == -INFINITY ? -INFINITY : __fmul_rn(raw[nb][c + 2], scale);
         const float top = max_over_g(fmaxf(x0, x1)), was = s.m[nb][c];
         const float m = first ? (top == -INFINITY ? 0.0f : top) : top - was > kLazy ? top : was;
         const float f = first ? 0.0f : exp2_(was - m), fo = f * fall;

@@ -59,6 +59,7 @@ constexpr int kUncut = 8;                // segments of fewer tiles are not shar
 constexpr float kNominal = 10.0f, kMostP = 15.0f;
 constexpr int kEven = 6;                  // log2 by which 32 tokens' sizes may differ under one scale
 constexpr float kLazySum = 20.0f;         // ... and a score that of l, where it is looked at
+constexpr float kFarScore = 0x1p22f;      // up to which bases and V's exponents add up exactly
 constexpr float kFarBack = 80.0f;         // log2 up to which P gives its share of l: probabilities below 2^-46 may vanish
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -285,52 +286,76 @@ __device__ __forceinline__ Exponents exponents(const uint32_t* scales, int none)
 // -inf is multiplied as well.
 __device__ __forceinline__ float score_factor(float row, float keys) { return fmaxf(row * keys, 0x1p-126f); }
 
-// The softmax of tiles whose tokens have exponents of their own, 32 at a time: the scores in s and the ev in v. By themselves,
-// so that the roles' code beside them stays as it is (within rows_kernel they cost 15 us of 142, called for or not).
-__device__ __forceinline__ void own_scores(uint32_t columns, int left, float qs, const int8_t* k, const int8_t* v_own, float* s, float* v) {
-  tld32(columns, (uint32_t*)s);
-  tld_wait_regs((uint32_t*)s);
-  hide((uint32_t*)s, left);
+// A finite score's: an infinite one's row is NaN anyway.
+__device__ __forceinline__ bool far_score(float base) { return fabsf(base) > kFarScore && fabsf(base) < INFINITY; }
+
+// A row's bases: of l, and of O relative to it, so that a score far from zero takes nothing from V's exponents.
+struct Bases {
+  float l, o;
+};
+// The softmax of one tile by itself, 32 keys at a time, for tiles whose tokens have exponents of their own (k_own, v_own),
+// and where one exponential does not serve both P and l or scores are too far from zero for the sums of bases that
+// rows_kernel makes. Apart from it, so that the roles' code beside it stays as it is (within rows_kernel this cost
+// 15 us of 142, called for or not). P goes over the scores; returns l, and moves the bases.
+__device__ __noinline__ float own_tile(uint32_t scores, int keys, uint32_t outputs, int channels, int left, float qs, const int8_t* k_own,
+                                       const int8_t* v_own, bool first, float l, Bases& base) {
+  auto load = [&](int c, float* s) {
+    tld32(scores + 32 * c, (uint32_t*)s);
+    tld_wait_regs((uint32_t*)s);
+    hide((uint32_t*)s, left - 32 * c);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    s[i] *= score_factor(qs, power(k[i]));
-    v[i] = (float)v_own[i];
-  }
-}
-// The largest x.
-__device__ __noinline__ float own_top(uint32_t columns, int left, float qs, const int8_t* k, const int8_t* v_own, int quarters) {
-  float top = -INFINITY;
+    for (int i = 0; i < 32; ++i) s[i] = __fmul_rn(s[i], score_factor(qs, power(k_own[32 * c + i])));  // rounded as the base is
+  };
+  float most = -INFINITY;
 #pragma unroll 1
-  for (int c = 0; c < quarters; ++c) {
-    float s[32], v[32];
-    own_scores(columns + 32 * c, left - 32 * c, qs, k + 32 * c, v_own + 32 * c, s, v);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i] + v[i]);
-  }
-  return top;
-}
-// P in place of the scores, and (l, ml) with the tile's share: the base of l moves where scores rise far above it.
-__device__ __noinline__ float2 own_weights(uint32_t columns, int left, float qs, const int8_t* k, const int8_t* v_own, int quarters, float m, float l, float ml) {
-#pragma unroll 1
-  for (int c = 0; c < quarters; ++c) {
-    float s[32], v[32];
-    uint32_t p[16];
-    own_scores(columns + 32 * c, left - 32 * c, qs, k + 32 * c, v_own + 32 * c, s, v);
-    float most = -INFINITY;
+  for (int c = 0; c < keys / 32; ++c) {
+    float s[32];
+    load(c, s);
 #pragma unroll
     for (int i = 0; i < 32; ++i) most = fmaxf(most, s[i]);
-    if (most > ml + kLazySum) {
-      l *= exp2_(ml - most);
-      ml = most;
+  }
+  if (first) base = {most == -INFINITY ? 0.0f : rintf(most), 0.0f};
+  else if (most > base.l + kLazySum) {
+    const float up = rintf(most) - base.l;
+    l *= exp2_(-up);
+    base = {rintf(most), base.o - up};
+  }
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < keys / 32; ++c) {
+    float s[32];
+    load(c, s);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i] - base.l + (float)v_own[32 * c + i]);
+  }
+  const float was = base.o;
+  if (first ? top != -INFINITY : top > was + kMostP) base.o = rintf(top) - kNominal;
+  if (__any_sync(0xffffffffu, !first && base.o != was)) {
+    const float f = exp2_(was - base.o);
+#pragma unroll 1
+    for (int c = 0; c < channels / 32; ++c) {
+      float o[32];
+      tld32(outputs + 32 * c, (uint32_t*)o);
+      tld_wait_regs((uint32_t*)o);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] *= f;
+      tst32(outputs + 32 * c, (const uint32_t*)o);
     }
+  }
+#pragma unroll 1
+  for (int c = 0; c < keys / 32; ++c) {
+    float s[32];
+    uint32_t p[16];
+    load(c, s);
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
-      l += exp2_(s[i] - ml) + exp2_(s[i + 1] - ml);
-      p[i >> 1] = f16x2(exp2_(s[i] + v[i] - m), exp2_(s[i + 1] + v[i + 1] - m));
+      const float x0 = s[i] - base.l, x1 = s[i + 1] - base.l;
+      l += exp2_(x0) + exp2_(x1);
+      p[i >> 1] = f16x2(exp2_(x0 + ((float)v_own[32 * c + i] - base.o)), exp2_(x1 + ((float)v_own[32 * c + i + 1] - base.o)));
     }
-    tst16(columns + 16 * c, p);
+    tst16(scores + 16 * c, p);
   }
-  return make_float2(l, ml);
+  return l;
 }
 
 template <int NG>
@@ -665,7 +690,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
     };
     bool ok = true;
     Item done;  // the segment whose output is still in O_t
-    float qs = 0.0f, m = 0.0f, l = 0.0f, ml = 0.0f;  // ml: the base of l
+    float qs = 0.0f, l = 0.0f;
+    Bases bases{0.0f, 0.0f};
     int n = 0;
     // Each part stands here once, in one place: the roles' code together has to stay in the instruction cache.
     for (int seg = 0; more || seg; ++seg) {
@@ -695,8 +721,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) ((float4*)part)[(8 * c + i) * 128 + r] = *(float4*)(o + 4 * i);
           }
-          part[D * 128 + r] = l == 0.0f ? kNone : m;  // a NaN sum stays one
-          part[D * 128 + 128 + r] = l == 0.0f ? kNone : ml;
+          part[D * 128 + r] = l == 0.0f ? kNone : bases.l;  // a NaN sum stays one
+          part[D * 128 + 128 + r] = bases.o;
           part[D * 128 + 256 + r] = l;
           c0 = shares.owner(done.at + kCost);
           c1 = shares.owner(done.at + done.tiles + kCost - 1);
@@ -712,18 +738,16 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
           output = last[t];
           if (!(ok = meet())) break;  // last[t] has been read
           if (output) {  // the parts' sum goes into O_t
-            m = ml = kNone;
+            bases = {kNone, 2.0f * kNone};
             l = 0.0f;
+#pragma unroll 4
+            for (int c = c0; c <= c1; ++c) bases.l = fmaxf(bases.l, __ldcg(slot(c, c == c0) + D * 128 + r));
 #pragma unroll 4
             for (int c = c0; c <= c1; ++c) {
               const float* q = slot(c, c == c0) + D * 128 + r;
-              m = fmaxf(m, __ldcg(q));
-              ml = fmaxf(ml, __ldcg(q + 128));
-            }
-#pragma unroll 4
-            for (int c = c0; c <= c1; ++c) {
-              const float* q = slot(c, c == c0) + D * 128 + 128 + r;
-              l = fmaf(exp2_(__ldcg(q) - ml), __ldcg(q + 128), l);
+              const float up = __ldcg(q) - bases.l;
+              l = fmaf(exp2_(up), __ldcg(q + 256), l);
+              bases.o = fmaxf(bases.o, up + __ldcg(q + 128));
             }
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -733,7 +757,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
 #pragma unroll 2
               for (int b = c0; b <= c1; ++b) {
                 const float* q = slot(b, b == c0);
-                const float f = exp2_(__ldcg(q + D * 128 + r) - m);
+                const float f = exp2_(__ldcg(q + D * 128 + r) - bases.l + __ldcg(q + D * 128 + 128 + r) - bases.o);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                   const float4 v = __ldcg((const float4*)q + (8 * c + i) * 128 + r);
@@ -747,8 +771,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
           }
         }
         if (output) {
-          // 2^(m - ml) / l, which may lie outside f32 where the outputs do not: then a part of it goes in ahead
-          float lift = m - ml;
+          // 2^lift / l, which may lie outside f32 where the outputs do not: then a part of it goes in ahead
+          float lift = bases.o;
           if (__any_sync(0xffffffffu, lift < -90.0f)) {
             scale_outputs(lift < -90.0f ? 0x1p-64f : 1.0f);
             if (lift < -90.0f) lift += 64.0f;
@@ -788,7 +812,8 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
       more = walk.next(it);  // while the first scores are on their way
       const int row = done.row0 + t * 128 + r;
       const int limit = row < done.s.rows ? seen(a, done.s, row) : done.s.keys;  // rows past the last are not stored
-      m = l = ml = 0.0f;
+      l = 0.0f;
+      bases = {0.0f, 0.0f};
       for (int kt = done.t0; kt < done.t1; ++kt, ++n) {
         ok = mbar_wait(smem_u32(&x_full[n & 3]), (n >> 2) & 1, abort_flag, a.err, 421) &&
              mbar_wait(smem_u32(&s_full[t]), n & 1, abort_flag, a.err, 422);
@@ -803,7 +828,6 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
         float top = -INFINITY, least = INFINITY;  // least: the smallest ev
         const int8_t *ko = k_own + (n & 3) * T::kKeys, *vo = v_own + (n & 3) * T::kKeys;
         const bool uneven = apart[n & 3] != 0;
-        if (uneven) top = own_top(tS, left, qs, ko, vo, T::kQuarters);
 #pragma unroll 1
         for (int h = 0; !uneven && h < T::kKeys / 64; ++h) {  // two loads at a time on their way
           uint32_t s[64];
@@ -829,27 +853,30 @@ __global__ void __launch_bounds__(kRowThreads, 1) rows_kernel(AttnArgs a) {
             least = fminf(least, vu[2 * h + c]);
           }
         }
-        const float base = first ? (top == -INFINITY ? 0.0f : top - kNominal) : top > m + kMostP ? top - kNominal : m;
+        // The bases are whole numbers, which makes the sums of them and V's exponents exact, up to kFarScore.
+        const float was = bases.l + bases.o;
+        const float m = first ? (top == -INFINITY ? 0.0f : rintf(top) - kNominal) : top > was + kMostP ? rintf(top) - kNominal : was;
+        float ml = bases.l;
         if (first) {  // not above the largest score
           float largest = vu[0];
 #pragma unroll
           for (int i = 1; i < T::kQuarters; ++i) largest = fmaxf(largest, vu[i]);
-          ml = base - largest;
+          ml = m - largest;
         }
         // Where V is far smaller than what set the base, or scores have risen far above l's, P has lost bits that l needs
-        // (or l would pass f32's range): the two part.
-        bool far = uneven || base - least - ml > kFarBack;
-        if (__any_sync(0xffffffffu, far || (!first && base != m))) {
-          // S_t was issued behind the last O_t += P_t V: it is complete
-          if (!first) scale_outputs(exp2_(m - base));
+        // (or l would pass f32's range).
+        bool far = uneven || m - least - ml > kFarBack || far_score(m) || far_score(ml);
+        if (__any_sync(0xffffffffu, far || (!first && m != was))) {
           far = __any_sync(0xffffffffu, far);
+          // S_t was issued behind the last O_t += P_t V: it is complete
+          if (!far && !first) scale_outputs(exp2_(was - m));
         }
-        m = base;
         if (far) {
-          const float2 sum = own_weights(tS, left, qs, ko, vo, T::kQuarters, m, l, ml);
-          l = sum.x;
-          ml = sum.y;
+          Bases moved = bases;
+          l = own_tile(tS, T::kKeys, tO, D, left, qs, ko, vo, first, l, moved);
+          bases = moved;
         } else {
+          bases = {ml, m - ml};
 #pragma unroll 1
           for (int h = 0; h < T::kKeys / 64; ++h) {  // P goes over columns whose scores have been read: 16 c .. 16 c + 15
             uint32_t s[64];
