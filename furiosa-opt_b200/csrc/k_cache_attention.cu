@@ -9,10 +9,11 @@
 // tokens_kernel: the products are mma.sync m16n8k16 (f16 in, f32 sums) with the TOKENS as the 16 rows and 8
 // query rows (the query heads of one key head, of one or more tokens) as the 8 columns. A single token's
 // queries fill 4 to 8 of 128 rows of a tcgen05 tile and would need the codes expanded through shared memory;
-// here a lane turns the words that it loaded into fragments in registers. What bounds it is the issue slots of 12
-// warps an SM (168 registers a thread), then the cache's bytes: 86 us for one token of each of 64 sequences of 64
-// to 8192 keys, 8 key heads of 128 and 4 query heads to each, which is 3.6 TB/s of codes and scales, 0.56 of a copy's
-// rate; 75 us for two tokens at 131072 and 100003 keys. 16 warps at 128 registers spill (95 us for the first).
+// here a lane turns the words that it loaded into fragments in registers. What bounds it are chains of dependent
+// instructions at 12 warps an SM (168 registers a thread): 57 % of the issue slots and 0.53 of a copy's rate are used,
+// and the first stall is an instruction's own latency. 90 us for one token of each of 64 sequences of 64 to 8192 keys, 8 key
+// heads of 128 and 4 query heads to each (3.5 TB/s of codes and scales); 77 us for two tokens at 131072 and 100003
+// keys. 16 warps at 128 registers spill (95 us for the first, where 12 took 86).
 //   * K operand: lane (g, i) = (lane / 4, lane % 4) takes the 16-byte (D = 128) run of token g that the
 //     layout [D % 32 / 8, D / 32, D % 8] puts at i: word j is 8 channels of group j, which make its operand
 //     registers of two k16 steps; q's fragments are permuted to match. (x & 0x000f000f) ^ 0x00080008 is a
@@ -28,7 +29,8 @@
 //     Its lower end is looked at behind the last key: a product p step is off by 2^-11 of itself or by 2^-25 at most,
 //     so a run of n keys is right to 2^-10 of the sum of its products if that sum is 2^-14 n at least. Where one is
 //     not (a group whose steps are far below another's, or whose tokens of weight have steps far below those of
-//     tokens without), the warp takes its run once more, with products in f32.
+//     tokens without), the warp takes its run once more, with products in f32 (a call takes five times as long where every
+//     run is).
 // Four warps take a run of 16-token tiles each, with their own rings of cp.async stages (no block barrier
 // while keys stream), and merge their (maximum, sum, output) at the end of a segment.
 //
@@ -48,7 +50,7 @@ constexpr int tokens_blocks() { return NG <= 4 && NB == 1 ? kBlocks : 2; }
 constexpr int kSegmentCost = 4;  // beginning and ending a segment takes about as long as this many tiles
 constexpr int kLeast = 2;        // tiles of a share
 // A part more to add up takes about a sixth of a tile. Shares of 2 tiles were best at 777 tokens of 8 heads
-// (12.4 us; 14.0 with 4), of 8 at 15179 of two heads (20.6; 29.3 with 2), of 8 to 16 at 131072 of one (24.8; 26.8 with 5).
+// (12.4 us; 14.0 with 4), of 8 at 15179 of two heads (20.6; 29.3 with 2), of 8 to 16 at 131072 of one (2 us less than with 5).
 constexpr float kByRoot = 0.4f;
 constexpr int kStages = 4;
 constexpr float kLazy = 6.0f;    // log2 by which a score may exceed the running maximum before it moves
@@ -772,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, tokens_blocks<NG, NB>()) tokens_kern
       if (last) {
         // Each part's weight of each row first, by all threads at once; then the sums over the parts, with the parts
         // of a column divided between threads where there are more threads than columns. (One token at 131072 keys
-        // of one head: 27 us; 68 with every thread looking at all maxima by itself.)
+        // of one head: 29 us; 68 with every thread looking at all maxima by itself.)
         const int parts = c1 - c0 + 1, mr = lane % R;
         constexpr int kEach = 32 / R, kStep = kWarps * kEach;
         const int from = c0 + warp * kEach + lane / R;
@@ -908,9 +910,9 @@ extern "C" fopt_status fopt_cache_attention(fopt_ctx* ctx, void* o, const void* 
     // A call that leaves most of the device to tokens_kernel's blocks is its own as well, for rows_kernel's few blocks
     // take longer to begin, to end and over each segment. What each block would have at most, in tiles of 64 keys, decides,
     // from the table's width; the more keys, the more rows_kernel's parts cost. At 8 key heads of 128 and 4 query heads
-    // to each (us, rows_kernel / tokens_kernel): 40 queries at 512 keys 26.7 / 18.5 (4 tiles a block), 106 at 2048
-    // 41.2 / 41.0 (26), 200 at 512 28.7 / 28.8 (16), 400 at 512 28.8 / 41.1 (32); of one head 400 at 2048 42.4 / 26.7
-    // (12), 512 at 8192 61.4 / 71.7 (57), 256 60.3 / 46.6 (29), 16 of 8 query heads at 131072 160 / 80 (55).
+    // to each (us, rows_kernel / tokens_kernel): 40 queries at 512 keys 27.4 / 18.6 (4 tiles a block), 106 at 2048
+    // 43.3 / 43.7 (26), 200 at 512 29.7 / 32.0 (16), 400 at 512 30.9 / 46.7 (32); of one head 400 at 2048 44.0 / 28.8
+    // (12), 512 at 8192 65.8 / 76.7 (57), 256 64.5 / 49.3 (29), 16 of 8 query heads at 131072 177 / 85 (55).
     const int64_t width = (int64_t)table_width * cache->page_size;
     const int64_t segments = ((int64_t)tokens * a.group / (two ? 16 : 8) + batch) * cache->heads;
     const double tiles = (double)segments * (double)(width / kv::kTileTokens + 1 + kv::kSegmentCost) / (sms * (two ? 2 : kv::kBlocks));

@@ -32,10 +32,11 @@
 // queries are stored in the same order, for V the output's columns are put right when they leave.
 //
 // What bounds it: the tensor cores take 34 steps of M 128, N 128, K 16 per key tile (about 3300 cycles, 1.75 us); the
-// exponentials take 2048, the expansion about 450 issue slots of each scheduler. A period is 3.0 us, since each of the
-// two tiles takes 1.9 us of softmax and then waits for 0.9 us of products: 138 us for 4 pieces of 512 tokens at 512 to
-// 4096 keys, 8 key heads of 128 and 4 query heads to each (0.56 PFLOP/s), 73 us for 8 prompts of 512, where 5.5 us
-// around the 1 to 4 periods of a segment go into its queries, first scores and output.
+// exponentials take 2048, the expansion about 450 issue slots of each scheduler. A period is 3.2 us, since each of the
+// two tiles takes about 2 us of softmax and then waits for 0.9 us of products: 150 us for 4 pieces of 512 tokens at 512
+// to 4096 keys, 8 key heads of 128 and 4 query heads to each (0.52 PFLOP/s), 81 us for 8 prompts of 512, where 5.5 us
+// around the 1 to 4 periods of a segment go into its queries, first scores and output. Tiles whose tokens have exponents of
+// their own take three times as long (431 us for the pieces if all had).
 #include "cache_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -51,7 +52,7 @@ constexpr int kOffsets = 128 * 32;        // 128 rows of 16 f16: the sums of a t
 constexpr int kCost = 2;                 // key tiles that beginning and ending a segment takes as long as
 constexpr int kLeast = 4;                // units of a share
 // A part more to add up (66 KB for each of two tiles, by one SM) takes about as long as a unit. Of 16 tokens at 131072
-// keys of one head of 8 query heads: 159 us; 347 without this rule, in shares of 7 units.
+// keys of one head of 8 query heads: 177 us; 347 without this rule, in shares of 7 units (159 with it then).
 constexpr float kByRoot = 1.0f;
 constexpr int kUncut = 8;                // segments of fewer tiles are not shared between blocks
 // log2 of the largest P as the base is set, and up to which it may grow before the base moves. (On the cases above
@@ -65,7 +66,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 // At D = 256 one 128-row tile of queries and 64 keys at a time are what tensor memory (64 columns of scores, 256 of
 // outputs) and shared memory hold; products and softmax take turns. 512 queries at 2382 keys and 370 at 370, 3 key
-// heads and 5 query heads to each: 79 us (203 by tokens_kernel).
+// heads and 5 query heads to each: 84 us (210 by tokens_kernel).
 template <int NG>
 struct Tiles {
   static constexpr int D = NG * kGroup, kHalves = D / 64;
@@ -935,7 +936,7 @@ void launch_rows(fopt_ctx* ctx, const AttnArgs& a, int head_dim, int sms) {
   auto go = [&](auto kernel, int smem) {
     allow_shared(ctx, done[head_dim / 128], (const void*)kernel, smem);
     // Beside tokens_kernel and not behind it: a batch of both kinds (6 sequences, 1999 keys the longest, 7 query heads
-    // to a key head of 64) takes 32 us instead of 43, and where there are prompts alone tokens_kernel's empty launch
+    // to a key head of 64) takes 34 us instead of 44, and where there are prompts alone tokens_kernel's empty launch
     // is hidden.
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;

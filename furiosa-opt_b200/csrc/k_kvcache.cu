@@ -10,9 +10,10 @@
 // code = rint((x - z) / s) in [-8, 7], the quotient rounded as IEEE division rounds it: bf16 inputs make exact halves
 // common, and those must go to even rather than to where a reciprocal's error sends them.
 //
-// What bounds them: the rotation memory (12.4 us for 4096 tokens of 32 heads of 128 in bf16, 67 MB: 5.4 TB/s), the
-// append instructions (15.4 us for 4096 tokens of 8 heads of 128, 21 MB, where memory would take 3.3), the read the
-// stores of its half-filled lines (10.4 us for 4608 such slots), single tokens the launch (4.3 us each).
+// What bounds them, on inputs that come from HBM: the rotation memory (16.3 us for 4096 tokens of 32 heads of 128 in
+// bf16, 67 MB: 4.1 TB/s, 0.63 of a copy's rate; 12.4 us where L2 still holds them), the append instructions (16.4 us for
+// 4096 tokens of 8 heads of 128, 21 MB, where memory would take 3.3; 14.6 from L2), the read the values' stores, which
+// fill half a line each (12.3 us for 4608 such slots; 10.3 from L2), single tokens the launch (4.3 us each).
 #include "kvcache.cuh"
 
 namespace fopt {
@@ -111,7 +112,7 @@ struct Raw {
 
 // (cos, sin) of the first `n` tokens' pairs, from their positions, into shared memory: [token][pair], or, for threads
 // that take 2^shift neighbouring pairs each, [token][two of a thread's pairs][thread][pair of the two], since lanes
-// that read 64 bytes apart share banks (which made the rotation of 4096 tokens of 32 heads of 128 take 16.5 us, not 12.4).
+// that read 64 bytes apart share banks (which made the rotation of 4096 tokens of 32 heads of 128 take 16.5 us, not 12.4, from L2).
 __device__ __forceinline__ void angles(float2* cs, const Rope& r, const int32_t* positions, int n, int shift) {
   // by a plain address: lanes that differ in it take turns at the constant bank
   const unsigned long long* turn = r.turn;
@@ -155,7 +156,7 @@ struct RotaryArgs {
 // A block has `each` tokens. With vectors their units are one range, of which a thread has AHEAD at a time, a block's
 // threads apart, on their way while the angles are computed (the sines take about as long as the loads). Without,
 // most time goes into addresses, so a thread takes the same unit of kOnes tokens: 5878 tokens of 21 heads of 96 with
-// 35 pairs in bf16 take 22.7 us, bound by instructions (45 as one range, 35 token after token).
+// 35 pairs in bf16 take 22.7 us, bound by instructions (from L2; 45 as one range, 35 token after token).
 constexpr int kOnes = 4;
 template <bool F32, bool VEC, int AHEAD>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, const __grid_constant__ Rope r) {
@@ -320,7 +321,7 @@ struct Steps {
 // g * (NG / 2) + j of a value is channels 4 g .. + 3 of groups 2 j and 2 j + 1; a thread has 8 neighbouring channels
 // of both, and their four threads lie NG / 2 apart. Extremes cross by shuffles. Instructions bound this kernel on
 // prompts; shuffles, scales and addresses are a large part of them, so a thread has as many values as that allows:
-// 15.4 us for 4096 tokens of 8 heads of 128 in bf16, where a thread per word with the tokens of its block one after
+// 14.6 us for 4096 tokens of 8 heads of 128 in bf16 from L2, where a thread per word with the tokens of its block one after
 // the other took 18 us, and all groups' channels to four and eight threads a row, with a division a value, 27 us.
 template <bool F32, int NG>
 __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, const __grid_constant__ Rope r) {
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, const __
 
 // ---- read ----
 // A thread per word, as they are stored: 8 neighbouring channels of a key, or 4 of each of two groups of a value.
-// Slots and heads are one range, so that few heads fill blocks too. (10.4 us for 4608 slots of 8 heads of 128 to
+// Slots and heads are one range, so that few heads fill blocks too. (10.3 us for 4608 slots of 8 heads of 128 from L2 to
 // bf16, with one, two, four or eight words of a thread on their way.)
 template <bool F32, int NG>
 __global__ void __launch_bounds__(kThreads) read_kernel(Cache cache, void* out_k, void* out_v, const int32_t* slots,
@@ -549,7 +550,7 @@ void launch_append(fopt_ctx* ctx, AppendArgs a, const Rope& r, int dim) {
 template <bool F32, bool VEC>
 void launch_rotary(fopt_ctx* ctx, RotaryArgs a, const Rope& r) {
   constexpr int kAhead = 2;
-  // tokens enough to occupy a block's threads kAhead times over (12 us for 14598 tokens of 3 heads of 128 in bf16,
+  // tokens enough to occupy a block's threads kAhead times over (12 us for 14598 tokens of 3 heads of 128 in bf16 from L2,
   // against 19 with two tokens a block), but not so many that SMs go without
   const int64_t per_token = (int64_t)a.heads * a.units, sms = sm_count(ctx);
   const int64_t fill = VEC ? std::min<int64_t>(kThreads * kAhead / per_token, 2048 / r.pairs) : kOnes;

@@ -252,7 +252,8 @@ class DecoderBlockW8A8:
         """The block over the new tokens of a batch of cached sequences (whole prompts, pieces of them or
         single tokens, mixed): queries and keys rotated by their positions, keys and values appended to
         the cache, attention over all that it then holds. x: bf16 [T, H], batch.tokens = T rows of which
-        those behind the last sequence are padding (their output means nothing)."""
+        those behind the last sequence are padding (their output means nothing). Pad to a multiple of 128
+        rows: the projections then are tensor-core GEMMs."""
         if cache.heads != self.Hkv or cache.head_dim != 128 or batch.tokens != self.T:
             raise ValueError("step: the cache or the batch is not of this block's shape")
 
