@@ -19,14 +19,16 @@
 // share of a score, sum_groups offset (sum of q), is one more step of the same product, over k = (part, group) with
 // the sums of q in two f16 parts.
 //
-// f16 holds 11 bits of a value where bf16 would hold 8, but not every size of it: every 32
-// tokens' K is scaled by a power of two and V by another, so that the largest is in [2^4, 2^9); where tokens are more
-// than 2^6 apart, each by its own, so that a large one, hidden or of no weight, takes nothing from its neighbours. K's
-// comes back with the scores. V's, 2^ev, goes into the exponent: with x = score + ev, P = 2^(x - m) and O = sum P V 2^-ev,
-// where the base m follows the largest x, which P brings to 2^10 at least: f16 holds 24 bits below that, so tokens of
-// little weight count, a hundred thousand of them too. What one scale has to hold are the groups of 32 channels of one
-// token: 2^-18 of the largest and less loses bits. The sum of probabilities has a base of its own, a score n near the largest: l = sum P
-// 2^(m - ev - n), so that V's size takes nothing from its range; outputs are O / l 2^(m - n).
+// f16 holds 11 bits of a value where bf16 would hold 8, but not every size of it: every 32 tokens' K is scaled by a
+// power of two and V by another, so that the largest is in [2^4, 2^9); where tokens are more than 2^6 apart, each by
+// its own, so that a large one, hidden or of no weight, takes nothing from its neighbours. K's comes back with the
+// scores. V's, 2^ev, goes into the exponent: with x = score + ev, P = 2^(x - m) and O = sum P V 2^-ev, where the base m
+// follows the largest x, which P brings to 2^10 at least: f16 holds 24 bits below that, so tokens of little weight
+// count, a hundred thousand of them too. What one scale has to hold are the groups of 32 channels of one token: 2^-18
+// of the largest and less loses bits.
+//
+// The sum of probabilities has a base of its own, a score n near the largest: l = sum P 2^(m - ev - n), so that V's
+// size takes nothing from its range; outputs are O / l 2^(m - n).
 //
 // A 16-byte chunk holds 8 codes in the order that pairs come out of a word (0, 4, 1, 5, 2, 6, 3, 7): for K the
 // queries are stored in the same order, for V the output's columns are put right when they leave.
@@ -35,8 +37,8 @@
 // exponentials take 2048, the expansion about 450 issue slots of each scheduler. A period is 3.2 us, since each of the
 // two tiles takes about 2 us of softmax and then waits for 0.9 us of products: 150 us for 4 pieces of 512 tokens at 512
 // to 4096 keys, 8 key heads of 128 and 4 query heads to each (0.52 PFLOP/s), 81 us for 8 prompts of 512, where 5.5 us
-// around the 1 to 4 periods of a segment go into its queries, first scores and output. Tiles whose tokens have exponents of
-// their own take three times as long (431 us for the pieces if all had).
+// around the 1 to 4 periods of a segment go into its queries, first scores and output. Tiles whose tokens have
+// exponents of their own take three times as long (431 us for the pieces if all had).
 #include "cache_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -281,7 +283,6 @@ __device__ __forceinline__ Exponents exponents(const uint32_t* scales, int none)
   e.own = e.apart ? exponent(size ? size : least) : e.all;
   return e;
 }
-
 
 // A tile's scores are the products times the row's factor and the keys' power of two: together not 0, for a hidden key's
 // -inf is multiplied as well.
