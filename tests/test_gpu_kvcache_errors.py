@@ -2,6 +2,7 @@
 write it, and arrivals are left in a workspace as a kernel that gave up would leave them; no wait runs out."""
 import ctypes as C
 import os
+import shutil
 import subprocess
 
 import numpy as np
@@ -27,7 +28,8 @@ def inside(tmp_path_factory):
     d = tmp_path_factory.mktemp("inside")
     (d / "inside.cu").write_text(SOURCE)
     csrc = os.path.join(os.path.dirname(HERE), "furiosa-opt_b200", "csrc")
-    subprocess.run(["nvcc", "-std=c++17", "-arch=sm_100a", "-shared", "-Xcompiler", "-fPIC", "-I", csrc, "-o", str(d / "inside.so"),
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    subprocess.run([nvcc, "-std=c++17", "-arch=sm_100a", "-shared", "-Xcompiler", "-fPIC", "-I", csrc, "-o", str(d / "inside.so"),
                     str(d / "inside.cu")], check=True)
     lib = C.CDLL(str(d / "inside.so"))
     for f in (lib.expired, lib.workspace):
